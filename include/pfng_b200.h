@@ -5,7 +5,9 @@
  *     C[m][n] = A_act[m][k] . W[n][k]^T
  * for the weight/activation pairs q4_0 x q8_0, q4_K x q8_K and
  * iq2_xxs x q8_K, plus the fp32 -> q8_0 / q8_K activation quantizers that
- * feed it and the fp32 -> q4_0 / q4_K weight quantizers that produce W.
+ * feed it and the fp32 -> q4_0 / q4_K weight quantizers that produce W; and
+ * the attention step between two such products over a key/value cache held in
+ * q4_0 (last section).
  *
  * All buffers are DEVICE pointers in the unmodified ggml block layouts of the
  * reference (include/ggml.h:125-159):
@@ -332,6 +334,105 @@ int pfng_b200_ipc_close(void *ptr);
 #define PFNG_B200_NOALLOC_SCRATCH_BYTES ((size_t)16 << 20)
 int pfng_b200_compute_q4_0_noalloc(const void *w, const float *x, int64_t ldx, float *c, int64_t m, int64_t n,
                                    int64_t k, int64_t ldc, void *stream);
+
+/* ---- the attention step over a q4_0 key/value cache -------------------------
+ * What stands between a layer's Q/K/V projection and its output projection,
+ * on a cache held in the library's 4-bit type: kv_plan (once per step), then
+ * per layer qk_norm_rope, kv_append_q4_0 and attention_q4_0.  No counterpart
+ * in the reference, which ends at the matmul.
+ *
+ * The cache: K and V are one buffer each, 16-byte aligned, of
+ * pfng_b200_kv_cache_bytes: [num_pages][heads_kv][page_size / 16] groups of
+ * 16 tokens.  page_size is a multiple of 16, head_dim (D) a multiple of 32.
+ * A group is 16 nibble rows of D / 2 bytes, then 16 rows of D / 32 fp16
+ * scales (9 D bytes).  The values are those of block_q4_0 along D (a value is
+ * d * (nibble - 8); byte i of a block holds value i in the low and value
+ * i + 16 in the high nibble); within a row the bytes of the B = D / 32
+ * blocks are interleaved: byte 4 t + e (t, e = 0..3) of block b is at
+ * t * 4 B + 4 b + e of a K row, byte 2 g + e (g = 0..7, e = 0, 1) at
+ * g * 2 B + 2 b + e of a V row.  A slot number is page * page_size + offset.
+ *
+ * Value formats of queries, keys, values and outputs are the codes
+ * PFNG_B200_OUT_F32 / _F16 / _BF16; rows are [tokens][heads * D] with a row
+ * stride in elements. */
+size_t pfng_b200_kv_cache_bytes(int64_t num_pages, int64_t page_size, int64_t heads_kv, int64_t head_dim);
+
+/* Plan of a step on the device, from the requests' lengths: request r has
+ * kv_len[r] tokens in the cache and brings q_len[r] new ones (a negative
+ * length counts as 0).  It keeps the ceil(kv_len / page_size) pages that its
+ * row of block_table [requests][max_pages] holds and takes what more it
+ * needs from free_pages [num_free], requests in order, first page first;
+ * these are written into its row.  Written:
+ *   seq_len [requests]     kv_len + q_len
+ *   cu_q [requests + 1]    first new token of each request, then their number
+ *   positions [max_tokens] kv_len + i for new token i of a request
+ *   slots [max_tokens]     its slot; -1 if it got no page (the free list or
+ *                          the table row is too short; a table entry < 0)
+ *   counts [3]             new tokens, pages wanted from the free list, new
+ *                          tokens left without a page
+ * Entries past the new tokens are -1 in positions and slots (max_tokens may be
+ * a fixed capacity); new tokens past max_tokens are not planned (counts[0]
+ * tells).  free_pages is not changed: the first counts[1] of it are in use. */
+int pfng_b200_kv_plan(const int32_t *kv_len, const int32_t *q_len, int64_t requests, int32_t *block_table,
+                      int64_t max_pages, const int32_t *free_pages, int64_t num_free, int64_t page_size,
+                      int32_t *seq_len, int32_t *cu_q, int32_t *positions, int64_t *slots, int64_t max_tokens,
+                      int32_t *counts, void *stream);
+
+/* RMS norm of every query and key head and the rotation by its position, in
+ * one pass.  x: rows of heads_q query heads, then heads_k key heads (what
+ * follows in a row, e.g. the values, is not read).  Per head
+ *   y = x / sqrt(mean(x^2) + eps) * weight      (as x where weight is NULL)
+ * and the first rot_dim values turn in pairs,
+ *   (a, b) -> (a cos - b sin, b cos + a sin),
+ * pairs (s, s + rot_dim / 2), or (2 s, 2 s + 1) when interleaved != 0.
+ * q_weight, k_weight: fp32 [head_dim] or NULL.  cos_sin: fp32
+ * [max_pos][rot_dim], rot_dim / 2 cosines then as many sines.  Computed in
+ * fp32, rounded once.  A row with a negative position (padding of kv_plan)
+ * is written as zeros, one with a position >= max_pos as NaN.
+ * head_dim even and <= 512, rot_dim even and <= head_dim.  q_out / k_out may
+ * be the heads of x themselves (same format, same strides). */
+int pfng_b200_qk_norm_rope(const void *x, int in_format, int64_t ldx, const float *q_weight, const float *k_weight,
+                           float eps, const int32_t *positions, const float *cos_sin, int64_t max_pos,
+                           int64_t rot_dim, int interleaved, void *q_out, int64_t ldq, void *k_out, int64_t ldk,
+                           int out_format, int64_t tokens, int64_t heads_q, int64_t heads_k, int64_t head_dim,
+                           void *stream);
+
+/* New keys and values into the cache: row t of k and v [tokens][heads_kv * D]
+ * is quantized to q4_0 (the bytes of pfng_b200_quantize_q4_0 of the same
+ * values) into slot slots[t]; a slot outside the cache (-1) skips the row.
+ * No two rows of a call may have the same slot.  head_dim <= 512. */
+int pfng_b200_kv_append_q4_0(const void *k, int64_t ldk, int k_format, const void *v, int64_t ldv, int v_format,
+                             const int64_t *slots, void *k_cache, void *v_cache, int64_t num_pages, int64_t page_size,
+                             int64_t tokens, int64_t heads_kv, int64_t head_dim, void *stream);
+
+/* Attention of new tokens over the cache: for new token i of request r (row
+ * cu_q[r] + i of q, position p = seq_len[r] - q_len + i) and query head h,
+ *   out = sum_j softmax_j(scale * q . k_j) v_j
+ * over the keys j < seq_len[r] of key head h / (heads_q / heads_kv), if
+ * causal != 0 only j <= p, and with window > 0 (causal only) only
+ * j > p - window.  A row that sees no key gives zeros (lse -inf).  Keys past
+ * seq_len and slots of other requests are never used, whatever they hold.
+ * Rows of q past cu_q[requests] are not computed; seq_len counts at most
+ * max_pages * page_size keys; keys on a page outside [0, num_pages) are not
+ * seen.
+ *   max_q, max_kv  upper bounds, known to the caller, of a request's new
+ *                  tokens and keys (they size the launch and the workspace)
+ *   lse            optional fp32 [tokens][heads_q]: ln sum_j e^(scale q.k_j)
+ *   workspace      pfng_b200_attention_q4_0_workspace_size bytes, 256-byte
+ *                  aligned (NULL when that is 0)
+ *   path           PFNG_B200_PATH_AUTO, or one of the others to force it
+ *                  (PFNG_B200_ERR_UNSUPPORTED where it cannot run)
+ * heads_q is a multiple of heads_kv; head_dim a multiple of 32, at most 256.
+ * Scores, softmax statistics and sums are fp32; results are the same for the
+ * same arguments (no atomics on values). */
+size_t pfng_b200_attention_q4_0_workspace_size(int64_t requests, int64_t tokens, int64_t max_q, int64_t max_kv,
+                                               int64_t heads_q, int64_t heads_kv, int64_t head_dim, int path);
+int pfng_b200_attention_q4_0(const void *q, int64_t ldq, int q_format, const void *k_cache, const void *v_cache,
+                             int64_t num_pages, int64_t page_size, const int32_t *block_table, int64_t max_pages,
+                             const int32_t *seq_len, const int32_t *cu_q, int64_t requests, int64_t tokens,
+                             int64_t max_q, int64_t max_kv, int64_t heads_q, int64_t heads_kv, int64_t head_dim,
+                             float scale, int causal, int64_t window, void *out, int64_t ldo, int out_format,
+                             float *lse, void *workspace, size_t workspace_bytes, int path, void *stream);
 
 #ifdef __cplusplus
 }

@@ -338,6 +338,11 @@ int device_sm_count() {
     return info ? info->sm_count : 148;
 }
 
+int device_status() {
+    DeviceInfo *info = nullptr;
+    return device_info(&info);
+}
+
 int *device_error_word() {
     DeviceInfo *info = current_info();
     return info ? info->error_word : nullptr;

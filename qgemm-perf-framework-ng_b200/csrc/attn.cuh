@@ -1,0 +1,30 @@
+// attn.cuh -- what the attention kernels share: which keys a query row sees
+// and where they are.
+#pragma once
+
+#include "kv_cache.cuh"
+
+namespace pfng {
+
+// Keys of request r: its length, within what its table row can address.
+PFNG_DEV int attn_seq_len(const AttnArgs &p, int64_t r) {
+    const int64_t most = p.max_pages * p.page_size, n = p.seq_len[r];
+    return static_cast<int>(n < 0 ? 0 : n > most ? most : n);
+}
+
+// Visible keys [lo, hi) of new token i of a request with `seq` keys, the last
+// q_len of them new: always one range (empty when hi <= lo).  A row without a
+// key (q_len > seq puts its position below zero) gives zeros.
+PFNG_DEV void attn_visible(const AttnArgs &p, int seq, int q_len, int i, int &lo, int &hi) {
+    const int pos = seq - q_len + i;
+    lo = p.window > 0 && pos >= p.window ? pos - static_cast<int>(p.window) + 1 : 0;
+    hi = p.causal ? min(pos + 1, seq) : seq;
+}
+
+// Page of key j of request r, -1 for an entry outside the cache.
+PFNG_DEV int attn_page(const AttnArgs &p, int64_t r, int j) {
+    const int page = p.table[r * p.max_pages + j / p.page_size];
+    return page >= 0 && page < p.num_pages ? page : -1;
+}
+
+}  // namespace pfng

@@ -1,0 +1,120 @@
+// attn_simple.cu -- attention over the q4_0 cache, one warp per query row and
+// head, for any head dimension the cache takes (pfng_b200_attention_q4_0).
+//
+// Per row with visible keys [lo, hi): s_j = scale q . k_j, then the running
+// maximum m and sum l of a softmax over chunks of 32 keys and
+// o = sum_j e^(s_j - m) v_j / l, all in fp32.  Lanes own keys for the scores
+// and dimensions for the values.  This is the path of head dimensions that
+// the tensor-core kernels do not tile; it is bound by instruction issue (a
+// few instructions per value and query row).
+#include "attn.cuh"
+
+namespace pfng {
+namespace {
+
+constexpr int kWarps = 4;
+
+__global__ void __launch_bounds__(kWarps * 32) attn_simple_kernel(const AttnArgs p) {
+    extern __shared__ float q_rows[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int dim = p.head_dim, blocks = dim / 32;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * kWarps + warp;
+    const int64_t token = row / p.heads_q;
+    const int head = static_cast<int>(row % p.heads_q), head_kv = head / (p.heads_q / p.heads_kv);
+    if (token >= p.tokens || token >= p.cu_q[p.requests]) return;
+    // the request of this token: last one whose first token is at or before it
+    int64_t a = 0, b = p.requests;
+    while (b - a > 1) {
+        const int64_t mid = (a + b) / 2;
+        if (p.cu_q[mid] <= token) a = mid;
+        else b = mid;
+    }
+    const int64_t r = a;
+    const int seq = attn_seq_len(p, r);
+    int lo, hi;
+    attn_visible(p, seq, p.cu_q[r + 1] - p.cu_q[r], static_cast<int>(token - p.cu_q[r]), lo, hi);
+
+    float *q = q_rows + warp * dim;
+    for (int i = lane; i < dim; i += 32) {
+        float one[1];
+        load_values<1>(p.q_format, p.q, token * p.ldq + static_cast<int64_t>(head) * dim + i, one);
+        q[i] = one[0];
+    }
+    __syncwarp();
+    const int groups = p.page_size / kKvGroup;
+    float m = -INFINITY, l = 0.0f, o[8] = {};
+    for (int base = lo & ~31; base < hi; base += 32) {
+        const int j = base + lane;
+        int page = -1;
+        if (j >= lo && j < hi) page = attn_page(p, r, j);
+        const int offset = j % p.page_size, in_group = offset % kKvGroup;
+        const int64_t at = page < 0 ? 0 : kv_group_offset(page, head_kv, offset, p.heads_kv, groups, dim);
+        float s = -INFINITY;
+        if (page >= 0) {
+            const uint8_t *group = p.k_cache + at;
+            const uint32_t *words = reinterpret_cast<const uint32_t *>(group + in_group * kv_row_bytes(dim));
+            const uint16_t *scales = reinterpret_cast<const uint16_t *>(group + kv_scale_offset(dim)) + in_group * blocks;
+            s = 0.0f;
+            for (int blk = 0; blk < blocks; ++blk) {
+                float sum = 0.0f;
+                for (int t = 0; t < 4; ++t) {
+                    const uint32_t w = words[t * blocks + blk];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        sum += q[32 * blk + 4 * t + e] * static_cast<float>(static_cast<int>((w >> (8 * e)) & 15u) - 8);
+                        sum += q[32 * blk + 16 + 4 * t + e] *
+                               static_cast<float>(static_cast<int>((w >> (8 * e + 4)) & 15u) - 8);
+                    }
+                }
+                s += f16_bits_to_f32(scales[blk]) * sum;
+            }
+            s *= p.scale;
+        }
+        float top = s;
+#pragma unroll
+        for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+        const float m_new = fmaxf(m, top);
+        if (m_new == -INFINITY) continue;  // nothing visible so far
+        const float keep = __expf(m - m_new);
+        const float e = page >= 0 ? __expf(s - m_new) : 0.0f;
+        float total = e;
+#pragma unroll
+        for (int x = 16; x > 0; x >>= 1) total += __shfl_xor_sync(0xffffffffu, total, x);
+        l = l * keep + total;
+        m = m_new;
+        for (int blk = 0; blk < blocks; ++blk) o[blk] *= keep;
+        const uint32_t present = __ballot_sync(0xffffffffu, page >= 0);
+        for (int c = 0; c < 32; ++c) {
+            const float pc = __shfl_sync(0xffffffffu, e, c);
+            const int64_t atc = __shfl_sync(0xffffffffu, at, c);
+            if (!((present >> c) & 1u)) continue;
+            const int rc = (base + c) % p.page_size % kKvGroup;
+            const uint8_t *group = p.v_cache + atc;
+            const uint8_t *bytes = group + rc * kv_row_bytes(dim);
+            const uint16_t *scales = reinterpret_cast<const uint16_t *>(group + kv_scale_offset(dim)) + rc * blocks;
+            const int i = lane & 15;
+            for (int blk = 0; blk < blocks; ++blk) {
+                const uint32_t byte = bytes[(i >> 1) * 2 * blocks + 2 * blk + (i & 1)];
+                const int n = static_cast<int>(lane < 16 ? byte & 15u : byte >> 4) - 8;
+                o[blk] += pc * f16_bits_to_f32(scales[blk]) * static_cast<float>(n);
+            }
+        }
+    }
+    const float inv = m == -INFINITY ? 0.0f : 1.0f / l;
+    for (int blk = 0; blk < blocks; ++blk) {
+        const float v[1] = {o[blk] * inv};
+        store_values<1>(p.out_format, p.out, token * p.ldo + static_cast<int64_t>(head) * dim + 32 * blk + lane, v);
+    }
+    if (p.lse && lane == 0) p.lse[token * p.heads_q + head] = m == -INFINITY ? -INFINITY : m + logf(l);
+}
+
+}  // namespace
+
+cudaError_t launch_attn_simple(const AttnArgs &p, cudaStream_t s) {
+    const int64_t rows = p.tokens * p.heads_q;
+    const unsigned grid = static_cast<unsigned>((rows + kWarps - 1) / kWarps);
+    attn_simple_kernel<<<grid, kWarps * 32, kWarps * p.head_dim * sizeof(float), s>>>(p);
+    return cudaGetLastError();
+}
+
+}  // namespace pfng

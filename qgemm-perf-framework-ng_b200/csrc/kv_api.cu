@@ -1,0 +1,164 @@
+// kv_api.cu -- extern "C" entry points of the attention step over the q4_0
+// cache: kv_plan, qk_norm_rope, kv_append_q4_0, attention_q4_0.
+//
+// As in api.cu, argument checks run on the host before any CUDA call, and an
+// empty problem is a valid no-op.
+#include "pfng_b200.h"
+#include "pfng_common.cuh"
+#include "pfng_internal.h"
+
+namespace pfng {
+namespace {
+
+int status_of(cudaError_t e) { return e == cudaSuccess ? PFNG_B200_OK : PFNG_B200_ERR_CUDA_BASE - static_cast<int>(e); }
+bool aligned(const void *p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+bool value_format(int fmt) { return fmt >= PFNG_B200_OUT_F32 && fmt <= PFNG_B200_OUT_BF16; }
+uintptr_t value_align(int fmt) { return fmt == PFNG_B200_OUT_F32 ? 4 : 2; }
+// Lengths, positions and page numbers are 32-bit on the device.
+constexpr int64_t kMaxCount = 0x7fffffff;
+bool page_size_ok(int64_t page_size) { return page_size > 0 && page_size % 16 == 0 && page_size <= (1 << 20); }
+
+// Checks of one attention call that need no pointers.
+int check_attention(int64_t requests, int64_t tokens, int64_t heads_q, int64_t heads_kv, int64_t head_dim,
+                    int64_t max_q, int64_t max_kv, int path) {
+    if (requests < 0 || tokens < 0 || heads_q < 0 || heads_kv < 0 || max_q < 0 || max_kv < 0)
+        return PFNG_B200_ERR_INVALID_ARGUMENT;
+    if (path < PFNG_B200_PATH_AUTO || path > PFNG_B200_PATH_SIMPLE) return PFNG_B200_ERR_INVALID_ARGUMENT;
+    if (requests > kMaxCount || tokens > kMaxCount || max_q > kMaxCount || max_kv > kMaxCount || heads_q > 65535)
+        return PFNG_B200_ERR_SHAPE;
+    if (head_dim < 32 || head_dim > 256 || head_dim % 32 != 0) return PFNG_B200_ERR_SHAPE;
+    if (heads_q > 0 && (heads_kv == 0 || heads_q % heads_kv != 0)) return PFNG_B200_ERR_SHAPE;
+    return PFNG_B200_OK;
+}
+
+}  // namespace
+}  // namespace pfng
+
+using namespace pfng;
+
+extern "C" {
+
+size_t pfng_b200_kv_cache_bytes(int64_t num_pages, int64_t page_size, int64_t heads_kv, int64_t head_dim) {
+    if (num_pages <= 0 || heads_kv <= 0 || !page_size_ok(page_size) || head_dim <= 0 || head_dim % 32 != 0) return 0;
+    return static_cast<size_t>(num_pages) * static_cast<size_t>(heads_kv) * static_cast<size_t>(page_size) *
+           static_cast<size_t>(head_dim / 2 + head_dim / 16);
+}
+
+int pfng_b200_kv_plan(const int32_t *kv_len, const int32_t *q_len, int64_t requests, int32_t *block_table,
+                      int64_t max_pages, const int32_t *free_pages, int64_t num_free, int64_t page_size,
+                      int32_t *seq_len, int32_t *cu_q, int32_t *positions, int64_t *slots, int64_t max_tokens,
+                      int32_t *counts, void *stream) {
+    if (requests < 0 || max_pages < 0 || num_free < 0 || max_tokens < 0) return PFNG_B200_ERR_INVALID_ARGUMENT;
+    if (!page_size_ok(page_size) || requests > kMaxCount || max_tokens > kMaxCount || max_pages > kMaxCount)
+        return PFNG_B200_ERR_SHAPE;
+    if (!cu_q || !counts) return PFNG_B200_ERR_INVALID_ARGUMENT;
+    if (requests > 0 && (!kv_len || !q_len || !seq_len || (max_pages > 0 && !block_table)))
+        return PFNG_B200_ERR_INVALID_ARGUMENT;
+    if ((num_free > 0 && !free_pages) || (max_tokens > 0 && (!positions || !slots)))
+        return PFNG_B200_ERR_INVALID_ARGUMENT;
+    for (const void *p : {static_cast<const void *>(kv_len), static_cast<const void *>(q_len),
+                          static_cast<const void *>(block_table), static_cast<const void *>(free_pages),
+                          static_cast<const void *>(seq_len), static_cast<const void *>(cu_q),
+                          static_cast<const void *>(positions), static_cast<const void *>(counts)})
+        if (!aligned(p, 4)) return PFNG_B200_ERR_ALIGNMENT;
+    if (!aligned(slots, 8)) return PFNG_B200_ERR_ALIGNMENT;
+    const int st = device_status();
+    if (st != PFNG_B200_OK) return st;
+    return status_of(launch_kv_plan(kv_len, q_len, requests, block_table, max_pages, free_pages, num_free, page_size,
+                                    seq_len, cu_q, positions, slots, max_tokens, counts,
+                                    static_cast<cudaStream_t>(stream)));
+}
+
+int pfng_b200_qk_norm_rope(const void *x, int in_format, int64_t ldx, const float *q_weight, const float *k_weight,
+                           float eps, const int32_t *positions, const float *cos_sin, int64_t max_pos,
+                           int64_t rot_dim, int interleaved, void *q_out, int64_t ldq, void *k_out, int64_t ldk,
+                           int out_format, int64_t tokens, int64_t heads_q, int64_t heads_k, int64_t head_dim,
+                           void *stream) {
+    if (!value_format(in_format) || !value_format(out_format)) return PFNG_B200_ERR_INVALID_ARGUMENT;
+    if (tokens < 0 || heads_q < 0 || heads_k < 0 || max_pos < 0 || rot_dim < 0) return PFNG_B200_ERR_INVALID_ARGUMENT;
+    if (head_dim <= 0 || head_dim > 512 || head_dim % 2 != 0 || rot_dim > head_dim || rot_dim % 2 != 0)
+        return PFNG_B200_ERR_SHAPE;
+    if (tokens > kMaxCount || heads_q > 65535 || heads_k > 65535 || max_pos > kMaxCount) return PFNG_B200_ERR_SHAPE;
+    if (tokens * (heads_q + heads_k) / 4 > kMaxCount) return PFNG_B200_ERR_SHAPE;  // rows of one launch
+    if (tokens > 0 && (ldx < (heads_q + heads_k) * head_dim || ldq < heads_q * head_dim || ldk < heads_k * head_dim))
+        return PFNG_B200_ERR_SHAPE;
+    if (tokens == 0 || heads_q + heads_k == 0) return PFNG_B200_OK;
+    if (!x || !positions || (rot_dim > 0 && !cos_sin) || (heads_q > 0 && !q_out) || (heads_k > 0 && !k_out))
+        return PFNG_B200_ERR_INVALID_ARGUMENT;
+    if (!aligned(x, value_align(in_format)) || !aligned(q_out, value_align(out_format)) ||
+        !aligned(k_out, value_align(out_format)) || !aligned(positions, 4) || !aligned(cos_sin, 4) ||
+        !aligned(q_weight, 4) || !aligned(k_weight, 4))
+        return PFNG_B200_ERR_ALIGNMENT;
+    const int st = device_status();
+    if (st != PFNG_B200_OK) return st;
+    const RopeArgs a{x, in_format, out_format, ldx, q_weight, k_weight, eps, positions, cos_sin, max_pos, rot_dim,
+                     interleaved, q_out, k_out, ldq, ldk, tokens, heads_q, heads_k, head_dim};
+    return status_of(launch_qk_norm_rope(a, static_cast<cudaStream_t>(stream)));
+}
+
+int pfng_b200_kv_append_q4_0(const void *k, int64_t ldk, int k_format, const void *v, int64_t ldv, int v_format,
+                             const int64_t *slots, void *k_cache, void *v_cache, int64_t num_pages, int64_t page_size,
+                             int64_t tokens, int64_t heads_kv, int64_t head_dim, void *stream) {
+    if (!value_format(k_format) || !value_format(v_format)) return PFNG_B200_ERR_INVALID_ARGUMENT;
+    if (tokens < 0 || heads_kv < 0 || num_pages < 0) return PFNG_B200_ERR_INVALID_ARGUMENT;
+    if (head_dim <= 0 || head_dim % 32 != 0 || head_dim > 512 || !page_size_ok(page_size)) return PFNG_B200_ERR_SHAPE;
+    if (tokens > kMaxCount || heads_kv > 65535 || num_pages > kMaxCount) return PFNG_B200_ERR_SHAPE;
+    if (tokens * heads_kv / 8 > kMaxCount) return PFNG_B200_ERR_SHAPE;  // rows of one launch
+    if (tokens > 0 && (ldk < heads_kv * head_dim || ldv < heads_kv * head_dim)) return PFNG_B200_ERR_SHAPE;
+    if (tokens == 0 || heads_kv == 0 || num_pages == 0) return PFNG_B200_OK;
+    if (!k || !v || !slots || !k_cache || !v_cache) return PFNG_B200_ERR_INVALID_ARGUMENT;
+    if (!aligned(k, value_align(k_format)) || !aligned(v, value_align(v_format)) || !aligned(slots, 8) ||
+        !aligned(k_cache, 16) || !aligned(v_cache, 16))
+        return PFNG_B200_ERR_ALIGNMENT;
+    const int st = device_status();
+    if (st != PFNG_B200_OK) return st;
+    const AppendArgs a{k, v, ldk, ldv, k_format, v_format, slots, static_cast<uint8_t *>(k_cache),
+                       static_cast<uint8_t *>(v_cache), num_pages, page_size, tokens, heads_kv, head_dim};
+    return status_of(launch_kv_append(a, static_cast<cudaStream_t>(stream)));
+}
+
+size_t pfng_b200_attention_q4_0_workspace_size(int64_t requests, int64_t tokens, int64_t max_q, int64_t max_kv,
+                                               int64_t heads_q, int64_t heads_kv, int64_t head_dim, int path) {
+    if (check_attention(requests, tokens, heads_q, heads_kv, head_dim, max_q, max_kv, path) != PFNG_B200_OK) return 0;
+    return 0;
+}
+
+int pfng_b200_attention_q4_0(const void *q, int64_t ldq, int q_format, const void *k_cache, const void *v_cache,
+                             int64_t num_pages, int64_t page_size, const int32_t *block_table, int64_t max_pages,
+                             const int32_t *seq_len, const int32_t *cu_q, int64_t requests, int64_t tokens,
+                             int64_t max_q, int64_t max_kv, int64_t heads_q, int64_t heads_kv, int64_t head_dim,
+                             float scale, int causal, int64_t window, void *out, int64_t ldo, int out_format,
+                             float *lse, void *workspace, size_t workspace_bytes, int path, void *stream) {
+    if (!value_format(q_format) || !value_format(out_format)) return PFNG_B200_ERR_INVALID_ARGUMENT;
+    int st = check_attention(requests, tokens, heads_q, heads_kv, head_dim, max_q, max_kv, path);
+    if (st != PFNG_B200_OK) return st;
+    if (window < 0 || (window > 0 && !causal) || num_pages < 0 || max_pages < 0) return PFNG_B200_ERR_INVALID_ARGUMENT;
+    if (!page_size_ok(page_size) || num_pages > kMaxCount || max_pages > kMaxCount || window > kMaxCount ||
+        max_pages * page_size > kMaxCount)
+        return PFNG_B200_ERR_SHAPE;
+    if (tokens > 0 && (ldq < heads_q * head_dim || ldo < heads_q * head_dim)) return PFNG_B200_ERR_SHAPE;
+    if (tokens == 0 || requests == 0 || heads_q == 0 || max_q == 0) return PFNG_B200_OK;
+    if (!q || !out || !seq_len || !cu_q) return PFNG_B200_ERR_INVALID_ARGUMENT;
+    if (num_pages > 0 && max_pages > 0 && (!k_cache || !v_cache || !block_table)) return PFNG_B200_ERR_INVALID_ARGUMENT;
+    if (!aligned(q, value_align(q_format)) || !aligned(out, value_align(out_format)) || !aligned(lse, 4) ||
+        !aligned(k_cache, 16) || !aligned(v_cache, 16) || !aligned(block_table, 4) || !aligned(seq_len, 4) ||
+        !aligned(cu_q, 4))
+        return PFNG_B200_ERR_ALIGNMENT;
+    if (path == PFNG_B200_PATH_GEMV || path == PFNG_B200_PATH_MMA) return PFNG_B200_ERR_UNSUPPORTED;
+    (void)workspace, (void)workspace_bytes;
+    if ((st = device_status()) != PFNG_B200_OK) return st;
+    AttnArgs a{};
+    a.q = q, a.q_format = q_format, a.ldq = ldq;
+    a.out = out, a.out_format = out_format, a.ldo = ldo;
+    a.k_cache = static_cast<const uint8_t *>(k_cache), a.v_cache = static_cast<const uint8_t *>(v_cache);
+    a.table = block_table, a.seq_len = seq_len, a.cu_q = cu_q, a.lse = lse;
+    // without pages no key is visible: the table is not read
+    a.num_pages = num_pages, a.max_pages = num_pages > 0 ? max_pages : 0;
+    a.requests = requests, a.tokens = tokens, a.max_q = max_q, a.max_kv = max_kv;
+    a.window = window, a.page_size = static_cast<int>(page_size), a.causal = causal != 0, a.scale = scale;
+    a.heads_q = static_cast<int>(heads_q), a.heads_kv = static_cast<int>(heads_kv);
+    a.head_dim = static_cast<int>(head_dim);
+    return status_of(launch_attn_simple(a, static_cast<cudaStream_t>(stream)));
+}
+
+}  // extern "C"

@@ -1,0 +1,151 @@
+// kv_plan.cu -- block table, slot map, positions and lengths of a serving
+// step, from the requests' lengths (pfng_b200_kv_plan).
+//
+// With S_r = kv_r + q_r, request r holds ceil(kv_r / p) pages of p tokens and
+// takes ceil(S_r / p) - ceil(kv_r / p) more from the free list, in request
+// order: two prefix sums over the requests (new tokens, new pages).  New token
+// i of request r stands at position kv_r + i, in slot page * p + offset.
+//
+// One launch without communication between its CTAs: each CTA owns kThreads
+// tokens, runs both prefix sums over all requests (a few KB that stay in L2)
+// and looks its tokens up in the scanned chunk that contains them.  The token
+// that opens a page (position a multiple of p) is the one that writes the
+// page into the table -- every new page begins with a new token -- so table
+// writes spread like the tokens do.  The call is bound by latency: launch,
+// load, two block scans, store.
+#include "kv_cache.cuh"
+#include "pfng_b200.h"
+
+namespace pfng {
+namespace {
+
+constexpr int kThreads = 512;
+
+struct PlanParams {
+    const int32_t *kv_len, *q_len, *free_pages;
+    int32_t *table, *seq_len, *cu_q, *positions, *counts;
+    int64_t *slots;
+    int64_t requests, max_pages, num_free, page_size, max_tokens;
+};
+
+// Inclusive sum over the CTA of (x, y) packed as two 64-bit counters.
+PFNG_DEV void block_scan(int64_t &x, int64_t &y, int64_t (*warp_sums)[2]) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t a = __shfl_up_sync(0xffffffffu, x, o), b = __shfl_up_sync(0xffffffffu, y, o);
+        if (lane >= o) x += a, y += b;
+    }
+    if (lane == 31) warp_sums[warp][0] = x, warp_sums[warp][1] = y;
+    __syncthreads();
+    if (warp == 0) {
+        int64_t a = lane < kThreads / 32 ? warp_sums[lane][0] : 0, b = lane < kThreads / 32 ? warp_sums[lane][1] : 0;
+#pragma unroll
+        for (int o = 1; o < kThreads / 32; o <<= 1) {
+            const int64_t c = __shfl_up_sync(0xffffffffu, a, o), d = __shfl_up_sync(0xffffffffu, b, o);
+            if (lane >= o) a += c, b += d;
+        }
+        if (lane < kThreads / 32) warp_sums[lane][0] = a, warp_sums[lane][1] = b;
+    }
+    __syncthreads();
+    if (warp > 0) x += warp_sums[warp - 1][0], y += warp_sums[warp - 1][1];
+}
+
+__global__ void __launch_bounds__(kThreads) kv_plan_kernel(const PlanParams p) {
+    __shared__ int64_t warp_sums[kThreads / 32][2];
+    __shared__ int64_t first_token[kThreads + 1], first_page[kThreads];
+    __shared__ int32_t kv_of[kThreads];
+    __shared__ int64_t lost_sums[kThreads / 32];
+    const int tid = threadIdx.x;
+    const int64_t token = static_cast<int64_t>(blockIdx.x) * kThreads + tid;
+    int64_t tokens_before = 0, pages_before = 0, lost = 0;
+    bool placed = false;
+    for (int64_t base = 0; base < p.requests; base += kThreads) {
+        const int64_t r = base + tid;
+        const bool live = r < p.requests;
+        const int64_t kv = live ? max(p.kv_len[r], 0) : 0, q = live ? max(p.q_len[r], 0) : 0;
+        const int64_t have = (kv + p.page_size - 1) / p.page_size;
+        const int64_t need = (kv + q + p.page_size - 1) / p.page_size - have;
+        int64_t t = q, n = need;
+        block_scan(t, n, warp_sums);
+        const int64_t all_tokens = warp_sums[kThreads / 32 - 1][0], all_pages = warp_sums[kThreads / 32 - 1][1];
+        first_token[tid] = tokens_before + t - q;
+        first_page[tid] = pages_before + n - need;
+        kv_of[tid] = static_cast<int32_t>(kv);
+        if (tid == 0) first_token[kThreads] = tokens_before + all_tokens;
+        if (live && (base / kThreads) % gridDim.x == blockIdx.x) {
+            p.seq_len[r] = static_cast<int32_t>(kv + q);
+            p.cu_q[r + 1] = static_cast<int32_t>(tokens_before + t);
+            if (r == 0) p.cu_q[0] = 0;
+        }
+        if (live && blockIdx.x == 0) {
+            // pages that request r has in the end, of those it wants
+            int64_t got = min(max(p.num_free - (pages_before + n - need), int64_t{0}), need) + have;
+            got = min(got, p.max_pages);
+            lost += min(q, max(kv + q - got * p.page_size, int64_t{0}));
+        }
+        __syncthreads();
+        if (!placed && token < tokens_before + all_tokens && token < p.max_tokens) {
+            // last request whose first token is at or before this one
+            int lo = 0, hi = kThreads;
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) / 2;
+                if (first_token[mid] <= token) lo = mid;
+                else hi = mid;
+            }
+            const int64_t kv_r = kv_of[lo], pos = kv_r + token - first_token[lo];
+            const int64_t page_at = pos / p.page_size, offset = pos % p.page_size;
+            const int64_t had = (kv_r + p.page_size - 1) / p.page_size;
+            int64_t page = -1;
+            if (page_at < p.max_pages) {
+                int32_t *entry = p.table + (base + lo) * p.max_pages + page_at;
+                if (page_at < had) {
+                    page = *entry;
+                } else {
+                    const int64_t at = first_page[lo] + page_at - had;
+                    if (at < p.num_free) page = p.free_pages[at];
+                    if (offset == 0) *entry = static_cast<int32_t>(page);
+                }
+            }
+            p.positions[token] = static_cast<int32_t>(pos);
+            p.slots[token] = page < 0 ? -1 : page * p.page_size + offset;
+            placed = true;
+        }
+        tokens_before += all_tokens;
+        pages_before += all_pages;
+        __syncthreads();
+    }
+    if (!placed && token < p.max_tokens) {
+        p.positions[token] = -1;
+        p.slots[token] = -1;
+    }
+    if (blockIdx.x == 0) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) lost += __shfl_xor_sync(0xffffffffu, lost, o);
+        if ((tid & 31) == 0) lost_sums[tid >> 5] = lost;
+        __syncthreads();
+        if (tid == 0) {
+            int64_t sum = 0;
+            for (int w = 0; w < kThreads / 32; ++w) sum += lost_sums[w];
+            if (p.requests == 0) p.cu_q[0] = 0;
+            p.counts[0] = static_cast<int32_t>(tokens_before);
+            p.counts[1] = static_cast<int32_t>(pages_before);
+            p.counts[2] = static_cast<int32_t>(sum);
+        }
+    }
+}
+
+}  // namespace
+
+cudaError_t launch_kv_plan(const int32_t *kv_len, const int32_t *q_len, int64_t requests, int32_t *table,
+                           int64_t max_pages, const int32_t *free_pages, int64_t num_free, int64_t page_size,
+                           int32_t *seq_len, int32_t *cu_q, int32_t *positions, int64_t *slots, int64_t max_tokens,
+                           int32_t *counts, cudaStream_t s) {
+    const PlanParams p{kv_len, q_len, free_pages, table, seq_len, cu_q, positions, counts, slots,
+                       requests, max_pages, num_free, page_size, max_tokens};
+    const int64_t grid = max_tokens > 0 ? (max_tokens + kThreads - 1) / kThreads : 1;
+    kv_plan_kernel<<<static_cast<unsigned>(grid), kThreads, 0, s>>>(p);
+    return cudaGetLastError();
+}
+
+}  // namespace pfng

@@ -135,11 +135,63 @@ cudaError_t launch_simple(const SimpleArgs &args, cudaStream_t s);
 cudaError_t launch_pack_q4_0_planar(const void *w, void *w_planar, int64_t n, int64_t k, cudaStream_t s);
 cudaError_t launch_unpack_q4_0_planar(const void *w_planar, void *w, int64_t n, int64_t k, cudaStream_t s);
 
+// kv_plan.cu -- block table, slots, positions and lengths of a serving step
+cudaError_t launch_kv_plan(const int32_t *kv_len, const int32_t *q_len, int64_t requests, int32_t *table,
+                           int64_t max_pages, const int32_t *free_pages, int64_t num_free, int64_t page_size,
+                           int32_t *seq_len, int32_t *cu_q, int32_t *positions, int64_t *slots, int64_t max_tokens,
+                           int32_t *counts, cudaStream_t s);
+
+// qk_norm_rope.cu -- formats are kOutF32 / kOutF16 / kOutBF16
+struct RopeArgs {
+    const void *x;
+    int in_format, out_format;
+    int64_t ldx;
+    const float *q_weight, *k_weight;
+    float eps;
+    const int32_t *positions;
+    const float *cos_sin;
+    int64_t max_pos, rot_dim;
+    int interleaved;
+    void *q_out, *k_out;
+    int64_t ldq, ldk;
+    int64_t tokens, heads_q, heads_k, head_dim;
+};
+cudaError_t launch_qk_norm_rope(const RopeArgs &args, cudaStream_t s);
+
+// kv_append.cu
+struct AppendArgs {
+    const void *k, *v;
+    int64_t ldk, ldv;
+    int k_format, v_format;
+    const int64_t *slots;
+    uint8_t *k_cache, *v_cache;
+    int64_t num_pages, page_size, tokens, heads_kv, head_dim;
+};
+cudaError_t launch_kv_append(const AppendArgs &args, cudaStream_t s);
+
+// attn_*.cu -- attention over the q4_0 cache
+struct AttnArgs {
+    const void *q;
+    int q_format, out_format;
+    int64_t ldq, ldo;
+    const uint8_t *k_cache, *v_cache;
+    const int32_t *table, *seq_len, *cu_q;
+    void *out;
+    float *lse;
+    int64_t num_pages, max_pages, requests, tokens;
+    int64_t max_q, max_kv;  // upper bounds of the requests' new tokens and keys
+    int64_t window;
+    int page_size, heads_q, heads_kv, head_dim, causal;
+    float scale;
+};
+cudaError_t launch_attn_simple(const AttnArgs &args, cudaStream_t s);
+
 // shard.cu
 cudaError_t launch_unshard_columns(const float *slices, float *c, int64_t m, int64_t n, int64_t ldc, int world,
                                    int64_t granule, int64_t slice_width, cudaStream_t s);
 
 int device_sm_count();
+int device_status();  // PFNG_B200_OK if the current device can run the library, else the status to return
 size_t device_smem_optin();
 int *device_error_word();  // the current device's error word, nullptr if unavailable
 

@@ -17,6 +17,7 @@ import ctypes
 import os
 import pathlib
 import re
+import typing
 
 PACKAGE_DIR = pathlib.Path(__file__).resolve().parent.parent
 REPO_ROOT = PACKAGE_DIR.parent
@@ -135,6 +136,21 @@ def _declare(L: ctypes.CDLL) -> None:
     L.pfng_b200_mm_prepared.argtypes = [I, P, P, P, I64, I64, I64, I64, P, S, P]
     L.pfng_b200_selftest_wait.restype = I
     L.pfng_b200_selftest_wait.argtypes = [ctypes.c_uint, I, P, P]
+    F = ctypes.c_float
+    L.pfng_b200_kv_cache_bytes.restype = S
+    L.pfng_b200_kv_cache_bytes.argtypes = [I64, I64, I64, I64]
+    L.pfng_b200_kv_plan.restype = I
+    L.pfng_b200_kv_plan.argtypes = [P, P, I64, P, I64, P, I64, I64, P, P, P, P, I64, P, P]
+    L.pfng_b200_qk_norm_rope.restype = I
+    L.pfng_b200_qk_norm_rope.argtypes = [P, I, I64, P, P, F, P, P, I64, I64, I, P, I64, P, I64, I, I64, I64, I64, I64,
+                                         P]
+    L.pfng_b200_kv_append_q4_0.restype = I
+    L.pfng_b200_kv_append_q4_0.argtypes = [P, I64, I, P, I64, I, P, P, P, I64, I64, I64, I64, I64, P]
+    L.pfng_b200_attention_q4_0_workspace_size.restype = S
+    L.pfng_b200_attention_q4_0_workspace_size.argtypes = [I64, I64, I64, I64, I64, I64, I64, I]
+    L.pfng_b200_attention_q4_0.restype = I
+    L.pfng_b200_attention_q4_0.argtypes = [P, I64, I, P, P, I64, I64, P, I64, P, P, I64, I64, I64, I64, I64, I64, I64,
+                                           F, I, I64, P, I64, I, P, P, S, I, P]
 
 
 def header_functions() -> list[str]:
@@ -415,6 +431,114 @@ def selftest_wait(attempts: int, skip_arrive: bool, stream=None):
            "selftest_wait")
     status = lib().pfng_b200_check_kernel_error(_stream(stream))
     return int(done.item()), status
+
+
+# ------------------------------------- the attention step over a q4_0 cache
+class KvPlan(typing.NamedTuple):
+    """What kv_plan writes (int32 on the device, slots int64)."""
+    seq_len: typing.Any    # [requests] cached and new tokens
+    cu_q: typing.Any       # [requests + 1] first new token of each request
+    positions: typing.Any  # [max_tokens]
+    slots: typing.Any      # [max_tokens] page * page_size + offset, -1 without a page
+    counts: typing.Any     # [3] new tokens, pages wanted from the free list, new tokens without a page
+
+
+_value_formats = {}
+
+
+def _value_format(t) -> int:
+    """Format code of a tensor's values (fp32, fp16 or bf16)."""
+    if not _value_formats:
+        import torch
+        _value_formats.update({torch.float32: OUT_F32, torch.float16: OUT_F16, torch.bfloat16: OUT_BF16})
+    if t.dtype not in _value_formats or t.stride(-1) != 1:
+        raise PfngError(ERR_INVALID_ARGUMENT, f"values of {t.dtype} with strides {tuple(t.stride())}")
+    return _value_formats[t.dtype]
+
+
+def _value_tensor(fmt, rows: int, cols: int, device):
+    import torch
+    fmt = _fmt(fmt)
+    if fmt not in (OUT_F32, OUT_F16, OUT_BF16):
+        raise PfngError(ERR_INVALID_ARGUMENT, f"out_format {fmt}")
+    return torch.empty((rows, cols), dtype=(torch.float32, torch.float16, torch.bfloat16)[fmt], device=device)
+
+
+def kv_cache_bytes(num_pages: int, page_size: int, heads_kv: int, head_dim: int) -> int:
+    """Bytes of the K (and of the V) buffer of a q4_0 cache; 0 for unsupported sizes."""
+    return lib().pfng_b200_kv_cache_bytes(num_pages, page_size, heads_kv, head_dim)
+
+
+def kv_plan(kv_len, q_len, block_table, free_pages, page_size: int, max_tokens: int, out=None, stream=None) -> KvPlan:
+    """Block table (updated in place), slots, positions and lengths of a step whose request r has kv_len[r] tokens
+    in the cache and brings q_len[r] new ones (int32 on the device; pfng_b200_kv_plan)."""
+    import torch
+    n = kv_len.numel()
+    if out is None:
+        dev = kv_len.device
+        out = KvPlan(torch.empty(n, dtype=torch.int32, device=dev), torch.empty(n + 1, dtype=torch.int32, device=dev),
+                     torch.empty(max_tokens, dtype=torch.int32, device=dev),
+                     torch.empty(max_tokens, dtype=torch.int64, device=dev),
+                     torch.empty(3, dtype=torch.int32, device=dev))
+    _check(lib().pfng_b200_kv_plan(_ptr(kv_len), _ptr(q_len), n, _ptr(block_table), block_table.shape[1],
+                                   _ptr(free_pages), free_pages.numel(), page_size, _ptr(out.seq_len), _ptr(out.cu_q),
+                                   _ptr(out.positions), _ptr(out.slots), max_tokens, _ptr(out.counts),
+                                   _stream(stream)), "kv_plan")
+    return out
+
+
+def qk_norm_rope(x, positions, cos_sin, heads_q: int, heads_k: int, head_dim: int, q_weight=None, k_weight=None,
+                 eps: float = 1e-6, interleaved: bool = False, out_format="bf16", q_out=None, k_out=None, stream=None):
+    """RMS norm (where a weight is given) and position rotation of the query and key heads of x [tokens][..];
+    cos_sin is fp32 [max_pos][rot_dim].  Returns (q [tokens][heads_q * head_dim], k [tokens][heads_k * head_dim])."""
+    tokens = x.shape[0]
+    if q_out is None:
+        q_out = _value_tensor(out_format, tokens, heads_q * head_dim, x.device)
+    if k_out is None:
+        k_out = _value_tensor(out_format, tokens, heads_k * head_dim, x.device)
+    fmt = _value_format(q_out)
+    if _value_format(k_out) != fmt:
+        raise PfngError(ERR_INVALID_ARGUMENT, "qk_norm_rope: q_out and k_out of two types")
+    _check(lib().pfng_b200_qk_norm_rope(
+        _ptr(x), _value_format(x), x.stride(0), _ptr(q_weight), _ptr(k_weight), eps, _ptr(positions), _ptr(cos_sin),
+        cos_sin.shape[0], cos_sin.shape[1], 1 if interleaved else 0, _ptr(q_out), q_out.stride(0), _ptr(k_out),
+        k_out.stride(0), fmt, tokens, heads_q, heads_k, head_dim, _stream(stream)), "qk_norm_rope")
+    return q_out, k_out
+
+
+def _cache_pages(cache, page_size: int, heads_kv: int, head_dim: int) -> int:
+    page = kv_cache_bytes(1, page_size, heads_kv, head_dim)
+    return cache.numel() // page if page else 0
+
+
+def kv_append_q4_0(k, v, slots, k_cache, v_cache, heads_kv: int, head_dim: int, page_size: int, stream=None) -> None:
+    """Rows of k and v [tokens][heads_kv * head_dim] quantized to q4_0 into the cache's slots (int64; -1 skips)."""
+    pages = min(_cache_pages(k_cache, page_size, heads_kv, head_dim),
+                _cache_pages(v_cache, page_size, heads_kv, head_dim))
+    _check(lib().pfng_b200_kv_append_q4_0(
+        _ptr(k), k.stride(0), _value_format(k), _ptr(v), v.stride(0), _value_format(v), _ptr(slots), _ptr(k_cache),
+        _ptr(v_cache), pages, page_size, k.shape[0], heads_kv, head_dim, _stream(stream)), "kv_append_q4_0")
+
+
+def attention_q4_0(q, k_cache, v_cache, block_table, seq_len, cu_q, heads_q: int, heads_kv: int, head_dim: int,
+                   page_size: int, max_q: int, max_kv: int, scale=None, causal: bool = True, window: int = 0,
+                   out_format="bf16", out=None, lse=None, path="auto", workspace=None, stream=None):
+    """Attention of the new tokens q [tokens][heads_q * head_dim] over the q4_0 cache (pfng_b200_attention_q4_0);
+    scale defaults to 1 / sqrt(head_dim), max_q and max_kv bound a request's new tokens and keys."""
+    tokens, requests, p = q.shape[0], seq_len.numel(), _path(path)
+    if out is None:
+        out = _value_tensor(out_format, tokens, heads_q * head_dim, q.device)
+    ws = _workspace(lib().pfng_b200_attention_q4_0_workspace_size(requests, tokens, max_q, max_kv, heads_q, heads_kv,
+                                                                  head_dim, p), q.device, workspace)
+    pages = min(_cache_pages(k_cache, page_size, heads_kv, head_dim),
+                _cache_pages(v_cache, page_size, heads_kv, head_dim))
+    _check(lib().pfng_b200_attention_q4_0(
+        _ptr(q), q.stride(0), _value_format(q), _ptr(k_cache), _ptr(v_cache), pages, page_size, _ptr(block_table),
+        block_table.shape[1], _ptr(seq_len), _ptr(cu_q), requests, tokens, max_q, max_kv, heads_q, heads_kv, head_dim,
+        head_dim ** -0.5 if scale is None else scale, 1 if causal else 0, window, _ptr(out), out.stride(0),
+        _value_format(out), _ptr(lse), _ptr(ws), 0 if ws is None else ws.numel(), p, _stream(stream)),
+        "attention_q4_0")
+    return out
 
 
 # ----------------------------------------------------------------- sharding
