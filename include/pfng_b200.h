@@ -413,10 +413,11 @@ int pfng_b200_kv_append_q4_0(const void *k, int64_t ldk, int k_format, const voi
  * j > p - window.  A row that sees no key gives zeros (lse -inf).  Keys past
  * seq_len and slots of other requests are never used, whatever they hold.
  * Rows of q past cu_q[requests] are not computed; seq_len counts at most
- * max_pages * page_size keys; keys on a page outside [0, num_pages) are not
+ * max_pages * page_size keys (<= 2^30); keys on a page outside [0, num_pages) are not
  * seen.
  *   max_q, max_kv  upper bounds, known to the caller, of a request's new
- *                  tokens and keys (they size the launch and the workspace)
+ *                  tokens and keys (they size the launch and the workspace;
+ *                  new tokens past max_q are not computed)
  *   lse            optional fp32 [tokens][heads_q]: ln sum_j e^(scale q.k_j)
  *   workspace      pfng_b200_attention_q4_0_workspace_size bytes, 256-byte
  *                  aligned (NULL when that is 0)

@@ -12,6 +12,16 @@ PFNG_DEV int attn_seq_len(const AttnArgs &p, int64_t r) {
     return static_cast<int>(n < 0 ? 0 : n > most ? most : n);
 }
 
+// New tokens of request r: `all` as its cu_q says (positions count from
+// there), of which the returned number lie within q and max_q.
+PFNG_DEV int attn_new_tokens(const AttnArgs &p, int64_t r, int &all) {
+    const int64_t first = p.cu_q[r], last = p.cu_q[r + 1];
+    all = static_cast<int>(last - first);
+    if (first < 0 || last <= first) return 0;
+    const int64_t n = min(min(last, p.tokens) - first, p.max_q);
+    return static_cast<int>(max(n, int64_t{0}));
+}
+
 // Visible keys [lo, hi) of new token i of a request with `seq` keys, the last
 // q_len of them new: always one range (empty when hi <= lo).  A row without a
 // key (q_len > seq puts its position below zero) gives zeros.

@@ -1,0 +1,791 @@
+// attn_stream.cu -- attention over the q4_0 cache for few query rows per key
+// head (decode, a few drafted tokens): bound by the bytes of the cache
+// (pfng_b200_attention_q4_0, PFNG_B200_PATH_GEMV).
+//
+// Work: the rows of a request that share a key head (new tokens x query heads
+// of the group) form row tiles of 8 * NT; an item is one (request, key head,
+// row tile), and a unit of it kUnit keys.  All units of all items lie on one
+// line, which is cut into equal pieces, one per warp of the GPU: every warp
+// streams the same number of keys whatever the lengths are.  A piece can end
+// inside an item; such an item leaves its (maximum, sum, unnormalised output)
+// per piece in the workspace, and a second kernel joins them in line order.
+//
+// A warp feeds itself: its lanes copy the 16-token groups of a unit (9 D
+// bytes each of K and V, contiguous whatever the page size) with bulk copies
+// into the warp's own ring of kStages, completed on an mbarrier per stage.
+// Nothing in the loop synchronises with another warp.
+//
+// Mathematics, per 16 keys, everything transposed so that the 8 columns of an
+// m16n8k16 are query rows (padding 1..8 rows to 8, not to 16):
+//   S^T = K Q^T   A = nibbles of K.  n & 15 in the low bits of an fp16 is the
+//     subnormal n 2^-24 (n 2^-20 for the high nibbles, whose q is scaled by
+//     1/16): one AND per two values, exact.  The accumulators start at
+//     -8 2^-24 sum(q) of the block, so a block ends as 2^-24 sum q (n - 8); the
+//     block's scale d is applied to that sum in fp32: keys are not rounded.
+//     Q is fp16, scaled per row by a power of two so that bf16 and fp32
+//     ranges fit (bf16 and fp16 values stay exact, fp32 loses 2^-11).
+//   P = 2^(S^T - M), M per row and warp: a maximum that is renewed (with a
+//     rescale of the sums) only when a score passes it by kSlack, as P up to
+//     2^kSlack is as exact as P up to 1.  Sums of P in fp32.
+//   O^T += V^T (d P)   A = n - 8 in fp16 (exact: 1024 + n minus 1032), B = d P
+//     in fp16, per block, brought from accumulator to operand layout by an
+//     8 x 8 transpose.  The rounding of d P to fp16 (2^-12 on average) is the
+//     only one between the cache and the fp32 output; a power of two that
+//     follows the largest d keeps d P in the middle of fp16's range.
+#include "attn.cuh"
+#include "pfng_tma.h"
+
+namespace pfng {
+namespace {
+
+constexpr int kWarps = 16;
+constexpr int kThreads = kWarps * 32;
+constexpr int kUnit = 32;    // keys of a unit: one stage of a warp's ring
+constexpr int kStages = 3;
+constexpr float kSlack = 6.0f;
+constexpr float kNoMax = -3.0e38f;  // the maximum before the first visible key
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct StreamParams {
+    AttnArgs a;
+    float *part_o;     // [slots][rows][dim]: unnormalised outputs of pieces
+    float2 *part_ml;   // [slots][rows]: maximum (log2) and sum
+    int vec_q;         // rows of q allow 4-value loads
+    int *err;
+};
+
+PFNG_DEV void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, "
+        "%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+PFNG_DEV uint32_t transpose8x8(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+PFNG_DEV float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+PFNG_DEV uint32_t h2(__half2 x) { return *reinterpret_cast<uint32_t *>(&x); }
+PFNG_DEV __half2 as_h2(uint32_t x) { return *reinterpret_cast<__half2 *>(&x); }
+PFNG_DEV float low_half(uint32_t x) { return __low2float(as_h2(x)); }
+PFNG_DEV float high_half(uint32_t x) { return __high2float(as_h2(x)); }
+
+// What a request contributes to the line: its row tiles and, per row tile,
+// the units that its rows see (at least one, so that rows without a key are
+// written too).
+struct RequestShape {
+    int seq, all, rows, tiles;  // keys, new tokens, query rows, row tiles
+};
+template <int NT>
+PFNG_DEV RequestShape request_shape(const AttnArgs &p, int64_t r) {
+    RequestShape s;
+    s.seq = attn_seq_len(p, r);
+    s.rows = attn_new_tokens(p, r, s.all) * (p.heads_q / p.heads_kv);
+    s.tiles = (s.rows + 8 * NT - 1) / (8 * NT);
+    return s;
+}
+// Units [first, first + count) of row tile `tile`.
+template <int NT>
+PFNG_DEV void tile_units(const AttnArgs &p, const RequestShape &s, int tile, int &first, int &count) {
+    const int group = p.heads_q / p.heads_kv;
+    int lo, hi, lo2, hi2;
+    attn_visible(p, s.seq, s.all, tile * 8 * NT / group, lo, hi2);
+    attn_visible(p, s.seq, s.all, (min(tile * 8 * NT + 8 * NT, s.rows) - 1) / group, lo2, hi);
+    first = max(lo, 0) / kUnit;
+    count = max((hi + kUnit - 1) / kUnit - first, 1);
+}
+template <int NT>
+PFNG_DEV int64_t request_units(const AttnArgs &p, int64_t r) {
+    const RequestShape s = request_shape<NT>(p, r);
+    int64_t sum = 0;
+    for (int t = 0; t < s.tiles; ++t) {
+        int first, count;
+        tile_units<NT>(p, s, t, first, count);
+        sum += count;
+    }
+    return sum * p.heads_kv;
+}
+
+// Sum over all requests of (units, items), and over the requests before `r`,
+// by all threads of a CTA.
+template <int NT, int THREADS>
+PFNG_DEV void line_totals(const AttnArgs &p, int64_t r, int64_t &units, int64_t &units_before, int64_t &items_before) {
+    __shared__ int64_t sums[THREADS / 32][3];
+    int64_t u = 0, ub = 0, ib = 0;
+    for (int64_t i = threadIdx.x; i < p.requests; i += THREADS) {
+        const int64_t n = request_units<NT>(p, i);
+        u += n;
+        if (i < r) ub += n, ib += static_cast<int64_t>(request_shape<NT>(p, i).tiles) * p.heads_kv;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        u += __shfl_xor_sync(0xffffffffu, u, o);
+        ub += __shfl_xor_sync(0xffffffffu, ub, o);
+        ib += __shfl_xor_sync(0xffffffffu, ib, o);
+    }
+    if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5][0] = u, sums[threadIdx.x >> 5][1] = ub, sums[threadIdx.x >> 5][2] = ib;
+    __syncthreads();
+    units = units_before = items_before = 0;
+    for (int w = 0; w < THREADS / 32; ++w) units += sums[w][0], units_before += sums[w][1], items_before += sums[w][2];
+}
+
+PFNG_DEV int64_t piece_start(int64_t worker, int64_t units, int64_t workers) { return worker * units / workers; }
+
+// Position of a warp on the line.
+struct Cursor {
+    int64_t r, item;       // request, item number
+    int head, tile;        // key head and row tile of the item
+    int first, count, at;  // units of the item, and the next one of them
+    RequestShape shape;
+};
+template <int NT>
+PFNG_DEV void open_request(const AttnArgs &p, Cursor &c) {  // at request c.r, which has rows, or the next that has
+    while (c.r < p.requests) {
+        c.shape = request_shape<NT>(p, c.r);
+        if (c.shape.tiles > 0) break;
+        ++c.r;
+    }
+    c.head = c.tile = c.at = 0;
+    if (c.r < p.requests) tile_units<NT>(p, c.shape, 0, c.first, c.count);
+}
+template <int NT>
+PFNG_DEV void next_item(const AttnArgs &p, Cursor &c) {
+    ++c.item;
+    c.at = 0;
+    if (++c.tile == c.shape.tiles) {
+        c.tile = 0;
+        if (++c.head == p.heads_kv) {
+            ++c.r;
+            open_request<NT>(p, c);
+            return;
+        }
+    }
+    tile_units<NT>(p, c.shape, c.tile, c.first, c.count);
+}
+// Cursor at unit `u` of the line, by one warp.
+template <int NT>
+PFNG_DEV Cursor seek(const AttnArgs &p, int64_t u) {
+    const int lane = threadIdx.x & 31;
+    Cursor c;
+    c.item = 0;
+    int64_t before = 0;
+    c.r = p.requests;
+    for (int64_t base = 0; base < p.requests; base += 32) {
+        const int64_t i = base + lane;
+        int64_t n = i < p.requests ? request_units<NT>(p, i) : 0;
+        int64_t items = i < p.requests ? static_cast<int64_t>(request_shape<NT>(p, i).tiles) * p.heads_kv : 0;
+        const int64_t own = n, own_items = items;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t x = __shfl_up_sync(0xffffffffu, n, o), y = __shfl_up_sync(0xffffffffu, items, o);
+            if (lane >= o) n += x, items += y;
+        }
+        const uint32_t past = __ballot_sync(0xffffffffu, before + n > u);
+        if (past) {
+            const int k = __ffs(past) - 1;
+            c.r = base + k;
+            before += __shfl_sync(0xffffffffu, n - own, k);
+            c.item += __shfl_sync(0xffffffffu, items - own_items, k);
+            break;
+        }
+        before += __shfl_sync(0xffffffffu, n, 31);
+        c.item += __shfl_sync(0xffffffffu, items, 31);
+    }
+    open_request<NT>(p, c);
+    if (c.r >= p.requests) return c;
+    int64_t left = u - before;
+    int64_t per_head = 0;
+    for (int t = 0; t < c.shape.tiles; ++t) {
+        int first, count;
+        tile_units<NT>(p, c.shape, t, first, count);
+        per_head += count;
+    }
+    c.head = static_cast<int>(left / per_head);
+    left -= c.head * per_head;
+    c.item += static_cast<int64_t>(c.head) * c.shape.tiles;
+    while (left >= c.count) {
+        left -= c.count;
+        ++c.tile, ++c.item;
+        tile_units<NT>(p, c.shape, c.tile, c.first, c.count);
+    }
+    c.at = static_cast<int>(left);
+    return c;
+}
+
+// Bulk copies of a unit's groups into a stage; returns the groups that are
+// there (bit i: keys 16 i .. of the unit).
+template <int DIM>
+PFNG_DEV uint32_t fetch_unit(const AttnArgs &p, const Cursor &c, uint8_t *stage, uint64_t *bar, uint64_t policy) {
+    constexpr int kGroups = kUnit / kKvGroup;
+    constexpr uint32_t kBytes = kv_group_bytes(DIM);
+    const int lane = threadIdx.x & 31;
+    const int g = lane % kGroups;
+    const bool is_v = lane >= kGroups;
+    const int key = (c.first + c.at) * kUnit + g * kKvGroup;
+    const int page = lane < 2 * kGroups && key < c.shape.seq ? attn_page(p, c.r, key) : -1;
+    const uint32_t there = __ballot_sync(0xffffffffu, page >= 0) & ((1u << kGroups) - 1);
+    if (lane == 0) mbar_arrive_expect_tx(bar, 2 * kBytes * __popc(there));
+    __syncwarp();
+    if (page >= 0) {
+        const int64_t at = kv_group_offset(page, c.head, key % p.page_size, p.heads_kv, p.page_size / kKvGroup, DIM);
+        bulk_copy_g2s(stage + lane * kBytes, (is_v ? p.v_cache : p.k_cache) + at, kBytes, bar, policy);
+    }
+    return there;
+}
+
+template <int DIM, int NT>
+struct RowTile {
+    static constexpr int kBlocks = DIM / 32;
+    uint32_t q[NT][kBlocks][4];   // B fragments: low nibbles (2), high nibbles / 16 (2)
+    float start[NT][kBlocks][2];  // -8 2^-24 sum(q) per block, of this thread's two rows
+    float mul[NT][2];             // score = accumulator * mul, in log2 units
+    int lo[NT][2], hi[NT][2];     // visible keys of this thread's two rows
+    int lo_max, hi_min;           // keys that every row sees
+    int lo_min, hi_max;           // keys that some row sees
+};
+
+template <int DIM, int NT>
+PFNG_DEV void load_rows(const StreamParams &sp, const Cursor &c, RowTile<DIM, NT> &t) {
+    const AttnArgs &p = sp.a;
+    const int lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
+    const int group = p.heads_q / p.heads_kv;
+    t.lo_max = 0, t.hi_min = 0x7fffffff, t.lo_min = 0x7fffffff, t.hi_max = 0;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int row = (c.tile * NT + n) * 8 + g;
+        const bool live = row < c.shape.rows;
+        float v[DIM / 32][2][4];
+        float top = 0.0f;
+        const int64_t at = (p.cu_q[c.r] + static_cast<int64_t>(live ? row / group : 0)) * p.ldq +
+                           (static_cast<int64_t>(c.head) * group + (live ? row % group : 0)) * DIM;
+#pragma unroll
+        for (int b = 0; b < DIM / 32; ++b)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[b][h][i] = 0.0f;
+                if (live) {
+                    if (sp.vec_q) {
+                        load_values<4>(p.q_format, p.q, at + 32 * b + 16 * h + 4 * q4, v[b][h]);
+                    } else {
+                        for (int i = 0; i < 4; ++i) {
+                            float one[1];
+                            load_values<1>(p.q_format, p.q, at + 32 * b + 16 * h + 4 * q4 + i, one);
+                            v[b][h][i] = one[0];
+                        }
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(v[b][h][i]));
+            }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // largest value into [2^13, 2^14): exact, and room for the 1/16
+        int e = 0;
+        if (top > 0.0f && top < INFINITY) e = ilogbf(top) - 13;
+        const float up0 = ldexpf(1.0f, -(e / 2)), up1 = ldexpf(1.0f, -(e - e / 2));
+        float sum[DIM / 32];
+#pragma unroll
+        for (int b = 0; b < DIM / 32; ++b) {
+            float x[2][4];
+            sum[b] = 0.0f;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    // high nibbles carry a factor 16: their q is divided by it
+                    const __half y = __float2half_rn(v[b][h][i] * up0 * up1 * (h ? 0.0625f : 1.0f));
+                    x[h][i] = __half2float(y);
+                    sum[b] += x[h][i] * (h ? 16.0f : 1.0f);
+                }
+            t.q[n][b][0] = h2(__floats2half2_rn(x[0][0], x[0][2]));
+            t.q[n][b][1] = h2(__floats2half2_rn(x[0][1], x[0][3]));
+            t.q[n][b][2] = h2(__floats2half2_rn(x[1][0], x[1][2]));
+            t.q[n][b][3] = h2(__floats2half2_rn(x[1][1], x[1][3]));
+            sum[b] += __shfl_xor_sync(0xffffffffu, sum[b], 1);
+            sum[b] += __shfl_xor_sync(0xffffffffu, sum[b], 2);
+        }
+        const float mul = ldexpf(p.scale * kLog2e, e + 24);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const int from = (2 * q4 + x) * 4;  // a lane that loaded row 2 q4 + x
+#pragma unroll
+            for (int b = 0; b < DIM / 32; ++b)
+                t.start[n][b][x] = -8.0f * 0x1p-24f * __shfl_sync(0xffffffffu, sum[b], from);
+            t.mul[n][x] = __shfl_sync(0xffffffffu, mul, from);
+            const int rr = (c.tile * NT + n) * 8 + 2 * q4 + x;
+            int lo = 0, hi = 0;
+            if (rr < c.shape.rows) {
+                attn_visible(p, c.shape.seq, c.shape.all, rr / group, lo, hi);
+                hi = max(hi, 0);
+                t.lo_max = max(t.lo_max, lo), t.hi_min = min(t.hi_min, hi);
+                t.lo_min = min(t.lo_min, lo), t.hi_max = max(t.hi_max, hi);
+            }
+            t.lo[n][x] = lo, t.hi[n][x] = hi;
+        }
+    }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+        t.lo_max = max(t.lo_max, __shfl_xor_sync(0xffffffffu, t.lo_max, o));
+        t.hi_min = min(t.hi_min, __shfl_xor_sync(0xffffffffu, t.hi_min, o));
+        t.lo_min = min(t.lo_min, __shfl_xor_sync(0xffffffffu, t.lo_min, o));
+        t.hi_max = max(t.hi_max, __shfl_xor_sync(0xffffffffu, t.hi_max, o));
+    }
+}
+
+template <int DIM, int NT>
+struct RowSums {
+    float o[NT][DIM / 16][4];  // O^T tiles: rows = 16 dimensions, columns = query rows
+    float l[NT][2];            // sums of P over this thread's keys
+    float m[NT][2];
+    float sv;                  // power of two that P d carries
+    float d_limit;             // largest |d| that sv takes
+};
+template <int DIM, int NT>
+PFNG_DEV void clear(RowSums<DIM, NT> &s) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int j = 0; j < DIM / 16; ++j) s.o[n][j][0] = s.o[n][j][1] = s.o[n][j][2] = s.o[n][j][3] = 0.0f;
+        s.l[n][0] = s.l[n][1] = 0.0f;
+        s.m[n][0] = s.m[n][1] = kNoMax;
+    }
+    s.sv = 1.0f;
+    s.d_limit = 0.0f;
+}
+
+// Key that row r of an MMA stands for (of 16): rows 2 t and 2 t + 1, the two
+// keys of one V operand register, are keys t and t + 4, so that the quads of
+// a warp read neighbouring rows of shared memory.
+PFNG_DEV int key_of_row(int r) { return (r & 8) | ((r & 7) >> 1) | ((r & 1) << 2); }
+
+// 16 keys: key0 is the first one's number, `kg` / `vg` their groups.
+template <int DIM, int NT, bool MASKED>
+PFNG_DEV void attend16(const RowTile<DIM, NT> &t, RowSums<DIM, NT> &s, const uint8_t *kg, const uint8_t *vg,
+                       int key0) {
+    constexpr int kBlocks = DIM / 32;
+    const int lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
+    const int ka = key_of_row(g), kb = ka + 8;  // this thread's keys (accumulator rows g and g + 8)
+
+    // ---- scores ----
+    uint32_t wa[kBlocks], wb[kBlocks], da[(kBlocks + 1) / 2], db[(kBlocks + 1) / 2];
+    if constexpr (kBlocks == 4) {
+        const uint4 x = *reinterpret_cast<const uint4 *>(kg + ka * 64 + q4 * 16);
+        const uint4 y = *reinterpret_cast<const uint4 *>(kg + kb * 64 + q4 * 16);
+        wa[0] = x.x, wa[1] = x.y, wa[2] = x.z, wa[3] = x.w;
+        wb[0] = y.x, wb[1] = y.y, wb[2] = y.z, wb[3] = y.w;
+        const uint2 u = *reinterpret_cast<const uint2 *>(kg + kv_scale_offset(DIM) + ka * 8);
+        const uint2 v = *reinterpret_cast<const uint2 *>(kg + kv_scale_offset(DIM) + kb * 8);
+        da[0] = u.x, da[1] = u.y, db[0] = v.x, db[1] = v.y;
+    } else {
+        const uint2 x = *reinterpret_cast<const uint2 *>(kg + ka * 32 + q4 * 8);
+        const uint2 y = *reinterpret_cast<const uint2 *>(kg + kb * 32 + q4 * 8);
+        wa[0] = x.x, wa[1] = x.y, wb[0] = y.x, wb[1] = y.y;
+        da[0] = *reinterpret_cast<const uint32_t *>(kg + kv_scale_offset(DIM) + ka * 4);
+        db[0] = *reinterpret_cast<const uint32_t *>(kg + kv_scale_offset(DIM) + kb * 4);
+    }
+    float sc[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.0f;
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b) {
+        const uint32_t a8 = wa[b] >> 8, b8 = wb[b] >> 8;
+        const float fa = (b & 1) ? high_half(da[b / 2]) : low_half(da[b / 2]);
+        const float fb = (b & 1) ? high_half(db[b / 2]) : low_half(db[b / 2]);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            float c[4] = {t.start[n][b][0], t.start[n][b][1], t.start[n][b][0], t.start[n][b][1]};
+            mma_f16(c, wa[b] & 0x000F000Fu, wb[b] & 0x000F000Fu, a8 & 0x000F000Fu, b8 & 0x000F000Fu, t.q[n][b][0],
+                    t.q[n][b][1]);
+            mma_f16(c, wa[b] & 0x00F000F0u, wb[b] & 0x00F000F0u, a8 & 0x00F000F0u, b8 & 0x00F000F0u, t.q[n][b][2],
+                    t.q[n][b][3]);
+            sc[n][0] = fmaf(fa, c[0], sc[n][0]);
+            sc[n][1] = fmaf(fa, c[1], sc[n][1]);
+            sc[n][2] = fmaf(fb, c[2], sc[n][2]);
+            sc[n][3] = fmaf(fb, c[3], sc[n][3]);
+        }
+    }
+    // scales of V for the same keys
+    if constexpr (kBlocks == 4) {
+        const uint2 u = *reinterpret_cast<const uint2 *>(vg + kv_scale_offset(DIM) + ka * 8);
+        const uint2 v = *reinterpret_cast<const uint2 *>(vg + kv_scale_offset(DIM) + kb * 8);
+        da[0] = u.x, da[1] = u.y, db[0] = v.x, db[1] = v.y;
+    } else {
+        da[0] = *reinterpret_cast<const uint32_t *>(vg + kv_scale_offset(DIM) + ka * 4);
+        db[0] = *reinterpret_cast<const uint32_t *>(vg + kv_scale_offset(DIM) + kb * 4);
+    }
+    bool keep[NT][4];
+    if constexpr (MASKED) {
+        // a key that no row sees may be anything: its scales are not looked at
+        const bool va = key0 + ka >= t.lo_min && key0 + ka < t.hi_max;
+        const bool vb = key0 + kb >= t.lo_min && key0 + kb < t.hi_max;
+#pragma unroll
+        for (int i = 0; i < (kBlocks + 1) / 2; ++i) da[i] = va ? da[i] : 0, db[i] = vb ? db[i] : 0;
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            sc[n][i] *= t.mul[n][i & 1];
+            if constexpr (MASKED) {
+                const int key = key0 + (i < 2 ? ka : kb);
+                keep[n][i] = key >= t.lo[n][i & 1] && key < t.hi[n][i & 1];
+                sc[n][i] = keep[n][i] ? sc[n][i] : -INFINITY;
+            }
+        }
+
+    // ---- maximum, renewed when a score or a scale passes its limit ----
+    __half2 d2 = __habs2(as_h2(da[0]));
+    d2 = __hmax2(d2, __habs2(as_h2(db[0])));
+    if constexpr (kBlocks == 4) {
+        d2 = __hmax2(d2, __habs2(as_h2(da[1])));
+        d2 = __hmax2(d2, __habs2(as_h2(db[1])));
+    }
+    float d_top = fmaxf(__low2float(d2), __high2float(d2));
+    bool past = d_top > s.d_limit;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) past |= sc[n][i] > s.m[n][i & 1] + kSlack;
+    if (__any_sync(0xffffffffu, past)) {
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) d_top = fmaxf(d_top, __shfl_xor_sync(0xffffffffu, d_top, o));
+        float keep_o = 1.0f;
+        if (d_top > s.d_limit) {
+            // |d| <= 2^e: P d sv <= 2^(kSlack + 8)
+            const int e = d_top < INFINITY ? ilogbf(d_top) + 1 : 16;
+            s.d_limit = ldexpf(1.0f, e);
+            const float sv = ldexpf(1.0f, 8 - e);
+            keep_o = sv / s.sv;
+            s.sv = sv;
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            float f[2];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                float top = fmaxf(sc[n][x], sc[n][x + 2]);
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                top = fmaxf(top, s.m[n][x]);
+                f[x] = exp2_approx(s.m[n][x] - top);
+                s.m[n][x] = top;
+                s.l[n][x] *= f[x];
+                f[x] *= keep_o;
+            }
+#pragma unroll
+            for (int j = 0; j < DIM / 16; ++j) {
+                s.o[n][j][0] *= f[0], s.o[n][j][1] *= f[1];
+                s.o[n][j][2] *= f[0], s.o[n][j][3] *= f[1];
+            }
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sc[n][i] = exp2_approx(sc[n][i] - s.m[n][i & 1]);
+        s.l[n][0] += sc[n][0] + sc[n][2];
+        s.l[n][1] += sc[n][1] + sc[n][3];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sc[n][i] *= s.sv;
+    }
+
+    // ---- O^T += V^T (d P) ----
+    // registers of V: keys q4, q4 + 4 (k = 2 q4, 2 q4 + 1) and q4 + 8, q4 + 12
+    uint32_t v[4][kBlocks / 2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (kBlocks == 4) {
+            const uint2 x = *reinterpret_cast<const uint2 *>(vg + (q4 + 4 * i) * 64 + g * 8);
+            v[i][0] = x.x, v[i][1] = x.y;
+        } else {
+            v[i][0] = *reinterpret_cast<const uint32_t *>(vg + (q4 + 4 * i) * 32 + g * 4);
+        }
+    }
+    const __half2 minus1032 = __float2half2_rn(-1032.0f), minus72 = __float2half2_rn(-72.0f),
+                  sixteenth = __float2half2_rn(0.0625f);
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b) {
+        const uint32_t sel = (b & 1) ? 0x7632u : 0x5410u;
+        const uint32_t x = __byte_perm(v[0][b / 2], v[1][b / 2], sel), y = __byte_perm(v[2][b / 2], v[3][b / 2], sel);
+        const float fa = (b & 1) ? high_half(da[b / 2]) : low_half(da[b / 2]);
+        const float fb = (b & 1) ? high_half(db[b / 2]) : low_half(db[b / 2]);
+        uint32_t p0[NT], p1[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            float w[4] = {sc[n][0] * fa, sc[n][1] * fa, sc[n][2] * fb, sc[n][3] * fb};
+            if constexpr (MASKED) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = keep[n][i] ? w[i] : 0.0f;
+            }
+            p0[n] = transpose8x8(h2(__floats2half2_rn(w[0], w[1])));
+            p1[n] = transpose8x8(h2(__floats2half2_rn(w[2], w[3])));
+        }
+        // low nibbles: 1024 + n - 1032; high ones: (1024 + 16 n) / 16 - 72
+        const auto low = [&](uint32_t z) { return h2(__hadd2(as_h2((z & 0x000F000Fu) | 0x64006400u), minus1032)); };
+        const auto high = [&](uint32_t z) {
+            return h2(__hfma2(as_h2((z & 0x00F000F0u) | 0x64006400u), sixteenth, minus72));
+        };
+        const uint32_t a0 = low(x), a1 = high(x), a2 = low(y), a3 = high(y);
+        const uint32_t x8 = x >> 8, y8 = y >> 8;
+        const uint32_t b0 = low(x8), b1 = high(x8), b2 = low(y8), b3 = high(y8);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            mma_f16(s.o[n][2 * b], a0, a1, a2, a3, p0[n], p1[n]);
+            mma_f16(s.o[n][2 * b + 1], b0, b1, b2, b3, p0[n], p1[n]);
+        }
+    }
+}
+
+// The rows of a piece that ends: to the output if the piece is the whole
+// item, else to its slot of the workspace.
+template <int DIM, int NT>
+PFNG_DEV void store_rows(const StreamParams &sp, const Cursor &c, RowSums<DIM, NT> &s, bool whole, int64_t slot) {
+    const AttnArgs &p = sp.a;
+    const int lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
+    const int group = p.heads_q / p.heads_kv;
+    const float back = 1.0f / s.sv;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            float l = s.l[n][x];
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+            const int in_tile = n * 8 + 2 * q4 + x, row = c.tile * NT * 8 + in_tile;
+            if (row >= c.shape.rows) continue;
+            const bool none = s.m[n][x] == kNoMax && l == 0.0f;
+            const int64_t token = p.cu_q[c.r] + row / group, head = static_cast<int64_t>(c.head) * group + row % group;
+            const float f = whole ? (none ? 0.0f : back / l) : back;
+#pragma unroll
+            for (int b = 0; b < DIM / 32; ++b)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float u = s.o[n][2 * b][2 * h + x] * f, w = s.o[n][2 * b + 1][2 * h + x] * f;
+                    const int dim = 32 * b + 16 * h + 2 * g;
+                    if (!whole) {
+                        *reinterpret_cast<float2 *>(sp.part_o + (slot * (8 * NT) + in_tile) * DIM + dim) =
+                            make_float2(u, w);
+                    } else {
+                        const float a[1] = {u}, z[1] = {w};
+                        const int64_t at = token * p.ldo + head * DIM + dim;
+                        store_values<1>(p.out_format, p.out, at, a);
+                        store_values<1>(p.out_format, p.out, at + 1, z);
+                    }
+                }
+            if (g == 0) {
+                if (!whole)
+                    sp.part_ml[slot * (8 * NT) + in_tile] = make_float2(s.m[n][x], l);
+                else if (p.lse)
+                    p.lse[token * p.heads_q + head] = none ? -INFINITY : (s.m[n][x] + log2f(l)) / kLog2e;
+            }
+        }
+}
+
+template <int DIM, int NT>
+__global__ void __launch_bounds__(kThreads, 1) attn_stream_kernel(const StreamParams sp) {
+    extern __shared__ __align__(128) uint8_t ring[];
+    __shared__ __align__(8) uint64_t bars[kWarps][kStages];
+    const AttnArgs &p = sp.a;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    constexpr uint32_t kHalf = (kUnit / kKvGroup) * kv_group_bytes(DIM);
+    if (lane == 0) {
+        for (int i = 0; i < kStages; ++i) mbar_init(&bars[warp][i], 1);
+        fence_mbar_init();
+    }
+    int64_t units, none0, none1;
+    line_totals<NT, kThreads>(p, 0, units, none0, none1);  // synchronises
+    pdl_trigger();
+    const int64_t workers = static_cast<int64_t>(gridDim.x) * kWarps;
+    const int64_t worker = static_cast<int64_t>(blockIdx.x) * kWarps + warp;
+    const int64_t begin = piece_start(worker, units, workers), end = piece_start(worker + 1, units, workers);
+    if (begin == end) return;
+
+    uint8_t *mine = ring + warp * kStages * 2 * kHalf;
+    const uint64_t policy = l2_policy_evict_first();
+    Cursor ahead = seek<NT>(p, begin), at = ahead;
+    int64_t fetched = begin;
+    uint32_t there[kStages];
+    const auto fetch = [&](int stage) {
+        there[stage] = fetch_unit<DIM>(p, ahead, mine + stage * 2 * kHalf, &bars[warp][stage], policy);
+        ++fetched;
+        if (++ahead.at == ahead.count) next_item<NT>(p, ahead);
+    };
+#pragma unroll
+    for (int i = 0; i < kStages; ++i)
+        if (fetched < end) fetch(i);
+
+    RowTile<DIM, NT> tile;
+    RowSums<DIM, NT> sums;
+    bool opened = false, whole = false, ok = true;
+    uint32_t phase = 0;
+    for (int64_t u = begin; u < end && ok;) {
+#pragma unroll
+        for (int stage = 0; stage < kStages; ++stage) {
+            if (u >= end || !ok) break;
+            if (!opened) {
+                load_rows<DIM, NT>(sp, at, tile);
+                clear(sums);
+                opened = true;
+                whole = at.at == 0;
+            }
+            ok = mbar_wait(&bars[warp][stage], phase, sp.err, kErrWaitFull);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            const uint8_t *k = mine + stage * 2 * kHalf, *v = k + kHalf;
+            const int key0 = (at.first + at.at) * kUnit;
+#pragma unroll 1
+            for (int i = 0; i < kUnit / kKvGroup; ++i) {
+                const int key = key0 + i * kKvGroup;
+                if (!((there[stage] >> i) & 1u) || key >= tile.hi_max || key + kKvGroup <= tile.lo_min) continue;
+                if (key >= tile.lo_max && key + kKvGroup <= tile.hi_min)
+                    attend16<DIM, NT, false>(tile, sums, k + i * kv_group_bytes(DIM), v + i * kv_group_bytes(DIM), key);
+                else
+                    attend16<DIM, NT, true>(tile, sums, k + i * kv_group_bytes(DIM), v + i * kv_group_bytes(DIM), key);
+            }
+            __syncwarp();
+            if (fetched < end) fetch(stage);
+            ++u;
+            if (++at.at == at.count || u == end) {
+                whole = whole && at.at == at.count;
+                store_rows<DIM, NT>(sp, at, sums, whole, worker + at.item);
+                opened = false;
+                if (at.at == at.count) next_item<NT>(p, at);
+            }
+        }
+        phase ^= 1;
+    }
+    if (!ok)  // copies in flight end before the CTA does
+        for (int i = 0; i < kStages; ++i) mbar_wait(&bars[warp][i], phase, sp.err, kErrWaitFull);
+}
+
+// Joins the pieces of an item: weights 2^(m_i - max m) in line order.
+constexpr int kJoinThreads = 128;
+template <int DIM, int NT>
+__global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const StreamParams sp, int64_t workers) {
+    const AttnArgs &p = sp.a;
+    const int64_t r = blockIdx.x / p.heads_kv;
+    const int head_kv = static_cast<int>(blockIdx.x % p.heads_kv);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int64_t units, before, item;
+    line_totals<NT, kJoinThreads>(p, r, units, before, item);
+    pdl_wait();
+    const RequestShape shape = request_shape<NT>(p, r);
+    const int group = p.heads_q / p.heads_kv;
+    int64_t per_head = 0;
+    for (int t = 0; t < shape.tiles; ++t) {
+        int first, count;
+        tile_units<NT>(p, shape, t, first, count);
+        per_head += count;
+    }
+    before += head_kv * per_head;
+    item += static_cast<int64_t>(head_kv) * shape.tiles;
+    for (int t = 0; t < shape.tiles; ++t, ++item) {
+        int first, count;
+        tile_units<NT>(p, shape, t, first, count);
+        const int64_t u0 = before, u1 = before + count;
+        before = u1;
+        // the worker of unit u: the last whose piece starts at or before it
+        const auto worker_of = [&](int64_t u) {
+            int64_t w = u * workers / units;
+            while (w + 1 < workers && piece_start(w + 1, units, workers) <= u) ++w;
+            while (piece_start(w, units, workers) > u) --w;
+            return w;
+        };
+        const int64_t w0 = worker_of(u0), w1 = worker_of(u1 - 1);
+        if (w0 == w1) continue;  // written by its one piece
+        for (int i = warp; i < 8 * NT; i += kJoinThreads / 32) {
+            const int row = t * 8 * NT + i;
+            if (row >= shape.rows) break;
+            float m = kNoMax;
+            for (int64_t w = w0 + lane; w <= w1; w += 32)
+                if (piece_start(w, units, workers) < piece_start(w + 1, units, workers))
+                    m = fmaxf(m, sp.part_ml[(w + item) * (8 * NT) + i].x);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            constexpr int kPer = DIM / 32;
+            float acc[kPer] = {}, l = 0.0f;
+#pragma unroll 4
+            for (int64_t w = w0; w <= w1; ++w) {
+                if (piece_start(w, units, workers) == piece_start(w + 1, units, workers)) continue;
+                const int64_t at = (w + item) * (8 * NT) + i;
+                const float2 ml = sp.part_ml[at];
+                const float f = exp2_approx(ml.x - m);
+                l += ml.y * f;
+#pragma unroll
+                for (int x = 0; x < kPer; ++x) acc[x] += f * sp.part_o[at * DIM + lane * kPer + x];
+            }
+            const bool none = m == kNoMax && l == 0.0f;
+            const float f = none ? 0.0f : 1.0f / l;
+            const int64_t token = p.cu_q[r] + row / group, head = static_cast<int64_t>(head_kv) * group + row % group;
+#pragma unroll
+            for (int x = 0; x < kPer; ++x) {
+                const float v[1] = {acc[x] * f};
+                store_values<1>(p.out_format, p.out, token * p.ldo + head * DIM + lane * kPer + x, v);
+            }
+            if (p.lse && lane == 0)
+                p.lse[token * p.heads_q + head] = none ? -INFINITY : (m + log2f(l)) / kLog2e;
+        }
+    }
+}
+
+int64_t max_rows(const AttnArgs &p) { return p.max_q * (p.heads_q / p.heads_kv); }
+int row_tiles_of_8(const AttnArgs &p) { return max_rows(p) <= 8 ? 1 : 2; }
+int64_t max_items(const AttnArgs &p) {
+    const int64_t tile = 8 * row_tiles_of_8(p);
+    return p.requests * p.heads_kv * ((max_rows(p) + tile - 1) / tile);
+}
+int64_t grid_size(const AttnArgs &) { return device_sm_count(); }
+int64_t slots(const AttnArgs &p) { return grid_size(p) * kWarps + max_items(p); }
+
+template <int DIM, int NT>
+cudaError_t launch(const StreamParams &sp, cudaStream_t s) {
+    constexpr size_t smem = static_cast<size_t>(kWarps) * kStages * 2 * (kUnit / kKvGroup) * kv_group_bytes(DIM);
+    cudaError_t e = cudaFuncSetAttribute(attn_stream_kernel<DIM, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         static_cast<int>(smem));
+    if (e != cudaSuccess) return e;
+    const int64_t grid = grid_size(sp.a);
+    attn_stream_kernel<DIM, NT><<<static_cast<unsigned>(grid), kThreads, smem, s>>>(sp);
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(sp.a.requests * sp.a.heads_kv));
+    cfg.blockDim = dim3(kJoinThreads);
+    cfg.stream = s;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, attn_join_kernel<DIM, NT>, sp, grid * kWarps);
+}
+
+}  // namespace
+
+bool attn_stream_supported(const AttnArgs &p) {
+    return (p.head_dim == 64 || p.head_dim == 128) && p.requests * p.heads_kv < 0x7fffffff;
+}
+
+size_t attn_stream_workspace(const AttnArgs &p) {
+    return static_cast<size_t>(slots(p)) * (8 * row_tiles_of_8(p)) * (p.head_dim + 2) * sizeof(float) + 256;
+}
+
+cudaError_t launch_attn_stream(const AttnArgs &p, void *workspace, int *err, cudaStream_t s) {
+    StreamParams sp{};
+    sp.a = p;
+    const int64_t rows = slots(p) * 8 * row_tiles_of_8(p);
+    sp.part_o = static_cast<float *>(workspace);
+    sp.part_ml = reinterpret_cast<float2 *>(sp.part_o + rows * p.head_dim);
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p.q);
+    sp.vec_q = p.ldq % 4 == 0 && at % (p.q_format == kOutF32 ? 16 : 8) == 0;
+    sp.err = err;
+    const bool one = row_tiles_of_8(p) == 1;
+    if (p.head_dim == 128) return one ? launch<128, 1>(sp, s) : launch<128, 2>(sp, s);
+    return one ? launch<64, 1>(sp, s) : launch<64, 2>(sp, s);
+}
+
+}  // namespace pfng

@@ -31,6 +31,19 @@ int check_attention(int64_t requests, int64_t tokens, int64_t heads_q, int64_t h
     return PFNG_B200_OK;
 }
 
+// Kernel path of a call, -1 for a forced path that cannot run it.
+int resolve_attention(const AttnArgs &a, int path) {
+    const bool stream = attn_stream_supported(a);
+    if (path == PFNG_B200_PATH_AUTO) return stream ? PFNG_B200_PATH_GEMV : PFNG_B200_PATH_SIMPLE;
+    if (path == PFNG_B200_PATH_GEMV && !stream) return -1;
+    if (path == PFNG_B200_PATH_MMA) return -1;
+    return path;
+}
+
+size_t attention_workspace(const AttnArgs &a, int resolved) {
+    return resolved == PFNG_B200_PATH_GEMV ? attn_stream_workspace(a) : 0;
+}
+
 }  // namespace
 }  // namespace pfng
 
@@ -120,7 +133,13 @@ int pfng_b200_kv_append_q4_0(const void *k, int64_t ldk, int k_format, const voi
 size_t pfng_b200_attention_q4_0_workspace_size(int64_t requests, int64_t tokens, int64_t max_q, int64_t max_kv,
                                                int64_t heads_q, int64_t heads_kv, int64_t head_dim, int path) {
     if (check_attention(requests, tokens, heads_q, heads_kv, head_dim, max_q, max_kv, path) != PFNG_B200_OK) return 0;
-    return 0;
+    if (requests == 0 || tokens == 0 || heads_q == 0 || max_q == 0) return 0;
+    AttnArgs a{};
+    a.requests = requests, a.tokens = tokens, a.max_q = max_q, a.max_kv = max_kv;
+    a.heads_q = static_cast<int>(heads_q), a.heads_kv = static_cast<int>(heads_kv);
+    a.head_dim = static_cast<int>(head_dim);
+    const int resolved = resolve_attention(a, path);
+    return resolved < 0 ? 0 : attention_workspace(a, resolved);
 }
 
 int pfng_b200_attention_q4_0(const void *q, int64_t ldq, int q_format, const void *k_cache, const void *v_cache,
@@ -134,7 +153,7 @@ int pfng_b200_attention_q4_0(const void *q, int64_t ldq, int q_format, const voi
     if (st != PFNG_B200_OK) return st;
     if (window < 0 || (window > 0 && !causal) || num_pages < 0 || max_pages < 0) return PFNG_B200_ERR_INVALID_ARGUMENT;
     if (!page_size_ok(page_size) || num_pages > kMaxCount || max_pages > kMaxCount || window > kMaxCount ||
-        max_pages * page_size > kMaxCount)
+        max_pages * page_size > (1 << 30))
         return PFNG_B200_ERR_SHAPE;
     if (tokens > 0 && (ldq < heads_q * head_dim || ldo < heads_q * head_dim)) return PFNG_B200_ERR_SHAPE;
     if (tokens == 0 || requests == 0 || heads_q == 0 || max_q == 0) return PFNG_B200_OK;
@@ -144,9 +163,6 @@ int pfng_b200_attention_q4_0(const void *q, int64_t ldq, int q_format, const voi
         !aligned(k_cache, 16) || !aligned(v_cache, 16) || !aligned(block_table, 4) || !aligned(seq_len, 4) ||
         !aligned(cu_q, 4))
         return PFNG_B200_ERR_ALIGNMENT;
-    if (path == PFNG_B200_PATH_GEMV || path == PFNG_B200_PATH_MMA) return PFNG_B200_ERR_UNSUPPORTED;
-    (void)workspace, (void)workspace_bytes;
-    if ((st = device_status()) != PFNG_B200_OK) return st;
     AttnArgs a{};
     a.q = q, a.q_format = q_format, a.ldq = ldq;
     a.out = out, a.out_format = out_format, a.ldo = ldo;
@@ -158,7 +174,15 @@ int pfng_b200_attention_q4_0(const void *q, int64_t ldq, int q_format, const voi
     a.window = window, a.page_size = static_cast<int>(page_size), a.causal = causal != 0, a.scale = scale;
     a.heads_q = static_cast<int>(heads_q), a.heads_kv = static_cast<int>(heads_kv);
     a.head_dim = static_cast<int>(head_dim);
-    return status_of(launch_attn_simple(a, static_cast<cudaStream_t>(stream)));
+    const int resolved = resolve_attention(a, path);
+    if (resolved < 0) return PFNG_B200_ERR_UNSUPPORTED;
+    if ((st = device_status()) != PFNG_B200_OK) return st;
+    const size_t need = attention_workspace(a, resolved);
+    if (need > 0 && (!workspace || workspace_bytes < need)) return PFNG_B200_ERR_WORKSPACE;
+    if (need > 0 && !aligned(workspace, 256)) return PFNG_B200_ERR_ALIGNMENT;
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (resolved == PFNG_B200_PATH_GEMV) return status_of(launch_attn_stream(a, workspace, device_error_word(), s));
+    return status_of(launch_attn_simple(a, s));
 }
 
 }  // extern "C"

@@ -185,6 +185,10 @@ struct AttnArgs {
     float scale;
 };
 cudaError_t launch_attn_simple(const AttnArgs &args, cudaStream_t s);
+// attn_stream.cu -- few query rows per key head; workspace 256-byte aligned
+bool attn_stream_supported(const AttnArgs &args);
+size_t attn_stream_workspace(const AttnArgs &args);
+cudaError_t launch_attn_stream(const AttnArgs &args, void *workspace, int *err, cudaStream_t s);
 
 // shard.cu
 cudaError_t launch_unshard_columns(const float *slices, float *c, int64_t m, int64_t n, int64_t ldc, int world,
