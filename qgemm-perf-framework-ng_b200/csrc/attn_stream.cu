@@ -25,23 +25,29 @@
 //     Q is fp16, scaled per row by a power of two so that bf16 and fp32
 //     ranges fit (bf16 and fp16 values stay exact, fp32 loses 2^-11).
 //   P = 2^(S^T - M), M per row and warp: a maximum that is renewed (with a
-//     rescale of the sums) only when a score passes it by kSlack, as P up to
-//     2^kSlack is as exact as P up to 1.  Sums of P in fp32.
+//     rescale of the sums) only when a score passes it by more than a slack, as
+//     P up to 2^kSlack is as exact as P up to 1.  Sums of P in fp32.
 //   O^T += V^T (d P)   A = n - 8 in fp16 (exact: 1024 + n minus 1032), B = d P
-//     in fp16, per block, brought from accumulator to operand layout by an
-//     8 x 8 transpose.  The rounding of d P to fp16 (2^-12 on average) is the
-//     only one between the cache and the fp32 output; a power of two that
-//     follows the largest d keeps d P in the middle of fp16's range.
+//     in fp16, per block, P brought from accumulator to operand layout by
+//     eight shuffles.  The rounding of d P to fp16 (2^-12 on average) is the
+//     only one between the cache and the fp32 output; M includes a power of two
+//     that follows the largest d and keeps d P in the middle of fp16's range.
 #include "attn.cuh"
 #include "pfng_tma.h"
 
 namespace pfng {
 namespace {
 
-constexpr int kWarps = 16;
-constexpr int kThreads = kWarps * 32;
-constexpr int kUnit = 32;    // keys of a unit: one stage of a warp's ring
-constexpr int kStages = 3;
+constexpr int kUnit = 64;    // keys of a unit: one stage of a warp's ring
+// Warps of a CTA (one CTA per SM) and stages of a warp's ring.  The rings take
+// 221 KB either way; one row tile of 8 fits 168 registers, two need 255.
+// 8 requests of 60000..100000 keys, one token: 196 us with 12 warps, 230 with
+// 8, 261 with 16 (128 registers, spills).  Three drafted tokens of 8 requests
+// of 4000..32000 keys (12 rows): 131 us with 8 warps, 184 with 12.
+template <int NT>
+struct Config {
+    static constexpr int kWarps = NT == 1 ? 12 : 8, kThreads = 32 * kWarps, kStages = NT == 1 ? 2 : 3;
+};
 constexpr float kSlack = 6.0f;
 constexpr float kNoMax = -3.0e38f;  // the maximum before the first visible key
 constexpr float kLog2e = 1.4426950408889634f;
@@ -60,20 +66,70 @@ PFNG_DEV void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-PFNG_DEV uint32_t transpose8x8(uint32_t x) {
-    uint32_t y;
-    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
-    return y;
+// (x, y) of accumulator rows g and columns 2 t, 2 t + 1 (g = lane / 4, t =
+// lane % 4) -> the values of rows 2 t and 2 t + 1, column g: accumulator to B
+// operand layout.  Lanes 8 t + g / 2 and 8 t + 4 + g / 2 have them.
+PFNG_DEV void rows_to_columns(float &x, float &y) {
+    const int lane = threadIdx.x & 31, from = 8 * (lane & 3) + (lane >> 3);
+    const bool odd = lane & 4;
+    const float x0 = __shfl_sync(0xffffffffu, x, from), y0 = __shfl_sync(0xffffffffu, y, from);
+    const float x1 = __shfl_sync(0xffffffffu, x, from + 4), y1 = __shfl_sync(0xffffffffu, y, from + 4);
+    x = odd ? y0 : x0;
+    y = odd ? y1 : x1;
 }
 PFNG_DEV float exp2_approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// Loads from shared memory at a 32-bit address plus a constant.
+PFNG_DEV uint32_t lds32(uint32_t at) {
+    uint32_t x;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(x) : "r"(at));
+    return x;
+}
+PFNG_DEV uint2 lds64(uint32_t at) {
+    uint2 x;
+    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(x.x), "=r"(x.y) : "r"(at));
+    return x;
+}
+PFNG_DEV uint4 lds128(uint32_t at) {
+    uint4 x;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(at));
+    return x;
+}
+// (x & MASK) | y in one instruction: y has to be a register (with a literal in
+// its place the compiler spends two).
+template <uint32_t MASK>
+PFNG_DEV uint32_t and_or(uint32_t x, uint32_t y) {
+    uint32_t z;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(z) : "r"(x), "n"(MASK), "r"(y));
+    return z;
+}
+// Larger magnitude per half (with a sign that does not matter).
+PFNG_DEV uint32_t larger(uint32_t x, uint32_t y) {
+    uint32_t z;
+    asm("max.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(z) : "r"(x), "r"(y));
+    return z;
+}
 PFNG_DEV uint32_t h2(__half2 x) { return *reinterpret_cast<uint32_t *>(&x); }
 PFNG_DEV __half2 as_h2(uint32_t x) { return *reinterpret_cast<__half2 *>(&x); }
-PFNG_DEV float low_half(uint32_t x) { return __low2float(as_h2(x)); }
-PFNG_DEV float high_half(uint32_t x) { return __high2float(as_h2(x)); }
+// fp16 halves of a register as fp32.  As a mixed-precision add, which runs at
+// the FMA rate; a conversion instruction takes twice the issue time.
+PFNG_DEV float low_half(uint32_t x) {
+    float y;
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tadd.f32.f16 %0, l, %2;\n\t}" : "=f"(y) : "r"(x), "f"(0.0f));
+    return y;
+}
+PFNG_DEV float high_half(uint32_t x) {
+    float y;
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tadd.f32.f16 %0, h, %2;\n\t}" : "=f"(y) : "r"(x), "f"(0.0f));
+    return y;
+}
+// floor(log2 x) of a positive finite x (at least -126), and 2^e for e in
+// [-126, 127]
+PFNG_DEV int exponent_of(float x) { return max(static_cast<int>(__float_as_uint(x) >> 23) - 127, -126); }
+PFNG_DEV float power_of_two(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
 
 // What a request contributes to the line: its row tiles and, per row tile,
 // the units that its rows see (at least one, so that rows without a key are
@@ -134,7 +190,17 @@ PFNG_DEV void line_totals(const AttnArgs &p, int64_t r, int64_t &units, int64_t 
     for (int w = 0; w < THREADS / 32; ++w) units += sums[w][0], units_before += sums[w][1], items_before += sums[w][2];
 }
 
-PFNG_DEV int64_t piece_start(int64_t worker, int64_t units, int64_t workers) { return worker * units / workers; }
+// The line cut into `workers` pieces of each or each + 1 units, the longer
+// ones first.
+struct Pieces {
+    int64_t each, more;  // units of a piece; pieces with one unit more
+    PFNG_DEV Pieces(int64_t units, int64_t workers) : each(units / workers), more(units - each * workers) {}
+    PFNG_DEV int64_t start(int64_t w) const { return w * each + min(w, more); }
+    PFNG_DEV int64_t worker_of(int64_t u) const {
+        const int64_t w = u / (each + 1);
+        return w < more ? w : more + (u - more * (each + 1)) / each;
+    }
+};
 
 // Position of a warp on the line.
 struct Cursor {
@@ -287,8 +353,8 @@ PFNG_DEV void load_rows(const StreamParams &sp, const Cursor &c, RowTile<DIM, NT
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         // largest value into [2^13, 2^14): exact, and room for the 1/16
         int e = 0;
-        if (top > 0.0f && top < INFINITY) e = ilogbf(top) - 13;
-        const float up0 = ldexpf(1.0f, -(e / 2)), up1 = ldexpf(1.0f, -(e - e / 2));
+        if (top > 0.0f && top < INFINITY) e = exponent_of(top) - 13;
+        const float up0 = power_of_two(-(e / 2)), up1 = power_of_two(-(e - e / 2));
         float sum[DIM / 32];
 #pragma unroll
         for (int b = 0; b < DIM / 32; ++b) {
@@ -310,7 +376,7 @@ PFNG_DEV void load_rows(const StreamParams &sp, const Cursor &c, RowTile<DIM, NT
             sum[b] += __shfl_xor_sync(0xffffffffu, sum[b], 1);
             sum[b] += __shfl_xor_sync(0xffffffffu, sum[b], 2);
         }
-        const float mul = ldexpf(p.scale * kLog2e, e + 24);
+        const float mul = p.scale * kLog2e * power_of_two((e + 24) / 2) * power_of_two(e + 24 - (e + 24) / 2);
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
             const int from = (2 * q4 + x) * 4;  // a lane that loaded row 2 q4 + x
@@ -342,9 +408,8 @@ template <int DIM, int NT>
 struct RowSums {
     float o[NT][DIM / 16][4];  // O^T tiles: rows = 16 dimensions, columns = query rows
     float l[NT][2];            // sums of P over this thread's keys
-    float m[NT][2];
-    float sv;                  // power of two that P d carries
-    float d_limit;             // largest |d| that sv takes
+    float m[NT][2];            // P = 2^(score - m)
+    float limit, d_limit;      // scores up to m + limit and scales up to d_limit in magnitude need no new m
 };
 template <int DIM, int NT>
 PFNG_DEV void clear(RowSums<DIM, NT> &s) {
@@ -355,7 +420,7 @@ PFNG_DEV void clear(RowSums<DIM, NT> &s) {
         s.l[n][0] = s.l[n][1] = 0.0f;
         s.m[n][0] = s.m[n][1] = kNoMax;
     }
-    s.sv = 1.0f;
+    s.limit = kSlack;
     s.d_limit = 0.0f;
 }
 
@@ -364,34 +429,31 @@ PFNG_DEV void clear(RowSums<DIM, NT> &s) {
 // a warp read neighbouring rows of shared memory.
 PFNG_DEV int key_of_row(int r) { return (r & 8) | ((r & 7) >> 1) | ((r & 1) << 2); }
 
-// 16 keys: key0 is the first one's number, `kg` / `vg` their groups.
+// 16 keys: key0 is the first one's number, kg and vg the shared addresses of
+// their groups; MASKED: some row does not see all of them.  magic: 0x64006400,
+// 1024 in both halves.
 template <int DIM, int NT, bool MASKED>
-PFNG_DEV void attend16(const RowTile<DIM, NT> &t, RowSums<DIM, NT> &s, const uint8_t *kg, const uint8_t *vg,
-                       int key0) {
-    constexpr int kBlocks = DIM / 32;
+PFNG_DEV void attend16(const RowTile<DIM, NT> &t, RowSums<DIM, NT> &s, uint32_t kg, uint32_t vg, int key0,
+                       uint32_t magic) {
+    constexpr int kBlocks = DIM / 32, kRow = DIM / 2, kScaleRow = DIM / 16, kScales = kv_scale_offset(DIM);
     const int lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
     const int ka = key_of_row(g), kb = ka + 8;  // this thread's keys (accumulator rows g and g + 8)
 
     // ---- scores ----
-    uint32_t wa[kBlocks], wb[kBlocks], da[(kBlocks + 1) / 2], db[(kBlocks + 1) / 2];
+    uint32_t wa[kBlocks], wb[kBlocks], da[kBlocks / 2], db[kBlocks / 2];
+    const uint32_t kw = kg + ka * kRow + q4 * 4 * kBlocks, ks = kg + ka * kScaleRow;
     if constexpr (kBlocks == 4) {
-        const uint4 x = *reinterpret_cast<const uint4 *>(kg + ka * 64 + q4 * 16);
-        const uint4 y = *reinterpret_cast<const uint4 *>(kg + kb * 64 + q4 * 16);
+        const uint4 x = lds128(kw), y = lds128(kw + 8 * kRow);
         wa[0] = x.x, wa[1] = x.y, wa[2] = x.z, wa[3] = x.w;
         wb[0] = y.x, wb[1] = y.y, wb[2] = y.z, wb[3] = y.w;
-        const uint2 u = *reinterpret_cast<const uint2 *>(kg + kv_scale_offset(DIM) + ka * 8);
-        const uint2 v = *reinterpret_cast<const uint2 *>(kg + kv_scale_offset(DIM) + kb * 8);
+        const uint2 u = lds64(ks + kScales), v = lds64(ks + kScales + 8 * kScaleRow);
         da[0] = u.x, da[1] = u.y, db[0] = v.x, db[1] = v.y;
     } else {
-        const uint2 x = *reinterpret_cast<const uint2 *>(kg + ka * 32 + q4 * 8);
-        const uint2 y = *reinterpret_cast<const uint2 *>(kg + kb * 32 + q4 * 8);
+        const uint2 x = lds64(kw), y = lds64(kw + 8 * kRow);
         wa[0] = x.x, wa[1] = x.y, wb[0] = y.x, wb[1] = y.y;
-        da[0] = *reinterpret_cast<const uint32_t *>(kg + kv_scale_offset(DIM) + ka * 4);
-        db[0] = *reinterpret_cast<const uint32_t *>(kg + kv_scale_offset(DIM) + kb * 4);
+        da[0] = lds32(ks + kScales), db[0] = lds32(ks + kScales + 8 * kScaleRow);
     }
-    float sc[NT][4];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.0f;
+    float sc[NT][4] = {};
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b) {
         const uint32_t a8 = wa[b] >> 8, b8 = wb[b] >> 8;
@@ -399,70 +461,73 @@ PFNG_DEV void attend16(const RowTile<DIM, NT> &t, RowSums<DIM, NT> &s, const uin
         const float fb = (b & 1) ? high_half(db[b / 2]) : low_half(db[b / 2]);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            float c[4] = {t.start[n][b][0], t.start[n][b][1], t.start[n][b][0], t.start[n][b][1]};
+            float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             mma_f16(c, wa[b] & 0x000F000Fu, wb[b] & 0x000F000Fu, a8 & 0x000F000Fu, b8 & 0x000F000Fu, t.q[n][b][0],
                     t.q[n][b][1]);
             mma_f16(c, wa[b] & 0x00F000F0u, wb[b] & 0x00F000F0u, a8 & 0x00F000F0u, b8 & 0x00F000F0u, t.q[n][b][2],
                     t.q[n][b][3]);
-            sc[n][0] = fmaf(fa, c[0], sc[n][0]);
-            sc[n][1] = fmaf(fa, c[1], sc[n][1]);
-            sc[n][2] = fmaf(fb, c[2], sc[n][2]);
-            sc[n][3] = fmaf(fb, c[3], sc[n][3]);
+            sc[n][0] = fmaf(fa, c[0] + t.start[n][b][0], sc[n][0]);
+            sc[n][1] = fmaf(fa, c[1] + t.start[n][b][1], sc[n][1]);
+            sc[n][2] = fmaf(fb, c[2] + t.start[n][b][0], sc[n][2]);
+            sc[n][3] = fmaf(fb, c[3] + t.start[n][b][1], sc[n][3]);
         }
     }
-    // scales of V for the same keys
-    if constexpr (kBlocks == 4) {
-        const uint2 u = *reinterpret_cast<const uint2 *>(vg + kv_scale_offset(DIM) + ka * 8);
-        const uint2 v = *reinterpret_cast<const uint2 *>(vg + kv_scale_offset(DIM) + kb * 8);
-        da[0] = u.x, da[1] = u.y, db[0] = v.x, db[1] = v.y;
-    } else {
-        da[0] = *reinterpret_cast<const uint32_t *>(vg + kv_scale_offset(DIM) + ka * 4);
-        db[0] = *reinterpret_cast<const uint32_t *>(vg + kv_scale_offset(DIM) + kb * 4);
+    // V: this thread's keys are q4 + 4 i (operand rows 2 q4, 2 q4 + 1, + 8, + 9)
+    uint32_t v[4][kBlocks / 2], dv[4][kBlocks / 2];
+    const uint32_t vw = vg + q4 * kRow + g * 2 * kBlocks, vs = vg + q4 * kScaleRow;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (kBlocks == 4) {
+            const uint2 x = lds64(vw + 4 * i * kRow), y = lds64(vs + kScales + 4 * i * kScaleRow);
+            v[i][0] = x.x, v[i][1] = x.y, dv[i][0] = y.x, dv[i][1] = y.y;
+        } else {
+            v[i][0] = lds32(vw + 4 * i * kRow), dv[i][0] = lds32(vs + kScales + 4 * i * kScaleRow);
+        }
     }
-    bool keep[NT][4];
     if constexpr (MASKED) {
-        // a key that no row sees may be anything: its scales are not looked at
-        const bool va = key0 + ka >= t.lo_min && key0 + ka < t.hi_max;
-        const bool vb = key0 + kb >= t.lo_min && key0 + kb < t.hi_max;
 #pragma unroll
-        for (int i = 0; i < (kBlocks + 1) / 2; ++i) da[i] = va ? da[i] : 0, db[i] = vb ? db[i] : 0;
-    }
+        for (int i = 0; i < 4; ++i) {  // a key that no row sees may be anything: its scales are not looked at
+            const int key = key0 + q4 + 4 * i;
+            const bool seen = key >= t.lo_min && key < t.hi_max;
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            sc[n][i] *= t.mul[n][i & 1];
-            if constexpr (MASKED) {
-                const int key = key0 + (i < 2 ? ka : kb);
-                keep[n][i] = key >= t.lo[n][i & 1] && key < t.hi[n][i & 1];
-                sc[n][i] = keep[n][i] ? sc[n][i] : -INFINITY;
-            }
+            for (int j = 0; j < kBlocks / 2; ++j) dv[i][j] = seen ? dv[i][j] : 0;
         }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int key = key0 + (i < 2 ? ka : kb);
+                sc[n][i] = key >= t.lo[n][i & 1] && key < t.hi[n][i & 1] ? sc[n][i] * t.mul[n][i & 1] : -INFINITY;
+            }
+    } else {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sc[n][i] *= t.mul[n][i & 1];
+    }
 
     // ---- maximum, renewed when a score or a scale passes its limit ----
-    __half2 d2 = __habs2(as_h2(da[0]));
-    d2 = __hmax2(d2, __habs2(as_h2(db[0])));
+    uint32_t d2 = larger(dv[0][0], dv[1][0]);
+    d2 = larger(larger(d2, dv[2][0]), dv[3][0]);
     if constexpr (kBlocks == 4) {
-        d2 = __hmax2(d2, __habs2(as_h2(da[1])));
-        d2 = __hmax2(d2, __habs2(as_h2(db[1])));
+        d2 = larger(larger(d2, dv[0][1]), dv[1][1]);
+        d2 = larger(larger(d2, dv[2][1]), dv[3][1]);
     }
-    float d_top = fmaxf(__low2float(d2), __high2float(d2));
-    bool past = d_top > s.d_limit;
+    float over = sc[0][0] - s.m[0][0];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) past |= sc[n][i] > s.m[n][i & 1] + kSlack;
-    if (__any_sync(0xffffffffu, past)) {
+        for (int i = 0; i < 4; ++i) over = fmaxf(over, sc[n][i] - s.m[n][i & 1]);
+    float d_top = fmaxf(fabsf(low_half(d2)), fabsf(high_half(d2)));
+    if (__any_sync(0xffffffffu, over > s.limit || d_top > s.d_limit)) {
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) d_top = fmaxf(d_top, __shfl_xor_sync(0xffffffffu, d_top, o));
-        float keep_o = 1.0f;
+        float up = s.limit - kSlack;  // log2 of the power of two that P carries
         if (d_top > s.d_limit) {
-            // |d| <= 2^e: P d sv <= 2^(kSlack + 8)
-            const int e = d_top < INFINITY ? ilogbf(d_top) + 1 : 16;
-            s.d_limit = ldexpf(1.0f, e);
-            const float sv = ldexpf(1.0f, 8 - e);
-            keep_o = sv / s.sv;
-            s.sv = sv;
+            const int e = d_top < INFINITY ? exponent_of(d_top) + 1 : 16;  // |d| <= 2^e
+            s.d_limit = power_of_two(e);
+            up = static_cast<float>(8 - e);
+            s.limit = up + kSlack;
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -472,11 +537,10 @@ PFNG_DEV void attend16(const RowTile<DIM, NT> &t, RowSums<DIM, NT> &s, const uin
                 float top = fmaxf(sc[n][x], sc[n][x + 2]);
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                top = fmaxf(top, s.m[n][x]);
+                top = fmaxf(top - up, s.m[n][x]);
                 f[x] = exp2_approx(s.m[n][x] - top);
                 s.m[n][x] = top;
                 s.l[n][x] *= f[x];
-                f[x] *= keep_o;
             }
 #pragma unroll
             for (int j = 0; j < DIM / 16; ++j) {
@@ -491,21 +555,14 @@ PFNG_DEV void attend16(const RowTile<DIM, NT> &t, RowSums<DIM, NT> &s, const uin
         for (int i = 0; i < 4; ++i) sc[n][i] = exp2_approx(sc[n][i] - s.m[n][i & 1]);
         s.l[n][0] += sc[n][0] + sc[n][2];
         s.l[n][1] += sc[n][1] + sc[n][3];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sc[n][i] *= s.sv;
     }
 
     // ---- O^T += V^T (d P) ----
-    // registers of V: keys q4, q4 + 4 (k = 2 q4, 2 q4 + 1) and q4 + 8, q4 + 12
-    uint32_t v[4][kBlocks / 2];
+    // P of this thread's four keys, query row g
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if constexpr (kBlocks == 4) {
-            const uint2 x = *reinterpret_cast<const uint2 *>(vg + (q4 + 4 * i) * 64 + g * 8);
-            v[i][0] = x.x, v[i][1] = x.y;
-        } else {
-            v[i][0] = *reinterpret_cast<const uint32_t *>(vg + (q4 + 4 * i) * 32 + g * 4);
-        }
+    for (int n = 0; n < NT; ++n) {
+        rows_to_columns(sc[n][0], sc[n][1]);
+        rows_to_columns(sc[n][2], sc[n][3]);
     }
     const __half2 minus1032 = __float2half2_rn(-1032.0f), minus72 = __float2half2_rn(-72.0f),
                   sixteenth = __float2half2_rn(0.0625f);
@@ -513,26 +570,29 @@ PFNG_DEV void attend16(const RowTile<DIM, NT> &t, RowSums<DIM, NT> &s, const uin
     for (int b = 0; b < kBlocks; ++b) {
         const uint32_t sel = (b & 1) ? 0x7632u : 0x5410u;
         const uint32_t x = __byte_perm(v[0][b / 2], v[1][b / 2], sel), y = __byte_perm(v[2][b / 2], v[3][b / 2], sel);
-        const float fa = (b & 1) ? high_half(da[b / 2]) : low_half(da[b / 2]);
-        const float fb = (b & 1) ? high_half(db[b / 2]) : low_half(db[b / 2]);
+        float d[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) d[i] = (b & 1) ? high_half(dv[i][b / 2]) : low_half(dv[i][b / 2]);
         uint32_t p0[NT], p1[NT];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            float w[4] = {sc[n][0] * fa, sc[n][1] * fa, sc[n][2] * fb, sc[n][3] * fb};
-            if constexpr (MASKED) {
+            float w[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] = keep[n][i] ? w[i] : 0.0f;
+            for (int i = 0; i < 4; ++i) w[i] = sc[n][i] * d[i];
+            if constexpr (MASKED) {  // 0 times an infinite scale is 0 where the row does not see the key
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = sc[n][i] == 0.0f ? 0.0f : w[i];
             }
-            p0[n] = transpose8x8(h2(__floats2half2_rn(w[0], w[1])));
-            p1[n] = transpose8x8(h2(__floats2half2_rn(w[2], w[3])));
+            p0[n] = h2(__floats2half2_rn(w[0], w[1]));
+            p1[n] = h2(__floats2half2_rn(w[2], w[3]));
         }
         // low nibbles: 1024 + n - 1032; high ones: (1024 + 16 n) / 16 - 72
-        const auto low = [&](uint32_t z) { return h2(__hadd2(as_h2((z & 0x000F000Fu) | 0x64006400u), minus1032)); };
+        const auto low = [&](uint32_t z) { return h2(__hadd2(as_h2(and_or<0x000F000Fu>(z, magic)), minus1032)); };
         const auto high = [&](uint32_t z) {
-            return h2(__hfma2(as_h2((z & 0x00F000F0u) | 0x64006400u), sixteenth, minus72));
+            return h2(__hfma2(as_h2(and_or<0x00F000F0u>(z, magic)), sixteenth, minus72));
         };
-        const uint32_t a0 = low(x), a1 = high(x), a2 = low(y), a3 = high(y);
         const uint32_t x8 = x >> 8, y8 = y >> 8;
+        const uint32_t a0 = low(x), a1 = high(x), a2 = low(y), a3 = high(y);
         const uint32_t b0 = low(x8), b1 = high(x8), b2 = low(y8), b3 = high(y8);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -549,7 +609,6 @@ PFNG_DEV void store_rows(const StreamParams &sp, const Cursor &c, RowSums<DIM, N
     const AttnArgs &p = sp.a;
     const int lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
     const int group = p.heads_q / p.heads_kv;
-    const float back = 1.0f / s.sv;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -561,7 +620,7 @@ PFNG_DEV void store_rows(const StreamParams &sp, const Cursor &c, RowSums<DIM, N
             if (row >= c.shape.rows) continue;
             const bool none = s.m[n][x] == kNoMax && l == 0.0f;
             const int64_t token = p.cu_q[c.r] + row / group, head = static_cast<int64_t>(c.head) * group + row % group;
-            const float f = whole ? (none ? 0.0f : back / l) : back;
+            const float f = !whole ? 1.0f : none ? 0.0f : 1.0f / l;
 #pragma unroll
             for (int b = 0; b < DIM / 32; ++b)
 #pragma unroll
@@ -588,7 +647,8 @@ PFNG_DEV void store_rows(const StreamParams &sp, const Cursor &c, RowSums<DIM, N
 }
 
 template <int DIM, int NT>
-__global__ void __launch_bounds__(kThreads, 1) attn_stream_kernel(const StreamParams sp) {
+__global__ void __launch_bounds__(Config<NT>::kThreads, 1) attn_stream_kernel(const StreamParams sp) {
+    constexpr int kWarps = Config<NT>::kWarps, kThreads = Config<NT>::kThreads, kStages = Config<NT>::kStages;
     extern __shared__ __align__(128) uint8_t ring[];
     __shared__ __align__(8) uint64_t bars[kWarps][kStages];
     const AttnArgs &p = sp.a;
@@ -602,66 +662,67 @@ __global__ void __launch_bounds__(kThreads, 1) attn_stream_kernel(const StreamPa
     line_totals<NT, kThreads>(p, 0, units, none0, none1);  // synchronises
     pdl_trigger();
     const int64_t workers = static_cast<int64_t>(gridDim.x) * kWarps;
-    const int64_t worker = static_cast<int64_t>(blockIdx.x) * kWarps + warp;
-    const int64_t begin = piece_start(worker, units, workers), end = piece_start(worker + 1, units, workers);
+    // a short line goes to the first warp of every SM, then to the second
+    const int64_t worker = static_cast<int64_t>(warp) * gridDim.x + blockIdx.x;
+    const Pieces pieces(units, workers);
+    const int64_t begin = pieces.start(worker), end = pieces.start(worker + 1);
     if (begin == end) return;
 
     uint8_t *mine = ring + warp * kStages * 2 * kHalf;
     const uint64_t policy = l2_policy_evict_first();
+    constexpr int kGroups = kUnit / kKvGroup;
+    constexpr uint32_t kGroupMask = (1u << kGroups) - 1;
     Cursor ahead = seek<NT>(p, begin), at = ahead;
     int64_t fetched = begin;
-    uint32_t there[kStages];
-    const auto fetch = [&](int stage) {
-        there[stage] = fetch_unit<DIM>(p, ahead, mine + stage * 2 * kHalf, &bars[warp][stage], policy);
-        ++fetched;
-        if (++ahead.at == ahead.count) next_item<NT>(p, ahead);
-    };
-#pragma unroll
-    for (int i = 0; i < kStages; ++i)
-        if (fetched < end) fetch(i);
+    int fetch_stage = 0, stage = 0;
+    uint32_t there = 0, phase = 0;  // groups present: kGroups bits a stage
 
     RowTile<DIM, NT> tile;
     RowSums<DIM, NT> sums;
     bool opened = false, whole = false, ok = true;
-    uint32_t phase = 0;
-    for (int64_t u = begin; u < end && ok;) {
-#pragma unroll
-        for (int stage = 0; stage < kStages; ++stage) {
-            if (u >= end || !ok) break;
-            if (!opened) {
-                load_rows<DIM, NT>(sp, at, tile);
-                clear(sums);
-                opened = true;
-                whole = at.at == 0;
-            }
-            ok = mbar_wait(&bars[warp][stage], phase, sp.err, kErrWaitFull);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            const uint8_t *k = mine + stage * 2 * kHalf, *v = k + kHalf;
-            const int key0 = (at.first + at.at) * kUnit;
+    uint32_t magic;
+    asm volatile("mov.b32 %0, 0x64006400;" : "=r"(magic));
 #pragma unroll 1
-            for (int i = 0; i < kUnit / kKvGroup; ++i) {
-                const int key = key0 + i * kKvGroup;
-                if (!((there[stage] >> i) & 1u) || key >= tile.hi_max || key + kKvGroup <= tile.lo_min) continue;
-                if (key >= tile.lo_max && key + kKvGroup <= tile.hi_min)
-                    attend16<DIM, NT, false>(tile, sums, k + i * kv_group_bytes(DIM), v + i * kv_group_bytes(DIM), key);
-                else
-                    attend16<DIM, NT, true>(tile, sums, k + i * kv_group_bytes(DIM), v + i * kv_group_bytes(DIM), key);
-            }
-            __syncwarp();
-            if (fetched < end) fetch(stage);
-            ++u;
-            if (++at.at == at.count || u == end) {
-                whole = whole && at.at == at.count;
-                store_rows<DIM, NT>(sp, at, sums, whole, worker + at.item);
-                opened = false;
-                if (at.at == at.count) next_item<NT>(p, at);
-            }
+    for (int64_t u = begin; u < end; ++u) {
+#pragma unroll 1
+        while (fetched < end && fetched < u + kStages) {
+            const uint32_t bits = fetch_unit<DIM>(p, ahead, mine + fetch_stage * 2 * kHalf, &bars[warp][fetch_stage], policy);
+            there = (there & ~(kGroupMask << (kGroups * fetch_stage))) | bits << (kGroups * fetch_stage);
+            ++fetched;
+            if (++fetch_stage == kStages) fetch_stage = 0;
+            if (++ahead.at == ahead.count) next_item<NT>(p, ahead);
         }
-        phase ^= 1;
+        if (!opened) {
+            load_rows<DIM, NT>(sp, at, tile);
+            clear(sums);
+            opened = true;
+            whole = at.at == 0;
+        }
+        ok = mbar_wait(&bars[warp][stage], phase, sp.err, kErrWaitFull);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const uint32_t k = smem_u32(mine) + stage * 2 * kHalf, v = k + kHalf;
+        const int key0 = (at.first + at.at) * kUnit;
+#pragma unroll 1
+        for (int i = 0; i < kGroups; ++i) {
+            const int key = key0 + i * kKvGroup;
+            if (!((there >> (kGroups * stage + i)) & 1u) || key >= tile.hi_max || key + kKvGroup <= tile.lo_min) continue;
+            if (key >= tile.lo_max && key + kKvGroup <= tile.hi_min)
+                attend16<DIM, NT, false>(tile, sums, k + i * kv_group_bytes(DIM), v + i * kv_group_bytes(DIM), key, magic);
+            else
+                attend16<DIM, NT, true>(tile, sums, k + i * kv_group_bytes(DIM), v + i * kv_group_bytes(DIM), key, magic);
+        }
+        __syncwarp();
+        if (++stage == kStages) stage = 0, phase ^= 1;
+        if (++at.at == at.count || u + 1 == end) {
+            whole = whole && at.at == at.count;
+            store_rows<DIM, NT>(sp, at, sums, whole, worker + at.item);
+            opened = false;
+            if (at.at == at.count) next_item<NT>(p, at);
+        }
     }
     if (!ok)  // copies in flight end before the CTA does
-        for (int i = 0; i < kStages; ++i) mbar_wait(&bars[warp][i], phase, sp.err, kErrWaitFull);
+        for (int i = 0; i < kStages; ++i) mbar_wait(&bars[warp][i], i >= stage ? phase : phase ^ 1, sp.err, kErrWaitFull);
 }
 
 // Joins the pieces of an item: weights 2^(m_i - max m) in line order.
@@ -674,6 +735,7 @@ __global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const StreamPar
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int64_t units, before, item;
     line_totals<NT, kJoinThreads>(p, r, units, before, item);
+    const Pieces pieces(units, workers);
     pdl_wait();
     const RequestShape shape = request_shape<NT>(p, r);
     const int group = p.heads_q / p.heads_kv;
@@ -690,29 +752,20 @@ __global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const StreamPar
         tile_units<NT>(p, shape, t, first, count);
         const int64_t u0 = before, u1 = before + count;
         before = u1;
-        // the worker of unit u: the last whose piece starts at or before it
-        const auto worker_of = [&](int64_t u) {
-            int64_t w = u * workers / units;
-            while (w + 1 < workers && piece_start(w + 1, units, workers) <= u) ++w;
-            while (piece_start(w, units, workers) > u) --w;
-            return w;
-        };
-        const int64_t w0 = worker_of(u0), w1 = worker_of(u1 - 1);
+        const int64_t w0 = pieces.worker_of(u0), w1 = pieces.worker_of(u1 - 1);
         if (w0 == w1) continue;  // written by its one piece
         for (int i = warp; i < 8 * NT; i += kJoinThreads / 32) {
             const int row = t * 8 * NT + i;
             if (row >= shape.rows) break;
             float m = kNoMax;
             for (int64_t w = w0 + lane; w <= w1; w += 32)
-                if (piece_start(w, units, workers) < piece_start(w + 1, units, workers))
-                    m = fmaxf(m, sp.part_ml[(w + item) * (8 * NT) + i].x);
+                m = fmaxf(m, sp.part_ml[(w + item) * (8 * NT) + i].x);
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
             constexpr int kPer = DIM / 32;
             float acc[kPer] = {}, l = 0.0f;
 #pragma unroll 4
             for (int64_t w = w0; w <= w1; ++w) {
-                if (piece_start(w, units, workers) == piece_start(w + 1, units, workers)) continue;
                 const int64_t at = (w + item) * (8 * NT) + i;
                 const float2 ml = sp.part_ml[at];
                 const float f = exp2_approx(ml.x - m);
@@ -741,16 +794,19 @@ int64_t max_items(const AttnArgs &p) {
     return p.requests * p.heads_kv * ((max_rows(p) + tile - 1) / tile);
 }
 int64_t grid_size(const AttnArgs &) { return device_sm_count(); }
-int64_t slots(const AttnArgs &p) { return grid_size(p) * kWarps + max_items(p); }
+int64_t workers(const AttnArgs &p) {
+    return grid_size(p) * (row_tiles_of_8(p) == 1 ? Config<1>::kWarps : Config<2>::kWarps);
+}
+int64_t slots(const AttnArgs &p) { return workers(p) + max_items(p); }
 
 template <int DIM, int NT>
 cudaError_t launch(const StreamParams &sp, cudaStream_t s) {
-    constexpr size_t smem = static_cast<size_t>(kWarps) * kStages * 2 * (kUnit / kKvGroup) * kv_group_bytes(DIM);
+    constexpr size_t smem = static_cast<size_t>(Config<NT>::kWarps) * Config<NT>::kStages * 2 * (kUnit / kKvGroup) * kv_group_bytes(DIM);
     cudaError_t e = cudaFuncSetAttribute(attn_stream_kernel<DIM, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          static_cast<int>(smem));
     if (e != cudaSuccess) return e;
     const int64_t grid = grid_size(sp.a);
-    attn_stream_kernel<DIM, NT><<<static_cast<unsigned>(grid), kThreads, smem, s>>>(sp);
+    attn_stream_kernel<DIM, NT><<<static_cast<unsigned>(grid), Config<NT>::kThreads, smem, s>>>(sp);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(sp.a.requests * sp.a.heads_kv));
@@ -761,7 +817,7 @@ cudaError_t launch(const StreamParams &sp, cudaStream_t s) {
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, attn_join_kernel<DIM, NT>, sp, grid * kWarps);
+    return cudaLaunchKernelEx(&cfg, attn_join_kernel<DIM, NT>, sp, workers(sp.a));
 }
 
 }  // namespace
