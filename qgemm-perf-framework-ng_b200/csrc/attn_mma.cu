@@ -1,0 +1,633 @@
+// attn_mma.cu -- attention over the q4_0 cache on the 5th-generation tensor
+// cores, for many query rows per key head: prompts and chunks of prompts
+// (pfng_b200_attention_q4_0, PFNG_B200_PATH_MMA).
+//
+// A CTA takes 256 query rows (new tokens x query heads of one key head, as
+// two tiles of 128) and walks the keys that they see in tiles of 128:
+//   S_i = Q_i K^T          tcgen05.mma, both operands in shared memory, S in TMEM
+//   P_i = 2^(S_i - m)      one thread per row: TMEM -> registers -> TMEM (fp16)
+//   O_i += P_i V           tcgen05.mma, P from TMEM, V from shared memory
+// for i = 0, 1 in turn, so that the tensor cores work on one tile while the
+// other's softmax runs.  Roles (512 threads, one CTA per SM):
+//   warps 0-7    softmax, a warpgroup per row tile; they load Q, rescale O
+//                and write the output
+//   warps 8-11   dequantization: nibbles and scales of a tile -> fp16 operand
+//                rows in the 128-byte swizzled layout
+//   warp 12      issues the MMAs (one thread)
+//   warp 13      copies the tiles' groups from the pages (bulk copies, a ring
+//                of three raw K or V tiles)
+// One dequantization serves 256 rows: 13 instructions per 8 values, a fifth of
+// the issue slots that the exponentials leave.  Bound: 16 exponentials per
+// cycle and SM (2048 cycles for 256 x 128) and as many cycles of MMA.
+//
+// Precision: d (n - 8) is rounded to fp16 (2^-12 on average), P to fp16 with
+// the row's largest at 2^8..2^15 (so that small ones stay normal numbers);
+// S, the row maxima and sums and O are fp32.  Q is fp16, scaled per row by a
+// power of two (bf16 and fp16 values stay exact).  A row's reference m moves
+// only when a score passes it by kSlack, and then O is rescaled in TMEM.
+//
+// The order of a head's dimensions within the operands is the order in which
+// a cache row's words unpack (8 values a word); Q is stored in the same order,
+// and the output is written back through the inverse of V's.
+#include "attn.cuh"
+#include "pfng_tc.cuh"
+#include "pfng_tma.h"
+
+namespace pfng {
+namespace {
+
+constexpr int kTile = 128;       // rows of a row tile, keys of a key tile
+constexpr int kRows = 2 * kTile;
+constexpr int kThreads = 512;
+constexpr int kRawSlots = 3;
+constexpr int kInfoSlots = 8;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNoMax = -3.0e38f;
+constexpr float kLift = 8.0f;    // log2 of P at a renewed maximum
+constexpr float kSlack = 7.0f;   // a score may pass the maximum by this before it is renewed
+constexpr uint32_t kTmemCols = 512;  // S0 S1 (P over S) at 0 and 128, O0 O1 at 256 and 384
+
+// What the softmax needs to know about a key tile beyond its numbers.
+struct TileInfo {
+    uint32_t groups;  // bit g: keys 16 g .. of the tile are on a page of the cache
+    uint32_t bad[4];  // keys whose V scale is not finite (their V operand is zero)
+};
+
+template <int DIM>
+struct Layout {
+    static constexpr uint32_t kOperand = kTile * DIM * 2;  // an operand tile, fp16
+    static constexpr uint32_t kRaw = (kTile / kKvGroup) * kv_group_bytes(DIM);
+    static constexpr uint32_t kQ = 0;                       // [2 row tiles]
+    static constexpr uint32_t kK = kQ + 2 * kOperand;       // [2]
+    static constexpr uint32_t kV = kK + 2 * kOperand;       // [2]
+    static constexpr uint32_t kRawAt = kV + 2 * kOperand;   // [kRawSlots]
+    static constexpr uint32_t kInfo = kRawAt + kRawSlots * kRaw;
+    static constexpr uint32_t kBars = kInfo + ((kInfoSlots * sizeof(TileInfo) + 7) & ~7u);
+    static constexpr uint32_t kNumBars = 2 * kRawSlots + 8 + 2 + 2 + 2 + 2;
+    static constexpr uint32_t kBytes = kBars + 8 * kNumBars + 16 + 1024;
+};
+
+struct MmaParams {
+    AttnArgs a;
+    int vec_q, vec_out;
+    int tiles;  // blocks of kRows per request and key head in the grid
+    int *err;
+};
+
+PFNG_DEV void umma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+PFNG_DEV void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+#define PFNG_OUT32(x) \
+    "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]), "=r"(x[6]), "=r"(x[7]), "=r"(x[8]), \
+        "=r"(x[9]), "=r"(x[10]), "=r"(x[11]), "=r"(x[12]), "=r"(x[13]), "=r"(x[14]), "=r"(x[15]), "=r"(x[16]), \
+        "=r"(x[17]), "=r"(x[18]), "=r"(x[19]), "=r"(x[20]), "=r"(x[21]), "=r"(x[22]), "=r"(x[23]), "=r"(x[24]), \
+        "=r"(x[25]), "=r"(x[26]), "=r"(x[27]), "=r"(x[28]), "=r"(x[29]), "=r"(x[30]), "=r"(x[31])
+#define PFNG_IN32(x) \
+    "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7]), "r"(x[8]), "r"(x[9]), \
+        "r"(x[10]), "r"(x[11]), "r"(x[12]), "r"(x[13]), "r"(x[14]), "r"(x[15]), "r"(x[16]), "r"(x[17]), "r"(x[18]), \
+        "r"(x[19]), "r"(x[20]), "r"(x[21]), "r"(x[22]), "r"(x[23]), "r"(x[24]), "r"(x[25]), "r"(x[26]), "r"(x[27]), \
+        "r"(x[28]), "r"(x[29]), "r"(x[30]), "r"(x[31])
+// 32 columns of this warp's 32 TMEM lanes, a lane per thread.  The loads of a
+// tile are issued together and waited for once.
+PFNG_DEV void tmem_ld32(uint32_t at, uint32_t *x) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : PFNG_OUT32(x)
+        : "r"(at)
+        : "memory");
+}
+PFNG_DEV void tmem_st32(uint32_t at, const uint32_t *x) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::PFNG_IN32(x),
+        "r"(at)
+        : "memory");
+}
+#define PFNG_IO16(x) \
+    "+r"(x[0]), "+r"(x[1]), "+r"(x[2]), "+r"(x[3]), "+r"(x[4]), "+r"(x[5]), "+r"(x[6]), "+r"(x[7]), "+r"(x[8]), \
+        "+r"(x[9]), "+r"(x[10]), "+r"(x[11]), "+r"(x[12]), "+r"(x[13]), "+r"(x[14]), "+r"(x[15])
+// Waits for the loads; the N registers that they filled are operands, so that
+// nothing computed from them moves above the wait.
+template <int N>
+PFNG_DEV void tmem_wait_ld(uint32_t *x) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < N; i += 16) {
+        uint32_t *y = x + i;
+        asm volatile("" : PFNG_IO16(y));
+    }
+}
+PFNG_DEV void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+template <int N>
+PFNG_DEV void registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+PFNG_DEV void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+PFNG_DEV float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+PFNG_DEV uint32_t h2(__half2 x) { return *reinterpret_cast<uint32_t *>(&x); }
+PFNG_DEV __half2 as_h2(uint32_t x) { return *reinterpret_cast<__half2 *>(&x); }
+template <uint32_t MASK>
+PFNG_DEV uint32_t and_or(uint32_t x, uint32_t y) {
+    uint32_t z;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(z) : "r"(x), "n"(MASK), "r"(y));
+    return z;
+}
+PFNG_DEV int exponent_of(float x) { return max(static_cast<int>(__float_as_uint(x) >> 23) - 127, -126); }
+PFNG_DEV float power_of_two(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
+
+// V operand: "MN-major" (a key's dimensions are contiguous), 128-byte swizzle:
+// atoms of 64 dimensions x 8 keys; 1024 bytes from one to the next 8 keys,
+// kTile * 128 bytes from one to the next 64 dimensions.
+PFNG_DEV uint64_t v_desc(uint32_t saddr) {
+    uint64_t d = static_cast<uint64_t>((saddr >> 4) & 0x3FFFu);
+    d |= static_cast<uint64_t>((kTile * 128u) >> 4) << 16;
+    d |= static_cast<uint64_t>(1024u >> 4) << 32;
+    d |= static_cast<uint64_t>(1u) << 46;
+    d |= static_cast<uint64_t>(2u) << 61;
+    return d;
+}
+// fp32 accumulator, fp16 A and B, M = 128; N and whether B is MN-major.
+constexpr uint32_t idesc_f16(int n, bool mn_major) {
+    return (1u << 4) | (mn_major ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) | ((kTile >> 4) << 24);
+}
+// Byte of 16-byte chunk c of row r in an operand tile (K-major Q and K: rows
+// of 64 dimensions; V: the same bytes seen as MN-major).
+PFNG_DEV uint32_t operand_at(int r, int c) {
+    return static_cast<uint32_t>((c >> 3) * (kTile * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+}
+
+// A word of a cache row as 8 fp16 values (n - 8) * s, in pairs: low nibbles of
+// bytes 0, 2; of bytes 1, 3; high nibbles of bytes 0, 2; of bytes 1, 3.
+PFNG_DEV uint4 unpack_word(uint32_t w, uint32_t scale, uint32_t magic) {
+    const __half2 minus1032 = __float2half2_rn(-1032.0f), minus72 = __float2half2_rn(-72.0f),
+                  sixteenth = __float2half2_rn(0.0625f), s = as_h2(scale);
+    const uint32_t w8 = w >> 8;
+    return make_uint4(h2(__hmul2(__hadd2(as_h2(and_or<0x000F000Fu>(w, magic)), minus1032), s)),
+                      h2(__hmul2(__hadd2(as_h2(and_or<0x000F000Fu>(w8, magic)), minus1032), s)),
+                      h2(__hmul2(__hfma2(as_h2(and_or<0x00F000F0u>(w, magic)), sixteenth, minus72), s)),
+                      h2(__hmul2(__hfma2(as_h2(and_or<0x00F000F0u>(w8, magic)), sixteenth, minus72), s)));
+}
+
+template <int DIM>
+__global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams mp) {
+    using L = Layout<DIM>;
+    constexpr int kBlocks = DIM / 32;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::kBars);
+    uint64_t *raw_full = bars, *raw_empty = raw_full + kRawSlots;
+    uint64_t *k_full = raw_empty + kRawSlots, *k_empty = k_full + 2, *v_full = k_empty + 2, *v_empty = v_full + 2;
+    uint64_t *s_full = v_empty + 2, *p_full = s_full + 2, *o_full = p_full + 2;
+    uint64_t *q_full = o_full + 2, *mma_done = q_full + 1;
+    uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(bars + L::kNumBars);
+    TileInfo *infos = reinterpret_cast<TileInfo *>(smem + L::kInfo);
+    __shared__ int abort_flag;
+
+    const AttnArgs &p = mp.a;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    // the last row tiles see the most keys: they come first
+    const int tile = mp.tiles - 1 - static_cast<int>(blockIdx.x / (p.requests * p.heads_kv));
+    const int64_t rest = blockIdx.x % (p.requests * p.heads_kv);
+    const int64_t r = rest / p.heads_kv;
+    const int head_kv = static_cast<int>(rest % p.heads_kv);
+    const int group = p.heads_q / p.heads_kv;
+    int all;
+    const int rows = attn_new_tokens(p, r, all) * group;
+    const int row0 = tile * kRows;
+    if (row0 >= rows) return;
+    const int seq = attn_seq_len(p, r);
+    const int row_tiles = rows - row0 > kTile ? 2 : 1;
+    int first, count;  // key tiles
+    {
+        int lo, hi, lo2, hi2;
+        attn_visible(p, seq, all, row0 / group, lo, hi2);
+        attn_visible(p, seq, all, (min(row0 + kRows, rows) - 1) / group, lo2, hi);
+        first = max(lo, 0) / kTile;
+        count = hi > first * kTile ? (hi + kTile - 1) / kTile - first : 0;
+    }
+
+    if (tid == 0) {
+        abort_flag = 0;
+        for (int i = 0; i < kRawSlots; ++i) mbar_init(&raw_full[i], 1), mbar_init(&raw_empty[i], 4);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&k_full[i], 4), mbar_init(&k_empty[i], 1);
+            mbar_init(&v_full[i], 4), mbar_init(&v_empty[i], 1);
+            mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 4), mbar_init(&o_full[i], 1);
+        }
+        mbar_init(q_full, 4 * row_tiles);
+        mbar_init(mma_done, 1);
+        fence_mbar_init();
+    }
+    if (warp == 12) {
+        tmem_alloc(tmem_holder, kTmemCols);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(tmem_holder);
+    const uint32_t base = smem_u32(smem);
+
+    if (warp < 8) {
+        // ---------------- softmax ----------------
+        registers_up<192>();
+        const int i = warp >> 2;  // row tile
+        const int in_tile = (warp & 3) * 32 + lane, row = row0 + i * kTile + in_tile;
+        const bool live = row < rows;
+        const int64_t token = p.cu_q[r] + (live ? row / group : 0);
+        const int64_t head = static_cast<int64_t>(head_kv) * group + (live ? row % group : 0);
+        int lo = 0, hi = 0;
+        if (live) attn_visible(p, seq, all, row / group, lo, hi);
+        if (i < row_tiles) {
+            float mul;
+            {  // Q: largest value of the row into [2^13, 2^14), sign of the softmax scale included
+                const int64_t at = token * p.ldq + head * DIM;
+                float top = 0.0f;
+#pragma unroll 4
+                for (int c = 0; c < DIM / 4; ++c) {
+                    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    if (live) {
+                        if (mp.vec_q) {
+                            load_values<4>(p.q_format, p.q, at + 4 * c, v);
+                        } else {
+                            for (int j = 0; j < 4; ++j) {
+                                float one[1];
+                                load_values<1>(p.q_format, p.q, at + 4 * c + j, one);
+                                v[j] = one[0];
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) top = fmaxf(top, fabsf(v[j]));
+                }
+                int e = 0;
+                if (top > 0.0f && top < INFINITY) e = exponent_of(top) - 13;
+                const float up0 = power_of_two(-(e / 2)) * (p.scale < 0.0f ? -1.0f : 1.0f),
+                            up1 = power_of_two(-(e - e / 2));
+                // a floor keeps -inf * mul at -inf for a scale of 0
+                mul = fmaxf(fabsf(p.scale) * kLog2e * power_of_two(e / 2) * power_of_two(e - e / 2), 1e-35f);
+#pragma unroll 2
+                for (int c = 0; c < DIM / 8; ++c) {
+                    const int t = c / kBlocks, b = c % kBlocks;
+                    float v[2][4] = {};
+                    if (live) {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            if (mp.vec_q) {
+                                load_values<4>(p.q_format, p.q, at + 32 * b + 16 * h + 4 * t, v[h]);
+                            } else {
+                                for (int j = 0; j < 4; ++j) {
+                                    float one[1];
+                                    load_values<1>(p.q_format, p.q, at + 32 * b + 16 * h + 4 * t + j, one);
+                                    v[h][j] = one[0];
+                                }
+                            }
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) v[h][j] = v[h][j] * up0 * up1;
+                        }
+                    }
+                    *reinterpret_cast<uint4 *>(smem + L::kQ + i * L::kOperand + operand_at(in_tile, c)) = make_uint4(
+                        h2(__floats2half2_rn(v[0][0], v[0][2])), h2(__floats2half2_rn(v[0][1], v[0][3])),
+                        h2(__floats2half2_rn(v[1][0], v[1][2])), h2(__floats2half2_rn(v[1][1], v[1][3])));
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(q_full);
+            }
+            const uint32_t s_at = tmem + static_cast<uint32_t>(i * kTile) + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+            const uint32_t o_at = s_at + 256;
+            float m = kNoMax, l = 0.0f;
+            bool ok = true;
+            // a key with a bad V scale makes the rows that see it NaN
+            const auto bad_keys = [&](int n) {
+                const TileInfo &info = infos[n % kInfoSlots];
+                const int key0 = (first + n) * kTile;
+                if (info.bad[0] | info.bad[1] | info.bad[2] | info.bad[3])
+                    for (int c = 0; c < kTile; ++c)
+                        if (((info.bad[c >> 5] >> (c & 31)) & 1u) && key0 + c >= lo && key0 + c < hi)
+                            l = __int_as_float(0x7fffffff);
+            };
+            for (int n = 0; n < count; ++n) {
+                if (!wait_bar(&s_full[i], n & 1, &abort_flag, mp.err, kErrWaitFull)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                uint32_t s[kTile];
+#pragma unroll
+                for (int c = 0; c < kTile; c += 32) tmem_ld32(s_at + c, s + c);
+                const uint32_t groups = infos[n % kInfoSlots].groups;
+                if (n > 0) bad_keys(n - 1);  // V of the last tile is complete: this tile's MMA came after its own
+                tmem_wait_ld<kTile>(s);
+                const int key0 = (first + n) * kTile;
+                if (__any_sync(0xffffffffu, key0 < lo || key0 + kTile > hi) || groups != 0xffu) {
+                    const int from = lo - key0, to = hi - key0;
+#pragma unroll
+                    for (int c = 0; c < kTile; ++c)
+                        if (!(c >= from && c < to && ((groups >> (c / kKvGroup)) & 1u))) s[c] = 0xff800000u;
+                }
+                float top = fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+#pragma unroll
+                for (int c = 2; c < kTile; c += 2)
+                    top = fmaxf(fmaxf(top, __uint_as_float(s[c])), __uint_as_float(s[c + 1]));
+                top *= mul;
+                if (__any_sync(0xffffffffu, top > m + (kLift + kSlack))) {
+                    const float m_new = fmaxf(top - kLift, m);
+                    const float f = exp2_approx(m - m_new);
+                    m = m_new;
+                    l *= f;
+                    if (n > 0) {
+#pragma unroll 1
+                        for (int c = 0; c < DIM; c += 32) {
+                            uint32_t o[32];
+                            tmem_ld32(o_at + c, o);
+                            tmem_wait_ld<32>(o);
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+                            tmem_st32(o_at + c, o);
+                        }
+                    }
+                }
+                float sum[4] = {};
+#pragma unroll
+                for (int c = 0; c < kTile; c += 2) {
+                    const float x = exp2_approx(fmaf(__uint_as_float(s[c]), mul, -m));
+                    const float y = exp2_approx(fmaf(__uint_as_float(s[c + 1]), mul, -m));
+                    sum[c & 2] += x;
+                    sum[(c & 2) + 1] += y;
+                    s[c / 2] = h2(__floats2half2_rn(x, y));
+                    if (c == kTile / 2 - 2) tmem_st32(s_at, s);
+                }
+                tmem_st32(s_at + 32, s + 32);
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[i]);
+            }
+            if (ok && count > 0) {
+                ok = wait_bar(&o_full[i], 0, &abort_flag, mp.err, kErrWaitFull);
+                if (ok) bad_keys(count - 1);
+            }
+            if (!ok) abort_flag = 1;
+            tc_fence_after();
+            const bool none = l == 0.0f;
+            const float f = none ? 0.0f : 1.0f / l;
+            if (ok) {
+                const int64_t at = token * p.ldo + head * DIM;
+#pragma unroll 1
+                for (int c = 0; c < DIM / 32; ++c) {
+                    uint32_t o[32] = {};
+                    if (count > 0) {
+                        tmem_ld32(o_at + 32 * c, o);
+                        tmem_wait_ld<32>(o);
+                    }
+                    if (!live) continue;
+#pragma unroll
+                    for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+#pragma unroll
+                            for (int x = 0; x < (kBlocks == 4 ? 1 : 2); ++x) {
+                                // words of a V row: (g, pair of blocks); element (b & 1) + 2 e + 4 h of a word is
+                                // dimension 2 g + e + 16 h of block b
+                                float v[4];
+                                int dim;
+                                if constexpr (kBlocks == 4) {
+                                    dim = 32 * b + 16 * h + 4 * c;
+#pragma unroll
+                                    for (int j = 0; j < 4; ++j)
+                                        v[j] = __uint_as_float(o[(2 * (j >> 1) + (b >> 1)) * 8 + (b & 1) + 2 * (j & 1) + 4 * h]) * f;
+                                } else {
+                                    dim = 32 * b + 16 * h + 8 * c + 4 * x;
+#pragma unroll
+                                    for (int j = 0; j < 4; ++j)
+                                        v[j] = __uint_as_float(o[(2 * x + (j >> 1)) * 8 + b + 2 * (j & 1) + 4 * h]) * f;
+                                }
+                                if (mp.vec_out) {
+                                    store_values<4>(p.out_format, p.out, at + dim, v);
+                                } else {
+#pragma unroll
+                                    for (int j = 0; j < 4; ++j) {
+                                        const float one[1] = {v[j]};
+                                        store_values<1>(p.out_format, p.out, at + dim + j, one);
+                                    }
+                                }
+                            }
+                }
+                if (live && p.lse)
+                    p.lse[token * p.heads_q + head] = none ? -INFINITY : (m + log2f(l)) / kLog2e;
+            }
+        }
+    } else if (warp < 12) {
+        // ---------------- dequantization ----------------
+        registers_down<80>();
+        const int t = tid - 256;
+        uint32_t magic;
+        asm volatile("mov.b32 %0, 0x64006400;" : "=r"(magic));
+        constexpr int kQuads = DIM / 32;  // 16-byte pieces of a row
+        bool ok = true;
+        for (int j = 0; j < 2 * count; ++j) {
+            const int n = j >> 1, slot = j % kRawSlots, stage = n & 1;
+            const bool is_v = j & 1;
+            if (!wait_bar(&raw_full[slot], (j / kRawSlots) & 1, &abort_flag, mp.err, kErrWaitFull) ||
+                (n >= 2 && !wait_bar(is_v ? &v_empty[stage] : &k_empty[stage], ((n >> 1) - 1) & 1, &abort_flag, mp.err,
+                                     kErrWaitEmpty))) {
+                ok = false;
+                break;
+            }
+            const uint8_t *raw = smem + L::kRawAt + slot * L::kRaw;
+            uint8_t *to = smem + (is_v ? L::kV : L::kK) + stage * L::kOperand;
+            TileInfo &info = infos[n % kInfoSlots];
+            const uint32_t groups = info.groups;
+            const int keys = seq - (first + n) * kTile;  // rows past the last key are zeros
+#pragma unroll
+            for (int i = 0; i < kQuads; ++i) {
+                const int idx = i * 128 + t, row = idx / kQuads, u = idx % kQuads;
+                const uint8_t *gr = raw + (row / kKvGroup) * kv_group_bytes(DIM);
+                const uint4 w = *reinterpret_cast<const uint4 *>(gr + (row % kKvGroup) * kv_row_bytes(DIM) + 16 * u);
+                const bool valid = row < keys && ((groups >> (row / kKvGroup)) & 1u);
+                uint32_t sc[kBlocks / 2];
+#pragma unroll
+                for (int b = 0; b < kBlocks / 2; ++b) {
+                    sc[b] = *reinterpret_cast<const uint32_t *>(gr + kv_scale_offset(DIM) + (row % kKvGroup) * (DIM / 16) + 4 * b);
+                    if (!valid) sc[b] = 0;
+                }
+                uint32_t s[4];
+                if (is_v) {
+                    bool bad = false;
+#pragma unroll
+                    for (int b = 0; b < kBlocks / 2; ++b)
+                        bad |= (sc[b] & 0x7c00u) == 0x7c00u || (sc[b] & 0x7c000000u) == 0x7c000000u;
+                    if (bad) {
+#pragma unroll
+                        for (int b = 0; b < kBlocks / 2; ++b) sc[b] = 0;
+                        if (u == 0) atomicOr(&info.bad[row >> 5], 1u << (row & 31));
+                    }
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) s[x] = sc[kBlocks == 4 ? (x & 1) : 0];
+                } else {
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        const int b = x % kBlocks;
+                        s[x] = __byte_perm(sc[b / 2], 0, (b & 1) ? 0x3232 : 0x1010);
+                    }
+                }
+                const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+                    *reinterpret_cast<uint4 *>(to + operand_at(row, 4 * u + x)) = unpack_word(words[x], s[x], magic);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(is_v ? &v_full[stage] : &k_full[stage]);
+                mbar_arrive(&raw_empty[slot]);
+            }
+        }
+        if (!ok) abort_flag = 1;
+    } else {
+        registers_down<48>();
+        if (warp == 12 && lane == 0) {
+            // ---------------- MMA issue ----------------
+            constexpr uint32_t kIdescS = idesc_f16(kTile, false), kIdescO = idesc_f16(DIM, true);
+            bool ok = count > 0 && wait_bar(q_full, 0, &abort_flag, mp.err, kErrWaitFull);
+            const auto scores = [&](int i, int stage) {
+#pragma unroll
+                for (int k = 0; k < DIM / 16; ++k) {
+                    const uint32_t off = (k >> 2) * (kTile * 128u) + (k & 3) * 32u;
+                    umma_f16_ss(tmem + i * kTile, sw128_desc(base + L::kQ + i * L::kOperand + off),
+                                sw128_desc(base + L::kK + stage * L::kOperand + off), kIdescS, k > 0);
+                }
+                umma_commit(&s_full[i]);
+            };
+            if (ok) ok = wait_bar(&k_full[0], 0, &abort_flag, mp.err, kErrWaitFull);
+            if (ok) {
+                tc_fence_after();
+                for (int i = 0; i < row_tiles; ++i) scores(i, 0);
+                umma_commit(&k_empty[0]);
+            }
+            for (int n = 0; n < count && ok; ++n) {
+                const int stage = n & 1, next = (n + 1) & 1;
+                ok = wait_bar(&v_full[stage], (n >> 1) & 1, &abort_flag, mp.err, kErrWaitFull);
+                if (ok && n + 1 < count) ok = wait_bar(&k_full[next], ((n + 1) >> 1) & 1, &abort_flag, mp.err, kErrWaitFull);
+                for (int i = 0; i < row_tiles && ok; ++i) {
+                    ok = wait_bar(&p_full[i], n & 1, &abort_flag, mp.err, kErrWaitFull);
+                    if (!ok) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int k = 0; k < kTile / 16; ++k)
+                        umma_f16_ts(tmem + 256 + i * kTile, tmem + i * kTile + 8 * k,
+                                    v_desc(base + L::kV + stage * L::kOperand + k * 2048u), kIdescO, n > 0 || k > 0);
+                    if (i == row_tiles - 1) umma_commit(&v_empty[stage]);
+                    if (n + 1 < count) {
+                        scores(i, next);
+                        if (i == row_tiles - 1) umma_commit(&k_empty[next]);
+                    } else {
+                        umma_commit(&o_full[i]);
+                    }
+                }
+            }
+            if (!ok && count > 0) abort_flag = 1;
+            umma_commit(mma_done);  // TMEM is freed at the end: no MMA may be in flight
+            if (!mbar_wait(mma_done, 0, mp.err, kErrWaitFull)) abort_flag = 1;
+        } else if (warp == 13) {
+            // ---------------- copies from the pages ----------------
+            const uint64_t policy = l2_policy_evict_normal();
+            bool ok = true;
+            int j = 0;
+            int page = -1, key = 0;
+            for (; j < 2 * count; ++j) {
+                const int n = j >> 1, slot = j % kRawSlots;
+                const bool is_v = j & 1;
+                if (j >= kRawSlots &&
+                    !wait_bar(&raw_empty[slot], ((j / kRawSlots) - 1) & 1, &abort_flag, mp.err, kErrWaitEmpty)) {
+                    ok = false;
+                    break;
+                }
+                if (!is_v) {
+                    key = (first + n) * kTile + lane * kKvGroup;
+                    page = lane < kTile / kKvGroup && key < seq ? attn_page(p, r, key) : -1;
+                }
+                const uint32_t there = __ballot_sync(0xffffffffu, page >= 0);
+                if (lane == 0) {
+                    if (!is_v) {
+                        TileInfo &info = infos[n % kInfoSlots];
+                        info.groups = there;
+                        info.bad[0] = info.bad[1] = info.bad[2] = info.bad[3] = 0;
+                    }
+                    mbar_arrive_expect_tx(&raw_full[slot], kv_group_bytes(DIM) * __popc(there));
+                }
+                __syncwarp();
+                if (page >= 0)
+                    bulk_copy_g2s(smem + L::kRawAt + slot * L::kRaw + lane * kv_group_bytes(DIM),
+                                  (is_v ? p.v_cache : p.k_cache) + kv_group_offset(page, head_kv, key % p.page_size, p.heads_kv,
+                                                                                   p.page_size / kKvGroup, DIM),
+                                  kv_group_bytes(DIM), &raw_full[slot], policy);
+            }
+            if (!ok) abort_flag = 1;
+            // copies in flight end before the CTA does
+            if (!ok || aborted(&abort_flag))
+                for (int x = max(j - kRawSlots, 0); x < j; ++x)
+                    mbar_wait(&raw_full[x % kRawSlots], (x / kRawSlots) & 1, mp.err, kErrWaitFull);
+        }
+        __syncwarp();
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 12) {
+        tc_fence_after();
+        tmem_dealloc(tmem, kTmemCols);
+    }
+}
+
+template <int DIM>
+cudaError_t launch(const MmaParams &mp, int64_t grid, cudaStream_t s) {
+    const cudaError_t e = cudaFuncSetAttribute(attn_mma_kernel<DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               static_cast<int>(Layout<DIM>::kBytes));
+    if (e != cudaSuccess) return e;
+    attn_mma_kernel<DIM><<<static_cast<unsigned>(grid), kThreads, Layout<DIM>::kBytes, s>>>(mp);
+    return cudaGetLastError();
+}
+
+int64_t row_blocks(const AttnArgs &p) { return (p.max_q * (p.heads_q / p.heads_kv) + kRows - 1) / kRows; }
+
+}  // namespace
+
+bool attn_mma_supported(const AttnArgs &p) {
+    return (p.head_dim == 64 || p.head_dim == 128) && row_blocks(p) * p.requests * p.heads_kv < 0x7fffffff;
+}
+
+cudaError_t launch_attn_mma(const AttnArgs &p, int *err, cudaStream_t s) {
+    MmaParams mp{};
+    mp.a = p;
+    const auto wide = [](const void *x, int64_t ld, int fmt) {
+        return ld % 4 == 0 && reinterpret_cast<uintptr_t>(x) % (fmt == kOutF32 ? 16 : 8) == 0;
+    };
+    mp.vec_q = wide(p.q, p.ldq, p.q_format);
+    mp.vec_out = wide(p.out, p.ldo, p.out_format);
+    mp.tiles = static_cast<int>(row_blocks(p));
+    mp.err = err;
+    const int64_t grid = row_blocks(p) * p.requests * p.heads_kv;
+    return p.head_dim == 128 ? launch<128>(mp, grid, s) : launch<64>(mp, grid, s);
+}
+
+}  // namespace pfng

@@ -53,6 +53,7 @@
 
 #include "pfng_common.cuh"
 #include "pfng_internal.h"
+#include "pfng_tc.cuh"
 #include "pfng_tma.h"
 
 namespace pfng {
@@ -97,21 +98,6 @@ struct TcParams {
     int *err;
 };
 
-// ---- TMA / tcgen05 / proxy primitives ----------------------------------------
-PFNG_DEV void fence_proxy_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-PFNG_DEV void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-PFNG_DEV void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
-PFNG_DEV void tmem_alloc(uint32_t *holder, uint32_t ncols) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(holder)),
-                 "r"(ncols)
-                 : "memory");
-}
-PFNG_DEV void tmem_relinquish() { asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory"); }
-PFNG_DEV void tmem_dealloc(uint32_t taddr, uint32_t ncols) {
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
-}
-
 // D[tmem] (+)= A[smem] . B[smem]^T, int8 x int8 -> int32; accumulate != 0 adds onto D.
 PFNG_DEV void umma_i8(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
@@ -121,12 +107,6 @@ PFNG_DEV void umma_i8(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_
         ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(0u)
         : "memory");
 }
-// Arrives on `bar` once every tcgen05.mma this thread issued before has completed.
-PFNG_DEV void umma_commit(uint64_t *bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-                 : "memory");
-}
-
 #define PFNG_R32(x) \
     "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]), "=r"(x[6]), "=r"(x[7]), "=r"(x[8]), \
         "=r"(x[9]), "=r"(x[10]), "=r"(x[11]), "=r"(x[12]), "=r"(x[13]), "=r"(x[14]), "=r"(x[15]), "=r"(x[16]), \
@@ -170,20 +150,6 @@ PFNG_DEV void tmem_ld_16x256b_2x4(uint32_t ta, uint32_t tb, uint64_t (&d)[16]) {
 #undef PFNG_R32
 
 
-// Shared-memory matrix descriptor, K-major operand with the 128-byte swizzle:
-// rows of 128 bytes, 8-row atoms of 1024 bytes stored back to back (stride
-// byte offset 1024), the 16-byte chunk j of row r stored at chunk j ^ (r % 8)
-// -- the layout a TMA copy with CU_TENSOR_MAP_SWIZZLE_128B and a 128-byte
-// inner box writes.  `saddr` is the operand's first byte for this MMA (atom
-// base + k offset).
-PFNG_DEV uint64_t sw128_desc(uint32_t saddr) {
-    uint64_t d = static_cast<uint64_t>((saddr >> 4) & 0x3FFFu);  // start address, 16-byte units
-    d |= static_cast<uint64_t>(1u) << 16;                         // leading byte offset (unused with this swizzle)
-    d |= static_cast<uint64_t>(1024u >> 4) << 32;                 // stride byte offset between 8-row atoms
-    d |= static_cast<uint64_t>(1u) << 46;                         // descriptor version of sm_100
-    d |= static_cast<uint64_t>(2u) << 61;                         // layout: 128-byte swizzle
-    return d;
-}
 // Instruction descriptor: int32 accumulator, signed int8 A and B, both
 // K-major, N = TN, M = TM.
 constexpr uint32_t kIdesc = (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(TN >> 3) << 17) |
@@ -193,51 +159,6 @@ constexpr uint32_t kIdesc = (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<ui
 // 128-row operand tile: column block c / 8, swizzled chunk within it.
 PFNG_DEV uint32_t op_off(uint32_t row, uint32_t c) {
     return (c >> 3) * TM * 128u + (row >> 3) * 1024u + (row & 7u) * 128u + (((c & 7u) ^ (row & 7u)) << 4);
-}
-
-// Bounded wait that also gives up (false) once the CTA's abort flag is up.
-// Each attempt is a hardware-suspended try_wait, so a waiting warp issues
-// almost nothing; the abort flag is looked at every 16 attempts.
-PFNG_DEV bool wait_bar(uint64_t *bar, uint32_t parity, const int *abort_flag, int *err, int code) {
-    for (uint32_t i = 0; i < kWaitAttempts; ++i) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if ((i & 15u) == 15u && *reinterpret_cast<const volatile int *>(abort_flag)) return false;
-    }
-    report_error(err, code);
-    return false;
-}
-PFNG_DEV bool aborted(const int *abort_flag) { return *reinterpret_cast<const volatile int *>(abort_flag) != 0; }
-// The wait of the roles off the critical path (producer, MMA issuer): each
-// attempt may suspend the thread for up to 20 us (or until the phase
-// completes), so that its polling does not take issue slots from the fold
-// warps on its scheduler; the wait is bounded by ~1 s of wall time
-// (%globaltimer), whatever the suspensions actually last.
-PFNG_DEV uint64_t global_ns() {
-    uint64_t t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    return t;
-}
-PFNG_DEV bool mbar_try_wait_long(uint64_t *bar, uint32_t parity) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 20000;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    return done != 0;
-}
-PFNG_DEV bool wait_bar_sleep(uint64_t *bar, uint32_t parity, const int *abort_flag, int *err, int code) {
-    if (mbar_try_wait_long(bar, parity)) return true;
-    const uint64_t t0 = global_ns();
-    for (;;) {
-        if (mbar_try_wait_long(bar, parity)) return true;
-        if (*reinterpret_cast<const volatile int *>(abort_flag)) return false;
-        if (global_ns() - t0 > 1000000000ull) break;
-    }
-    report_error(err, code);
-    return false;
 }
 
 __global__ void __launch_bounds__(kThreads, 1)

@@ -33,10 +33,15 @@ int check_attention(int64_t requests, int64_t tokens, int64_t heads_q, int64_t h
 
 // Kernel path of a call, -1 for a forced path that cannot run it.
 int resolve_attention(const AttnArgs &a, int path) {
-    const bool stream = attn_stream_supported(a);
-    if (path == PFNG_B200_PATH_AUTO) return stream ? PFNG_B200_PATH_GEMV : PFNG_B200_PATH_SIMPLE;
+    const bool stream = attn_stream_supported(a), mma = attn_mma_supported(a);
+    if (path == PFNG_B200_PATH_AUTO) {
+        // up to 16 query rows per key head are one tile of the streaming kernel
+        const bool few = a.max_q * (a.heads_q / a.heads_kv) <= 16;
+        if (few && stream) return PFNG_B200_PATH_GEMV;
+        return mma ? PFNG_B200_PATH_MMA : PFNG_B200_PATH_SIMPLE;
+    }
     if (path == PFNG_B200_PATH_GEMV && !stream) return -1;
-    if (path == PFNG_B200_PATH_MMA) return -1;
+    if (path == PFNG_B200_PATH_MMA && !mma) return -1;
     return path;
 }
 
@@ -182,6 +187,7 @@ int pfng_b200_attention_q4_0(const void *q, int64_t ldq, int q_format, const voi
     if (need > 0 && !aligned(workspace, 256)) return PFNG_B200_ERR_ALIGNMENT;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (resolved == PFNG_B200_PATH_GEMV) return status_of(launch_attn_stream(a, workspace, device_error_word(), s));
+    if (resolved == PFNG_B200_PATH_MMA) return status_of(launch_attn_mma(a, device_error_word(), s));
     return status_of(launch_attn_simple(a, s));
 }
 

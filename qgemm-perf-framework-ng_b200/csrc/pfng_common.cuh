@@ -128,6 +128,11 @@ PFNG_DEV uint64_t l2_policy_evict_first() {
     asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
     return policy;
 }
+PFNG_DEV uint64_t l2_policy_evict_normal() {
+    uint64_t policy;
+    asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(policy));
+    return policy;
+}
 
 // ---- programmatic dependent launch --------------------------------------------
 // pdl_trigger: kernels launched after this one with programmatic stream

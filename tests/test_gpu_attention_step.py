@@ -256,7 +256,7 @@ class Case:
         assert bool((off <= bound).all()), f"lse {float((off / bound).max())}"
 
 
-PATHS = ["simple", "auto"]
+PATHS = ["simple", "gemv", "mma", "auto"]
 
 
 @pytest.mark.parametrize("path", PATHS)
@@ -272,6 +272,11 @@ def test_attention_single_tokens(path, dim, hq, hk):
 def test_attention_other_head_dims(path, dim):
     if path == "auto":
         Case([70, 3], [1, 1], 4, 2, dim, 16).check("f16")
+    if path in ("gemv", "mma"):  # no such kernel for these
+        with pytest.raises(pb.PfngError) as e:
+            Case([70, 40], [5, 40], 4, 2, dim, 32).run("f16", path)
+        assert e.value.status == -7
+        return
     Case([70, 40], [5, 40], 4, 2, dim, 32).check("f16", path=path)
 
 
