@@ -97,7 +97,7 @@ int pfng_b200_qk_norm_rope(const void *x, int in_format, int64_t ldx, const floa
     if (head_dim <= 0 || head_dim > 512 || head_dim % 2 != 0 || rot_dim > head_dim || rot_dim % 2 != 0)
         return PFNG_B200_ERR_SHAPE;
     if (tokens > kMaxCount || heads_q > 65535 || heads_k > 65535 || max_pos > kMaxCount) return PFNG_B200_ERR_SHAPE;
-    if (tokens * (heads_q + heads_k) / 4 > kMaxCount) return PFNG_B200_ERR_SHAPE;  // rows of one launch
+    if (tokens * (heads_q + heads_k) > kMaxCount) return PFNG_B200_ERR_SHAPE;  // rows of one launch
     if (tokens > 0 && (ldx < (heads_q + heads_k) * head_dim || ldq < heads_q * head_dim || ldk < heads_k * head_dim))
         return PFNG_B200_ERR_SHAPE;
     if (tokens == 0 || heads_q + heads_k == 0) return PFNG_B200_OK;
@@ -121,7 +121,7 @@ int pfng_b200_kv_append_q4_0(const void *k, int64_t ldk, int k_format, const voi
     if (tokens < 0 || heads_kv < 0 || num_pages < 0) return PFNG_B200_ERR_INVALID_ARGUMENT;
     if (head_dim <= 0 || head_dim % 32 != 0 || head_dim > 512 || !page_size_ok(page_size)) return PFNG_B200_ERR_SHAPE;
     if (tokens > kMaxCount || heads_kv > 65535 || num_pages > kMaxCount) return PFNG_B200_ERR_SHAPE;
-    if (tokens * heads_kv / 8 > kMaxCount) return PFNG_B200_ERR_SHAPE;  // rows of one launch
+    if (tokens * heads_kv * (head_dim / 32) > kMaxCount) return PFNG_B200_ERR_SHAPE;  // blocks of one launch
     if (tokens > 0 && (ldk < heads_kv * head_dim || ldv < heads_kv * head_dim)) return PFNG_B200_ERR_SHAPE;
     if (tokens == 0 || heads_kv == 0 || num_pages == 0) return PFNG_B200_OK;
     if (!k || !v || !slots || !k_cache || !v_cache) return PFNG_B200_ERR_INVALID_ARGUMENT;

@@ -8,8 +8,8 @@
 //
 // Four lanes hold a block, eight values each (16 or 32 bytes, one or two wide
 // loads), so the search for m is two shuffle steps; each lane then trades its
-// nibbles with the lane that holds the other half of its bytes and stores
-// four bytes of the row.  The 16 rows of a group are contiguous, so a run of
+// nibbles with the lane that holds the other half of its bytes (and, for V, with
+// the neighbouring block) and stores four bytes of the row.  The 16 rows of a group are contiguous, so a run of
 // tokens is written in whole sectors.
 #include "kv_cache.cuh"
 
@@ -18,83 +18,130 @@ namespace {
 
 constexpr int kThreads = 256;
 
-template <bool kVec>
-PFNG_DEV void load8(int fmt, const void *p, int64_t at, float (&v)[8]) {
-    if constexpr (kVec) {
-        load_values<8>(fmt, p, at, v);
-    } else {
+// Blocks of four lanes, kBatch of them a lane: their loads are in flight
+// together.
+constexpr int kBatch = 4;
+
+// The part of one CTA, K (is_v false) or V in the format FMT; wide: rows allow
+// 16-byte loads.
+// FIXED: q4_0 blocks of a head where they are known, else 0.
+template <int FMT, bool WIDE, int FIXED>
+PFNG_DEV void append(const AppendArgs &p, bool is_v) {
+    const uint32_t blocks = FIXED ? FIXED : static_cast<uint32_t>(p.head_dim / 32);
+    const uint32_t per_token = static_cast<uint32_t>(p.heads_kv) * blocks;
+    const uint32_t total = static_cast<uint32_t>(p.tokens) * per_token;
+    const int quad = threadIdx.x & 3;
+    const void *x = is_v ? p.v : p.k;
+    const int64_t ld = is_v ? p.ldv : p.ldk;
+    uint8_t *cache = is_v ? p.v_cache : p.k_cache;
+    const int dim = static_cast<int>(p.head_dim);
+    RawValues<FMT, WIDE ? 8 : 1> raw[kBatch][WIDE ? 1 : 8];
+    // a warp's 8 * kBatch blocks are consecutive
+    const uint32_t first_id = (blockIdx.x * (kThreads / 32) + threadIdx.x / 32) * (8 * kBatch) + (threadIdx.x & 31) / 4;
+    uint32_t token[kBatch];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            float one[1];
-            load_values<1>(fmt, p, at + i, one);
-            v[i] = one[0];
+    for (int i = 0; i < kBatch; ++i) {
+        const uint32_t id = min(first_id + 8 * i, total - 1);
+        token[i] = i > 0 && id < (token[i - 1] + 1) * per_token ? token[i - 1] : id / per_token;
+#pragma unroll
+        for (int j = 0; j < (WIDE ? 1 : 8); ++j)
+            raw[i][j].load(x, token[i] * ld + static_cast<int64_t>(id - token[i] * per_token) * 32 + 8 * quad + j);
+    }
+    uint32_t at_token = 0xffffffffu, offset = 0;  // of the slot looked up last
+    int64_t page = -1;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if constexpr (WIDE) v[j] = raw[i][0][j];
+            else v[j] = raw[i][j][0];
         }
+        // the value of largest magnitude; where both signs have it, the first
+        float hi = 0.0f, lo = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) hi = fmaxf(hi, v[j]), lo = fminf(lo, v[j]);
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) {
+            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        }
+        float m = hi > -lo ? hi : lo;
+        if (__any_sync(0xffffffffu, hi == -lo)) {
+            int first = 64;  // 2 * index + sign
+#pragma unroll
+            for (int j = 7; j >= 0; --j)
+                if (fabsf(v[j]) == hi) first = 2 * (8 * quad + j) + (v[j] < 0.0f);
+#pragma unroll
+            for (int o = 1; o < 4; o <<= 1) first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
+            if (hi == -lo) m = (first & 1) ? lo : hi;
+        }
+        const float d = m * -0.125f;  // m / -8: the same rounding
+        const float inv = d != 0.0f ? __frcp_rn(d) : 0.0f;
+        // x / d + 8.5 lies in [0.5, 16.5] (NaN counts as 0): with 2^23 added
+        // towards zero its whole part is the low bits
+        uint32_t q[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float y = fminf(fmaxf(__fadd_rn(__fmul_rn(v[j], inv), 8.5f), 0.0f), 15.5f);
+            q[j] = __float_as_uint(__fadd_rz(y, 8388608.0f));
+        }
+        // nibbles of values 8 quad .. + 3 and + 4 .. + 7, one a byte
+        const uint32_t n[2] = {
+            __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410),
+            __byte_perm(__byte_perm(q[4], q[5], 0x0040), __byte_perm(q[6], q[7], 0x0040), 0x5410)};
+        // bytes 8 a .. 8 a + 7 of the block are lanes a (low nibbles) and a + 2
+        // (high nibbles), a = 0, 1: lane a keeps the first four, lane a + 2 the
+        // last four, so each needs one word of the other
+        const uint32_t other = __shfl_xor_sync(0xffffffffu, quad < 2 ? n[1] : n[0], 2);
+        const uint32_t bytes = quad < 2 ? n[0] | (other << 4) : other | (n[1] << 4);
+        const uint32_t word = 2 * (quad & 1) + (quad >> 1);  // bytes 4 word .. 4 word + 3
+        const uint32_t next = __shfl_xor_sync(0xffffffffu, bytes, 4);  // of the neighbouring block
+        const uint32_t id = first_id + 8 * i;
+        if (token[i] != at_token) {
+            at_token = token[i];
+            const int64_t slot = p.slots[at_token];
+            if (slot < 0 || slot >= p.num_pages * p.page_size) {
+                page = -1;
+            } else if (slot >> 32) {
+                page = slot / p.page_size;
+                offset = static_cast<uint32_t>(slot - page * p.page_size);
+            } else {
+                page = static_cast<uint32_t>(slot) / static_cast<uint32_t>(p.page_size);
+                offset = static_cast<uint32_t>(slot) % static_cast<uint32_t>(p.page_size);
+            }
+        }
+        if (id >= total || page < 0) continue;
+        const uint32_t in_row = id - token[i] * per_token, head = in_row / blocks, block = in_row % blocks;
+        const uint32_t row = offset % kKvGroup;
+        uint8_t *group = cache + kv_group_offset(page, static_cast<int>(head), static_cast<int>(offset),
+                                                 static_cast<int>(p.heads_kv),
+                                                 static_cast<int>(p.page_size) / kKvGroup, dim);
+        uint8_t *to = group + row * kv_row_bytes(dim);
+        if (!is_v) {
+            *reinterpret_cast<uint32_t *>(to + word * 4 * blocks + 4 * block) = bytes;
+        } else if (blocks % 2 == 0) {
+            // two bytes a block and g = 2 word, 2 word + 1: with the neighbour's
+            // they make a word of two blocks, one for each of the two lanes
+            const uint32_t g = 2 * word + (block & 1);
+            *reinterpret_cast<uint32_t *>(to + g * 2 * blocks + 2 * (block & ~1u)) =
+                (block & 1) ? __byte_perm(next, bytes, 0x7632) : __byte_perm(bytes, next, 0x5410);
+        } else {
+            *reinterpret_cast<uint16_t *>(to + 2 * word * 2 * blocks + 2 * block) = static_cast<uint16_t>(bytes);
+            *reinterpret_cast<uint16_t *>(to + (2 * word + 1) * 2 * blocks + 2 * block) = static_cast<uint16_t>(bytes >> 16);
+        }
+        if (quad == 0)
+            *reinterpret_cast<uint16_t *>(group + kv_scale_offset(dim) + 2 * (row * blocks + block)) = f32_to_f16_bits(d);
     }
 }
 
-template <bool kVec>
+template <bool WIDE, int FIXED>
 __global__ void __launch_bounds__(kThreads) kv_append_kernel(const AppendArgs p) {
-    const int blocks = static_cast<int>(p.head_dim / 32);
-    const int64_t per_token = p.heads_kv * blocks;  // q4_0 blocks of K (and of V) of a token
-    const int64_t half = p.tokens * per_token;
-    const int quad = threadIdx.x & 3;
-    const int64_t id = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) >> 2;
-    const bool is_v = id >= half;
-    const int64_t bi = is_v ? id - half : id;
-    const bool live = bi < half;
-    const int64_t token = live ? bi / per_token : 0;
-    const int rest = live ? static_cast<int>(bi % per_token) : 0;
-    const int head = rest / blocks, block = rest % blocks;
-    const int64_t slot = live ? p.slots[token] : -1;
-    const bool write = slot >= 0 && slot < p.num_pages * p.page_size;
-    float v[8] = {};
-    if (write)
-        load8<kVec>(is_v ? p.v_format : p.k_format, is_v ? p.v : p.k,
-                    token * (is_v ? p.ldv : p.ldk) + static_cast<int64_t>(head) * p.head_dim + 32 * block + 8 * quad,
-                    v);
-    float amax = 0.0f, smax = 0.0f;
-    int first = 1 << 30;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if (amax < fabsf(v[i])) amax = fabsf(v[i]), smax = v[i], first = 8 * quad + i;
-#pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
-        const float oa = __shfl_xor_sync(0xffffffffu, amax, o), os = __shfl_xor_sync(0xffffffffu, smax, o);
-        const int oi = __shfl_xor_sync(0xffffffffu, first, o);
-        if (oa > amax || (oa == amax && oi < first)) amax = oa, smax = os, first = oi;
-    }
-    const float d = __fdiv_rn(smax, -8.0f);
-    const float inv = d != 0.0f ? __fdiv_rn(1.0f, d) : 0.0f;
-    uint32_t n[2] = {0, 0};  // nibbles of values 8 quad .. + 3 and + 4 .. + 7, one a byte
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        int q = __float2int_rz(__fadd_rn(__fmul_rn(v[i], inv), 8.5f));
-        q = min(static_cast<int>(static_cast<int8_t>(q)), 15);
-        n[i / 4] |= (static_cast<uint32_t>(q) & 15u) << (8 * (i % 4));
-    }
-    // bytes 8 a .. 8 a + 7 of the block are lanes a (low nibbles) and a + 2
-    // (high nibbles), a = 0, 1: lane a stores the first four, lane a + 2 the
-    // last four, so each needs one word of the other
-    const uint32_t other = __shfl_xor_sync(0xffffffffu, quad < 2 ? n[1] : n[0], 2);
-    const uint32_t bytes = quad < 2 ? n[0] | (other << 4) : other | (n[1] << 4);
-    const int word = 2 * (quad & 1) + (quad >> 1);  // bytes 4 word .. 4 word + 3
-    if (!write) return;
-    const int64_t page = slot / p.page_size;
-    const int offset = static_cast<int>(slot % p.page_size), row = offset % kKvGroup;
-    const int dim = static_cast<int>(p.head_dim);
-    uint8_t *group = (is_v ? p.v_cache : p.k_cache) +
-                     kv_group_offset(page, head, offset, static_cast<int>(p.heads_kv),
-                                     static_cast<int>(p.page_size / kKvGroup), dim);
-    uint8_t *to = group + row * kv_row_bytes(dim);
-    if (!is_v) {
-        *reinterpret_cast<uint32_t *>(to + word * 4 * blocks + 4 * block) = bytes;
-    } else {
-        *reinterpret_cast<uint16_t *>(to + (2 * word) * 2 * blocks + 2 * block) = static_cast<uint16_t>(bytes);
-        *reinterpret_cast<uint16_t *>(to + (2 * word + 1) * 2 * blocks + 2 * block) =
-            static_cast<uint16_t>(bytes >> 16);
-    }
-    if (quad == 0)
-        *reinterpret_cast<uint16_t *>(group + kv_scale_offset(dim) + 2 * (row * blocks + block)) = f32_to_f16_bits(d);
+    const bool is_v = blockIdx.y != 0;
+    const int fmt = is_v ? p.v_format : p.k_format;
+    if (fmt == kOutF32) append<kOutF32, WIDE, FIXED>(p, is_v);
+    else if (fmt == kOutF16) append<kOutF16, WIDE, FIXED>(p, is_v);
+    else append<kOutBF16, WIDE, FIXED>(p, is_v);
 }
 
 }  // namespace
@@ -103,12 +150,14 @@ cudaError_t launch_kv_append(const AppendArgs &p, cudaStream_t s) {
     const auto wide = [](const void *x, int64_t ld, int fmt) {
         return (reinterpret_cast<uintptr_t>(x) & 15u) == 0 && ld % (fmt == kOutF32 ? 4 : 8) == 0;
     };
-    const int64_t threads = 2 * p.tokens * p.heads_kv * (p.head_dim / 32) * 4;
-    const unsigned grid = static_cast<unsigned>((threads + kThreads - 1) / kThreads);
+    const int64_t total = p.tokens * p.heads_kv * (p.head_dim / 32), per_block = kBatch * kThreads / 4;
+    const dim3 grid(static_cast<unsigned>((total + per_block - 1) / per_block), 2);
     if (wide(p.k, p.ldk, p.k_format) && wide(p.v, p.ldv, p.v_format))
-        kv_append_kernel<true><<<grid, kThreads, 0, s>>>(p);
+        p.head_dim == 128  ? kv_append_kernel<true, 4><<<grid, kThreads, 0, s>>>(p)
+        : p.head_dim == 64 ? kv_append_kernel<true, 2><<<grid, kThreads, 0, s>>>(p)
+                           : kv_append_kernel<true, 0><<<grid, kThreads, 0, s>>>(p);
     else
-        kv_append_kernel<false><<<grid, kThreads, 0, s>>>(p);
+        kv_append_kernel<false, 0><<<grid, kThreads, 0, s>>>(p);
     return cudaGetLastError();
 }
 

@@ -86,6 +86,38 @@ PFNG_DEV uint32_t pack_values(int fmt, float a, float b) {
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
+// load_values in two steps, for loops that start several loads before they use
+// the first: the bits, then their values.
+template <int FMT, int N>
+struct RawValues {
+    static constexpr int kWords = FMT == kOutF32 ? N : (N + 1) / 2;
+    uint32_t w[kWords];
+    PFNG_DEV void zero() {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) w[i] = 0;
+    }
+    PFNG_DEV void load(const void *p, int64_t at) {
+        const uint8_t *b = static_cast<const uint8_t *>(p) + at * (FMT == kOutF32 ? 4 : 2);
+        if constexpr (N == 1) {
+            w[0] = FMT == kOutF32 ? *reinterpret_cast<const uint32_t *>(b) : *reinterpret_cast<const uint16_t *>(b);
+        } else if constexpr (kWords == 2) {
+            const uint2 q = *reinterpret_cast<const uint2 *>(b);
+            w[0] = q.x, w[1] = q.y;
+        } else {
+#pragma unroll
+            for (int i = 0; i < kWords; i += 4) {
+                const uint4 q = *reinterpret_cast<const uint4 *>(b + 4 * i);
+                w[i] = q.x, w[i + 1] = q.y, w[i + 2] = q.z, w[i + 3] = q.w;
+            }
+        }
+    }
+    PFNG_DEV float operator[](int i) const {
+        if constexpr (FMT == kOutF32) return __uint_as_float(w[i]);
+        const uint32_t b = (w[i / 2] >> (16 * (i & 1))) & 0xffffu;
+        return FMT == kOutBF16 ? __uint_as_float(b << 16) : f16_bits_to_f32(b);
+    }
+};
+
 // The counterpart of load_values; fp32 -> fp16 / bf16 rounds to nearest even,
 // the one rounding of a result.
 template <int N>

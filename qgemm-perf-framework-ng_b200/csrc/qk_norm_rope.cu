@@ -12,113 +12,153 @@
 // fp32 registers between one read and one write (rounded once, at the write).
 #include "kv_cache.cuh"
 
+#ifndef KT
+#define KT 128
+#define KH 4
+#endif
 namespace pfng {
 namespace {
 
-constexpr int kThreads = 128;
+constexpr int kThreads = KT;
 
 // Elements of slots s .. s + N - 1: N values from a and N from b.  Interleaved
 // pairs are adjacent: 2 N values in a row, b = a + N.
-template <int N>
-PFNG_DEV void slot_elements(const RopeArgs &p, int s, int &a, int &b, bool &turns, bool &adjacent) {
-    const int half = static_cast<int>(p.rot_dim / 2);
+template <int N, bool INTERLEAVED>
+PFNG_DEV void slot_elements(const RopeArgs &p, int s, int &a, int &b, bool &turns) {
+    const int half = static_cast<int>(p.rot_dim) / 2;
     turns = s < half;
-    adjacent = turns && p.interleaved;
     if (turns) {
-        a = p.interleaved ? 2 * s : s;
-        b = p.interleaved ? 2 * s + N : s + half;
+        a = INTERLEAVED ? 2 * s : s;
+        b = INTERLEAVED ? 2 * s + N : s + half;
     } else {
-        a = static_cast<int>(p.rot_dim) + s - half;
+        a = half + s;
         b = a + static_cast<int>(p.head_dim - p.rot_dim) / 2;
     }
 }
 
-template <int N>
+// H heads of one token (all query or all key heads) by one group of `lanes`
+// lanes: their loads are in flight together, and cosines, sines and weights
+// are read once for all of them.
+template <int FMT, int N, int H, bool INTERLEAVED>
 __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const RopeArgs p, int lanes) {
-    const int heads = static_cast<int>(p.heads_q + p.heads_k);
-    const int lane = threadIdx.x & 31, sub = lane % lanes;
-    const int slots = static_cast<int>(p.head_dim / 2);
-    const int per_warp = 32 / lanes;
-    const int64_t rows = p.tokens * heads;
-    const int64_t row = ((static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) >> 5) * per_warp + lane / lanes;
-    const bool live = row < rows;
-    const int64_t token = live ? row / heads : 0;
-    const int head = live ? static_cast<int>(row % heads) : 0;
-    const bool is_q = head < p.heads_q;
+    const uint32_t q_parts = static_cast<uint32_t>((p.heads_q + H - 1) / H);
+    const uint32_t parts = q_parts + static_cast<uint32_t>((p.heads_k + H - 1) / H);
+    const int sub = threadIdx.x % lanes;
+    const uint32_t part = blockIdx.x * (kThreads / lanes) + threadIdx.x / lanes;
+    const uint32_t at_token = part / parts, at_part = part % parts;
+    const bool live = at_token < p.tokens;
+    const int64_t token = live ? at_token : 0;
+    const bool is_q = at_part < q_parts;
+    const int heads = static_cast<int>(is_q ? p.heads_q : p.heads_k);
+    const int head0 = static_cast<int>(is_q ? at_part : at_part - q_parts) * H;
+    const int count = live ? min(H, heads - head0) : 0;
+    const int dim = static_cast<int>(p.head_dim), slots = dim / 2;
+    const int64_t from = token * p.ldx + static_cast<int64_t>((is_q ? 0 : p.heads_q) + head0) * dim;
+    const int64_t pos = p.positions[token];
+    // slots (i * lanes + sub) * N: head_dim <= 512, and <= 256 for several heads
+    constexpr int kPieces = H > 1 ? 1 : 8 / N;
+    RawValues<FMT, N> x[H][kPieces][2];
+#pragma unroll
+    for (int h = 0; h < H; ++h)
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            const int s = (i * lanes + sub) * N;
+            x[h][i][0].zero();
+            x[h][i][1].zero();
+            if (h < count && s < slots) {
+                int a, b;
+                bool turns;
+                slot_elements<N, INTERLEAVED>(p, s, a, b, turns);
+                x[h][i][0].load(p.x, from + h * dim + a);
+                x[h][i][1].load(p.x, from + h * dim + b);
+            }
+        }
     const float *weight = is_q ? p.q_weight : p.k_weight;
-    float v[2][8 / N][N] = {};
-    // slots of this lane: sub * N + i * lanes * N
-    constexpr int kMost = 8 / N;  // head_dim <= 512: at most kMost pieces a lane
-    const int pieces = (slots + lanes * N - 1) / (lanes * N);
-    float sum = 0.0f;
+    float scale[H];
 #pragma unroll
-    for (int i = 0; i < kMost; ++i) {
-        const int s = (i * lanes + sub) * N;
-        if (i < pieces && live && s < slots) {
-            int a, b;
-            bool turns, adjacent;
-            slot_elements<N>(p, s, a, b, turns, adjacent);
-            const int64_t at = token * p.ldx + static_cast<int64_t>(head) * p.head_dim;
-            load_values<N>(p.in_format, p.x, at + a, v[0][i]);
-            load_values<N>(p.in_format, p.x, at + b, v[1][i]);
+    for (int h = 0; h < H; ++h) scale[h] = 1.0f;
+    if (weight) {
 #pragma unroll
-            for (int j = 0; j < N; ++j) sum += v[0][i][j] * v[0][i][j] + v[1][i][j] * v[1][i][j];
+        for (int h = 0; h < H; ++h) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i)
+#pragma unroll
+                for (int j = 0; j < N; ++j) sum += x[h][i][0][j] * x[h][i][0][j] + x[h][i][1][j] * x[h][i][1][j];
+            for (int o = 1; o < lanes; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            scale[h] = 1.0f / sqrtf(sum / static_cast<float>(dim) + p.eps);
         }
     }
-    for (int o = 1; o < lanes; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (!live) return;
-    const float scale = weight ? 1.0f / sqrtf(sum / static_cast<float>(p.head_dim) + p.eps) : 1.0f;
-    const int64_t pos = p.positions[token];
+    if (count <= 0) return;
     const bool known = pos >= 0 && pos < p.max_pos;
-    void *out = is_q ? p.q_out : p.k_out;
-    const int64_t to = is_q ? token * p.ldq + static_cast<int64_t>(head) * p.head_dim
-                            : token * p.ldk + static_cast<int64_t>(head - p.heads_q) * p.head_dim;
     // padding rows (no position) are zeros, a position past the table is NaN
     const float blank = pos < 0 ? 0.0f : __int_as_float(0x7fffffff);
+    void *out = is_q ? p.q_out : p.k_out;
+    const int64_t to = token * (is_q ? p.ldq : p.ldk) + static_cast<int64_t>(head0) * dim;
 #pragma unroll
-    for (int i = 0; i < kMost; ++i) {
+    for (int i = 0; i < kPieces; ++i) {
         const int s = (i * lanes + sub) * N;
-        if (i >= pieces || s >= slots) continue;
+        if (s >= slots) continue;
         int a, b;
-        bool turns, adjacent;
-        slot_elements<N>(p, s, a, b, turns, adjacent);
-        float c[N], z[N], u[N], w[N];
+        bool turns;
+        slot_elements<N, INTERLEAVED>(p, s, a, b, turns);
+        const bool adjacent = INTERLEAVED && turns;
+        float c[N], z[N], w0[N], w1[N];
 #pragma unroll
-        for (int j = 0; j < N; ++j) c[j] = 1.0f, z[j] = 0.0f;
+        for (int j = 0; j < N; ++j) c[j] = 1.0f, z[j] = 0.0f, w0[j] = w1[j] = 1.0f;
         if (turns && known) {
             load_values<N>(kOutF32, p.cos_sin, pos * p.rot_dim + s, c);
             load_values<N>(kOutF32, p.cos_sin, pos * p.rot_dim + p.rot_dim / 2 + s, z);
         }
-        // adjacent pairs come in as 2 N values in a row
-        float first[N], second[N];
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const int e0 = 2 * j, e1 = 2 * j + 1;
-            first[j] = adjacent ? (e0 < N ? v[0][i][e0 % N] : v[1][i][e0 % N]) : v[0][i][j];
-            second[j] = adjacent ? (e1 < N ? v[0][i][e1 % N] : v[1][i][e1 % N]) : v[1][i][j];
+        if (weight) {
+            load_values<N>(kOutF32, weight, a, w0);
+            load_values<N>(kOutF32, weight, b, w1);
         }
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const int fa = adjacent ? a + 2 * j : a + j, sa = adjacent ? a + 2 * j + 1 : b + j;
-            const float x0 = weight ? first[j] * scale * weight[fa] : first[j];
-            const float x1 = weight ? second[j] * scale * weight[sa] : second[j];
-            u[j] = known ? x0 * c[j] - x1 * z[j] : blank;
-            w[j] = known ? x1 * c[j] + x0 * z[j] : blank;
-        }
-        if (adjacent) {
-            float lo[N], hi[N];
+        for (int h = 0; h < H; ++h) {
+            if (h >= count) break;
+            float u[N], w[N];  // the values of a .. and b .., normed
 #pragma unroll
             for (int j = 0; j < N; ++j) {
-                lo[j] = (j & 1) ? w[j / 2] : u[j / 2];
-                hi[j] = ((N + j) & 1) ? w[(N + j) / 2] : u[(N + j) / 2];
+                u[j] = weight ? x[h][i][0][j] * scale[h] * w0[j] : x[h][i][0][j];
+                w[j] = weight ? x[h][i][1][j] * scale[h] * w1[j] : x[h][i][1][j];
             }
-            store_values<N>(p.out_format, out, to + a, lo);
-            store_values<N>(p.out_format, out, to + b, hi);
-        } else {
-            store_values<N>(p.out_format, out, to + a, u);
-            store_values<N>(p.out_format, out, to + b, w);
+            // pair j: (u[j], w[j]); adjacent: values 2 j and 2 j + 1 of the 2 N in u, w
+            float y[2 * N];
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const float v0 = adjacent ? (2 * j < N ? u[(2 * j) % N] : w[(2 * j) % N]) : u[j];
+                const float v1 = adjacent ? (2 * j + 1 < N ? u[(2 * j + 1) % N] : w[(2 * j + 1) % N]) : w[j];
+                y[j] = known ? v0 * c[j] - v1 * z[j] : blank;
+                y[N + j] = known ? v1 * c[j] + v0 * z[j] : blank;
+            }
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                u[j] = adjacent ? y[(j & 1) * N + j / 2] : y[j];
+                w[j] = adjacent ? y[((N + j) & 1) * N + (N + j) / 2] : y[N + j];
+            }
+            store_values<N>(p.out_format, out, to + h * dim + a, u);
+            store_values<N>(p.out_format, out, to + h * dim + b, w);
         }
     }
+}
+
+template <int N, int H>
+cudaError_t launch(const RopeArgs &p, int lanes, cudaStream_t s) {
+    const int64_t parts = p.tokens * ((p.heads_q + H - 1) / H + (p.heads_k + H - 1) / H);
+    const int64_t per_block = kThreads / lanes;
+    const unsigned grid = static_cast<unsigned>((parts + per_block - 1) / per_block);
+    const auto run = [&](auto kernel) { kernel<<<grid, kThreads, 0, s>>>(p, lanes); };
+    if (p.interleaved) {
+        if (p.in_format == kOutF32) run(qk_norm_rope_kernel<kOutF32, N, H, true>);
+        else if (p.in_format == kOutF16) run(qk_norm_rope_kernel<kOutF16, N, H, true>);
+        else run(qk_norm_rope_kernel<kOutBF16, N, H, true>);
+    } else {
+        if (p.in_format == kOutF32) run(qk_norm_rope_kernel<kOutF32, N, H, false>);
+        else if (p.in_format == kOutF16) run(qk_norm_rope_kernel<kOutF16, N, H, false>);
+        else run(qk_norm_rope_kernel<kOutBF16, N, H, false>);
+    }
+    return cudaGetLastError();
 }
 
 bool aligned_to(const void *p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
@@ -132,18 +172,14 @@ cudaError_t launch_qk_norm_rope(const RopeArgs &p, cudaStream_t s) {
     const bool vec = p.rot_dim % 8 == 0 && p.head_dim % 8 == 0 && p.ldx % 4 == 0 && p.ldq % 4 == 0 &&
                      p.ldk % 4 == 0 && aligned_to(p.x, vec_bytes(p.in_format)) &&
                      aligned_to(p.q_out, vec_bytes(p.out_format)) && aligned_to(p.k_out, vec_bytes(p.out_format)) &&
-                     aligned_to(p.cos_sin, 16);
-    const int64_t rows = p.tokens * (p.heads_q + p.heads_k);
+                     aligned_to(p.cos_sin, 16) && aligned_to(p.q_weight, 16) && aligned_to(p.k_weight, 16);
     const int slots = static_cast<int>(p.head_dim / 2);
     int lanes = 1;
     while (lanes < 32 && lanes * (vec ? 4 : 1) < slots) lanes *= 2;
-    const int64_t per_block = kThreads / lanes;
-    const unsigned grid = static_cast<unsigned>((rows + per_block - 1) / per_block);
-    if (vec)
-        qk_norm_rope_kernel<4><<<grid, kThreads, 0, s>>>(p, lanes);
-    else
-        qk_norm_rope_kernel<1><<<grid, kThreads, 0, s>>>(p, lanes);
-    return cudaGetLastError();
+    if (!vec) return launch<1, 1>(p, lanes, s);
+    // Four heads a lane group where that still leaves every SM its threads.
+    const bool many = p.head_dim <= 256 && p.tokens * (p.heads_q + p.heads_k) * lanes >= int64_t{4} * 2048 * device_sm_count();
+    return many ? launch<4, KH>(p, lanes, s) : launch<4, 1>(p, lanes, s);
 }
 
 }  // namespace pfng
