@@ -13,12 +13,13 @@
 //                and write the output
 //   warps 8-11   dequantization: nibbles and scales of a tile -> fp16 operand
 //                rows in the 128-byte swizzled layout
-//   warp 12      issues the MMAs (one thread)
+//   warp 12      issues the MMAs
 //   warp 13      copies the tiles' groups from the pages (bulk copies, a ring
-//                of three raw K or V tiles)
-// One dequantization serves 256 rows: 13 instructions per 8 values, a fifth of
-// the issue slots that the exponentials leave.  Bound: 16 exponentials per
-// cycle and SM (2048 cycles for 256 x 128) and as many cycles of MMA.
+//                of six raw K or V tiles)
+// One dequantization serves 256 rows: 13 instructions per 8 values.  Bounds per
+// 256 x 128 step, in cycles: 2048 of MMA, 2048 of exponentials (16 per cycle and
+// SM), about 2300 of shared memory (operands read by the MMAs, dequantized
+// tiles written).
 //
 // Precision: d (n - 8) is rounded to fp16 (2^-12 on average), P to fp16 with
 // the row's largest at 2^8..2^15 (so that small ones stay normal numbers);
@@ -39,8 +40,10 @@ namespace {
 constexpr int kTile = 128;       // rows of a row tile, keys of a key tile
 constexpr int kRows = 2 * kTile;
 constexpr int kThreads = 512;
-constexpr int kRawSlots = 3;
-constexpr int kInfoSlots = 8;
+constexpr int kDequantWarps = 4;
+constexpr int kRawSlots = 6;
+constexpr int kOperands = 3;     // dequantized K or V tiles: unit 2 n is K of key tile n, unit 2 n + 1 its V
+constexpr int kInfoSlots = 16;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNoMax = -3.0e38f;
 constexpr float kLift = 8.0f;    // log2 of P at a renewed maximum
@@ -58,12 +61,11 @@ struct Layout {
     static constexpr uint32_t kOperand = kTile * DIM * 2;  // an operand tile, fp16
     static constexpr uint32_t kRaw = (kTile / kKvGroup) * kv_group_bytes(DIM);
     static constexpr uint32_t kQ = 0;                       // [2 row tiles]
-    static constexpr uint32_t kK = kQ + 2 * kOperand;       // [2]
-    static constexpr uint32_t kV = kK + 2 * kOperand;       // [2]
-    static constexpr uint32_t kRawAt = kV + 2 * kOperand;   // [kRawSlots]
+    static constexpr uint32_t kKV = kQ + 2 * kOperand;      // [kOperands]
+    static constexpr uint32_t kRawAt = kKV + kOperands * kOperand;  // [kRawSlots]
     static constexpr uint32_t kInfo = kRawAt + kRawSlots * kRaw;
     static constexpr uint32_t kBars = kInfo + ((kInfoSlots * sizeof(TileInfo) + 7) & ~7u);
-    static constexpr uint32_t kNumBars = 2 * kRawSlots + 8 + 2 + 2 + 2 + 2;
+    static constexpr uint32_t kNumBars = 2 * kRawSlots + 2 * kOperands + 2 + 4 + 2 + 2;
     static constexpr uint32_t kBytes = kBars + 8 * kNumBars + 16 + 1024;
 };
 
@@ -74,20 +76,41 @@ struct MmaParams {
     int *err;
 };
 
-PFNG_DEV void umma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// The MMAs run in a warp whose control flow is uniform, so that descriptors
+// stay in uniform registers; `leader` is 1 in the one lane that issues.
+PFNG_DEV uint32_t elect_leader() {
+    uint32_t x;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(x));
+    return x;
+}
+PFNG_DEV void umma_f16_ss(uint32_t leader, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 q, %0, 0;\n\t"
+        "setp.ne.b32 p, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%1], %2, %3, %4, p;\n\t}" ::"r"(leader),
+        "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-PFNG_DEV void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+PFNG_DEV void umma_f16_ts(uint32_t leader, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 q, %0, 0;\n\t"
+        "setp.ne.b32 p, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%1], [%2], %3, %4, p;\n\t}" ::"r"(leader),
+        "r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+PFNG_DEV void umma_commit_by(uint32_t leader, uint64_t *bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "setp.ne.b32 q, %0, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%1];\n\t}" ::"r"(leader),
+        "r"(smem_u32(bar))
         : "memory");
 }
 #define PFNG_OUT32(x) \
@@ -194,8 +217,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
     uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::kBars);
     uint64_t *raw_full = bars, *raw_empty = raw_full + kRawSlots;
-    uint64_t *k_full = raw_empty + kRawSlots, *k_empty = k_full + 2, *v_full = k_empty + 2, *v_empty = v_full + 2;
-    uint64_t *s_full = v_empty + 2, *p_full = s_full + 2, *o_full = p_full + 2;
+    uint64_t *op_full = raw_empty + kRawSlots, *op_empty = op_full + kOperands;
+    uint64_t *s_full = op_empty + kOperands, *p_full = s_full + 2, *o_full = p_full + 4;
     uint64_t *q_full = o_full + 2, *mma_done = q_full + 1;
     uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(bars + L::kNumBars);
     TileInfo *infos = reinterpret_cast<TileInfo *>(smem + L::kInfo);
@@ -226,11 +249,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
 
     if (tid == 0) {
         abort_flag = 0;
-        for (int i = 0; i < kRawSlots; ++i) mbar_init(&raw_full[i], 1), mbar_init(&raw_empty[i], 4);
+        for (int i = 0; i < kRawSlots; ++i) mbar_init(&raw_full[i], 1), mbar_init(&raw_empty[i], kDequantWarps);
+        for (int i = 0; i < kOperands; ++i) mbar_init(&op_full[i], kDequantWarps), mbar_init(&op_empty[i], 1);
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&k_full[i], 4), mbar_init(&k_empty[i], 1);
-            mbar_init(&v_full[i], 4), mbar_init(&v_empty[i], 1);
-            mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 4), mbar_init(&o_full[i], 1);
+            mbar_init(&s_full[i], 1), mbar_init(&o_full[i], 1);
+            mbar_init(&p_full[2 * i], 4), mbar_init(&p_full[2 * i + 1], 4);
+
         }
         mbar_init(q_full, 4 * row_tiles);
         mbar_init(mma_done, 1);
@@ -246,6 +270,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(tmem_holder);
     const uint32_t base = smem_u32(smem);
 
+    // Registers: 512 threads x 128 at launch, 2 x 192 + 80 + 48 a thread of the
+    // four warpgroups after this.
     if (warp < 8) {
         // ---------------- softmax ----------------
         registers_up<192>();
@@ -331,24 +357,28 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
                     break;
                 }
                 tc_fence_after();
+                const uint32_t groups = infos[n % kInfoSlots].groups;
+                if (n > 0) bad_keys(n - 1);  // V of the last tile is complete: this tile's MMA came after its own
+                const int from = lo - (first + n) * kTile, to = hi - (first + n) * kTile;
+                const bool masked = __any_sync(0xffffffffu, from > 0 || to < kTile) || groups != 0xffu;
                 uint32_t s[kTile];
 #pragma unroll
                 for (int c = 0; c < kTile; c += 32) tmem_ld32(s_at + c, s + c);
-                const uint32_t groups = infos[n % kInfoSlots].groups;
-                if (n > 0) bad_keys(n - 1);  // V of the last tile is complete: this tile's MMA came after its own
                 tmem_wait_ld<kTile>(s);
-                const int key0 = (first + n) * kTile;
-                if (__any_sync(0xffffffffu, key0 < lo || key0 + kTile > hi) || groups != 0xffu) {
-                    const int from = lo - key0, to = hi - key0;
+                if (masked) {  // what a row does not see is -inf
 #pragma unroll
                     for (int c = 0; c < kTile; ++c)
                         if (!(c >= from && c < to && ((groups >> (c / kKvGroup)) & 1u))) s[c] = 0xff800000u;
                 }
-                float top = fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+                float tops[4];
 #pragma unroll
-                for (int c = 2; c < kTile; c += 2)
-                    top = fmaxf(fmaxf(top, __uint_as_float(s[c])), __uint_as_float(s[c + 1]));
-                top *= mul;
+                for (int x = 0; x < 4; ++x) tops[x] = -INFINITY;
+#pragma unroll
+                for (int x = 0; x < kTile; x += 8)
+#pragma unroll
+                    for (int y = 0; y < 4; ++y)
+                        tops[y] = fmaxf(fmaxf(tops[y], __uint_as_float(s[x + y])), __uint_as_float(s[x + y + 4]));
+                const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * mul;
                 if (__any_sync(0xffffffffu, top > m + (kLift + kSlack))) {
                     const float m_new = fmaxf(top - kLift, m);
                     const float f = exp2_approx(m - m_new);
@@ -361,27 +391,29 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
                             tmem_ld32(o_at + c, o);
                             tmem_wait_ld<32>(o);
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+                            for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
                             tmem_st32(o_at + c, o);
                         }
                     }
                 }
                 float sum[4] = {};
 #pragma unroll
-                for (int c = 0; c < kTile; c += 2) {
-                    const float x = exp2_approx(fmaf(__uint_as_float(s[c]), mul, -m));
-                    const float y = exp2_approx(fmaf(__uint_as_float(s[c + 1]), mul, -m));
-                    sum[c & 2] += x;
-                    sum[(c & 2) + 1] += y;
-                    s[c / 2] = h2(__floats2half2_rn(x, y));
-                    if (c == kTile / 2 - 2) tmem_st32(s_at, s);
+                for (int h = 0; h < 2; ++h) {  // by halves of the keys: their part of O += P V can start
+#pragma unroll
+                    for (int x = 64 * h; x < 64 * h + 64; x += 2) {
+                        const float u = exp2_approx(fmaf(__uint_as_float(s[x]), mul, -m));
+                        const float w = exp2_approx(fmaf(__uint_as_float(s[x + 1]), mul, -m));
+                        sum[x & 2] += u;
+                        sum[(x & 2) + 1] += w;
+                        s[x / 2] = h2(__floats2half2_rn(u, w));
+                    }
+                    tmem_st32(s_at + 32 * h, s + 32 * h);  // P over S
+                    tmem_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&p_full[2 * i + h]);
                 }
-                tmem_st32(s_at + 32, s + 32);
                 l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                tmem_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[i]);
             }
             if (ok && count > 0) {
                 ok = wait_bar(&o_full[i], 0, &abort_flag, mp.err, kErrWaitFull);
@@ -444,117 +476,165 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
         uint32_t magic;
         asm volatile("mov.b32 %0, 0x64006400;" : "=r"(magic));
         constexpr int kQuads = DIM / 32;  // 16-byte pieces of a row
+        constexpr int kLoads = kQuads * kTile / (32 * kDequantWarps);  // pieces of a thread
         bool ok = true;
         for (int j = 0; j < 2 * count; ++j) {
-            const int n = j >> 1, slot = j % kRawSlots, stage = n & 1;
+            const int n = j >> 1, slot = j % kRawSlots, buf = j % kOperands;
             const bool is_v = j & 1;
-            if (!wait_bar(&raw_full[slot], (j / kRawSlots) & 1, &abort_flag, mp.err, kErrWaitFull) ||
-                (n >= 2 && !wait_bar(is_v ? &v_empty[stage] : &k_empty[stage], ((n >> 1) - 1) & 1, &abort_flag, mp.err,
-                                     kErrWaitEmpty))) {
+            if (!wait_bar(&raw_full[slot], (j / kRawSlots) & 1, &abort_flag, mp.err, kErrWaitFull)) {
                 ok = false;
                 break;
             }
             const uint8_t *raw = smem + L::kRawAt + slot * L::kRaw;
-            uint8_t *to = smem + (is_v ? L::kV : L::kK) + stage * L::kOperand;
             TileInfo &info = infos[n % kInfoSlots];
             const uint32_t groups = info.groups;
             const int keys = seq - (first + n) * kTile;  // rows past the last key are zeros
+            // the whole tile into registers, so that its slot can be refilled
+            uint4 words[kLoads];
+            uint32_t scales[kLoads][kBlocks / 2];
 #pragma unroll
-            for (int i = 0; i < kQuads; ++i) {
-                const int idx = i * 128 + t, row = idx / kQuads, u = idx % kQuads;
+            for (int i = 0; i < kLoads; ++i) {
+                const int idx = i * (32 * kDequantWarps) + t, row = idx / kQuads, u = idx % kQuads;
                 const uint8_t *gr = raw + (row / kKvGroup) * kv_group_bytes(DIM);
-                const uint4 w = *reinterpret_cast<const uint4 *>(gr + (row % kKvGroup) * kv_row_bytes(DIM) + 16 * u);
-                const bool valid = row < keys && ((groups >> (row / kKvGroup)) & 1u);
-                uint32_t sc[kBlocks / 2];
+                words[i] = *reinterpret_cast<const uint4 *>(gr + (row % kKvGroup) * kv_row_bytes(DIM) + 16 * u);
 #pragma unroll
-                for (int b = 0; b < kBlocks / 2; ++b) {
-                    sc[b] = *reinterpret_cast<const uint32_t *>(gr + kv_scale_offset(DIM) + (row % kKvGroup) * (DIM / 16) + 4 * b);
-                    if (!valid) sc[b] = 0;
-                }
+                for (int b = 0; b < kBlocks / 2; ++b)
+                    scales[i][b] = *reinterpret_cast<const uint32_t *>(gr + kv_scale_offset(DIM) +
+                                                                       (row % kKvGroup) * (DIM / 16) + 4 * b);
+            }
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const int row = (i * (32 * kDequantWarps) + t) / kQuads;
+                const bool valid = row < keys && ((groups >> (row / kKvGroup)) & 1u);
+#pragma unroll
+                for (int b = 0; b < kBlocks / 2; ++b)
+                    if (!valid) scales[i][b] = 0;
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&raw_empty[slot]);
+            if (j >= kOperands &&
+                !wait_bar(&op_empty[buf], ((j / kOperands) - 1) & 1, &abort_flag, mp.err, kErrWaitEmpty)) {
+                ok = false;
+                break;
+            }
+            uint8_t *to = smem + L::kKV + buf * L::kOperand;
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const int idx = i * (32 * kDequantWarps) + t, row = idx / kQuads, u = idx % kQuads;
                 uint32_t s[4];
                 if (is_v) {
                     bool bad = false;
 #pragma unroll
                     for (int b = 0; b < kBlocks / 2; ++b)
-                        bad |= (sc[b] & 0x7c00u) == 0x7c00u || (sc[b] & 0x7c000000u) == 0x7c000000u;
+                        bad |= (scales[i][b] & 0x7c00u) == 0x7c00u || (scales[i][b] & 0x7c000000u) == 0x7c000000u;
                     if (bad) {
 #pragma unroll
-                        for (int b = 0; b < kBlocks / 2; ++b) sc[b] = 0;
+                        for (int b = 0; b < kBlocks / 2; ++b) scales[i][b] = 0;
                         if (u == 0) atomicOr(&info.bad[row >> 5], 1u << (row & 31));
                     }
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) s[x] = sc[kBlocks == 4 ? (x & 1) : 0];
+                    for (int x = 0; x < 4; ++x) s[x] = scales[i][kBlocks == 4 ? (x & 1) : 0];
                 } else {
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
                         const int b = x % kBlocks;
-                        s[x] = __byte_perm(sc[b / 2], 0, (b & 1) ? 0x3232 : 0x1010);
+                        s[x] = __byte_perm(scales[i][b / 2], 0, (b & 1) ? 0x3232 : 0x1010);
                     }
                 }
-                const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+                const uint32_t w[4] = {words[i].x, words[i].y, words[i].z, words[i].w};
 #pragma unroll
                 for (int x = 0; x < 4; ++x)
-                    *reinterpret_cast<uint4 *>(to + operand_at(row, 4 * u + x)) = unpack_word(words[x], s[x], magic);
+                    *reinterpret_cast<uint4 *>(to + operand_at(row, 4 * u + x)) = unpack_word(w[x], s[x], magic);
             }
             fence_proxy_async_smem();
             __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(is_v ? &v_full[stage] : &k_full[stage]);
-                mbar_arrive(&raw_empty[slot]);
-            }
+            if (lane == 0) mbar_arrive(&op_full[buf]);
         }
         if (!ok) abort_flag = 1;
     } else {
         registers_down<48>();
-        if (warp == 12 && lane == 0) {
+        if (warp == 12) {
             // ---------------- MMA issue ----------------
+            const uint32_t leader = elect_leader();
+            // The tensor cores idle whenever this thread is late, so it does
+            // little more than wait.  Descriptors differ by their address
+            // field, in the low word, only.  (A thread per row tile measured
+            // 13 % slower: MMAs of two accumulators then alternate.)
             constexpr uint32_t kIdescS = idesc_f16(kTile, false), kIdescO = idesc_f16(DIM, true);
-            bool ok = count > 0 && wait_bar(q_full, 0, &abort_flag, mp.err, kErrWaitFull);
-            const auto scores = [&](int i, int stage) {
+            constexpr uint32_t kHalf = (kTile * 128) >> 4, kBuf = L::kOperand >> 4;
+            const uint64_t q_desc = sw128_desc(base + L::kQ);
+            const uint64_t k_desc = sw128_desc(base + L::kKV), v_desc0 = v_desc(base + L::kKV);
+            bool ok = count > 0;
+            const auto scores = [&](int i, uint32_t buf) {  // S_i = Q_i K^T
+                const uint64_t q = q_desc + i * kBuf, k = k_desc + buf * kBuf;
 #pragma unroll
-                for (int k = 0; k < DIM / 16; ++k) {
-                    const uint32_t off = (k >> 2) * (kTile * 128u) + (k & 3) * 32u;
-                    umma_f16_ss(tmem + i * kTile, sw128_desc(base + L::kQ + i * L::kOperand + off),
-                                sw128_desc(base + L::kK + stage * L::kOperand + off), kIdescS, k > 0);
-                }
-                umma_commit(&s_full[i]);
+                for (int x = 0; x < DIM / 16; ++x)
+                    umma_f16_ss(leader, tmem + i * kTile, q + (x >> 2) * kHalf + (x & 3) * 2, k + (x >> 2) * kHalf + (x & 3) * 2,
+                                kIdescS, x > 0);
+                umma_commit_by(leader, &s_full[i]);
             };
-            if (ok) ok = wait_bar(&k_full[0], 0, &abort_flag, mp.err, kErrWaitFull);
+            const auto ready = [&](uint64_t *bar, uint32_t parity) {
+                return __all_sync(0xffffffffu, mbar_test_wait(bar, parity) ||
+                                                   wait_bar(bar, parity, &abort_flag, mp.err, kErrWaitFull)) != 0;
+            };
+            if (ok) ok = ready(q_full, 0) && ready(&op_full[0], 0);
             if (ok) {
                 tc_fence_after();
-                for (int i = 0; i < row_tiles; ++i) scores(i, 0);
-                umma_commit(&k_empty[0]);
+                scores(0, 0);
+                if (row_tiles > 1) scores(1, 0);
+                umma_commit_by(leader, &op_empty[0]);
             }
+            uint32_t vb = 1, v_phase = 0;  // buffer of V(n); K(n + 1) is in the one after it
+#pragma unroll 1
             for (int n = 0; n < count && ok; ++n) {
-                const int stage = n & 1, next = (n + 1) & 1;
-                ok = wait_bar(&v_full[stage], (n >> 1) & 1, &abort_flag, mp.err, kErrWaitFull);
-                if (ok && n + 1 < count) ok = wait_bar(&k_full[next], ((n + 1) >> 1) & 1, &abort_flag, mp.err, kErrWaitFull);
+                const uint32_t kb = vb + 1 == kOperands ? 0 : vb + 1, k_phase = vb + 1 == kOperands ? v_phase ^ 1 : v_phase;
+                const bool more = n + 1 < count;
+                const uint64_t v = v_desc0 + vb * kBuf;
+                ok = ready(&op_full[vb], v_phase);
+#pragma unroll 1
                 for (int i = 0; i < row_tiles && ok; ++i) {
-                    ok = wait_bar(&p_full[i], n & 1, &abort_flag, mp.err, kErrWaitFull);
-                    if (!ok) break;
-                    tc_fence_after();
 #pragma unroll
-                    for (int k = 0; k < kTile / 16; ++k)
-                        umma_f16_ts(tmem + 256 + i * kTile, tmem + i * kTile + 8 * k,
-                                    v_desc(base + L::kV + stage * L::kOperand + k * 2048u), kIdescO, n > 0 || k > 0);
-                    if (i == row_tiles - 1) umma_commit(&v_empty[stage]);
-                    if (n + 1 < count) {
-                        scores(i, next);
-                        if (i == row_tiles - 1) umma_commit(&k_empty[next]);
-                    } else {
-                        umma_commit(&o_full[i]);
+                    for (int h = 0; h < 2 && ok; ++h) {  // O_i += P_i V, by halves of the keys
+                        ok = ready(&p_full[2 * i + h], n & 1);
+                        tc_fence_after();
+                        if (!ok) break;
+#pragma unroll
+                        for (int x = 4 * h; x < 4 * h + 4; ++x)
+                            umma_f16_ts(leader, tmem + 256 + i * kTile, tmem + i * kTile + 8 * x, v + x * (2048 >> 4), kIdescO,
+                                        n > 0 || x > 0);
                     }
+                    if (!ok) break;
+                    if (i == row_tiles - 1) umma_commit_by(leader, &op_empty[vb]);
+                    if (!more) {
+                        umma_commit_by(leader, &o_full[i]);
+                        continue;
+                    }
+                    if (i == 0) ok = ready(&op_full[kb], k_phase);
+                    if (!ok) break;
+                    scores(i, kb);
+                    if (i == row_tiles - 1) umma_commit_by(leader, &op_empty[kb]);
                 }
+                vb = kb + 1 == kOperands ? 0 : kb + 1;
+                v_phase = kb + 1 == kOperands ? k_phase ^ 1 : k_phase;
             }
             if (!ok && count > 0) abort_flag = 1;
-            umma_commit(mma_done);  // TMEM is freed at the end: no MMA may be in flight
+            umma_commit_by(leader, mma_done);  // TMEM is freed at the end: no MMA may be in flight
             if (!mbar_wait(mma_done, 0, mp.err, kErrWaitFull)) abort_flag = 1;
         } else if (warp == 13) {
             // ---------------- copies from the pages ----------------
             const uint64_t policy = l2_policy_evict_normal();
             bool ok = true;
             int j = 0;
-            int page = -1, key = 0;
+            // the pages of a key tile are looked up while the copies before it wait
+            int64_t at = -1, next = -1;  // this lane's group in the caches
+            const auto look_up = [&](int n) {
+                const int key = (first + n) * kTile + lane * kKvGroup;
+                if (n >= count || lane >= kTile / kKvGroup || key >= seq) return int64_t{-1};
+                const int page = attn_page(p, r, key);
+                return page < 0 ? int64_t{-1}
+                                : kv_group_offset(page, head_kv, key % p.page_size, p.heads_kv, p.page_size / kKvGroup, DIM);
+            };
+            next = look_up(0);
             for (; j < 2 * count; ++j) {
                 const int n = j >> 1, slot = j % kRawSlots;
                 const bool is_v = j & 1;
@@ -563,11 +643,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
                     ok = false;
                     break;
                 }
-                if (!is_v) {
-                    key = (first + n) * kTile + lane * kKvGroup;
-                    page = lane < kTile / kKvGroup && key < seq ? attn_page(p, r, key) : -1;
-                }
-                const uint32_t there = __ballot_sync(0xffffffffu, page >= 0);
+                if (!is_v) at = next;
+                const uint32_t there = __ballot_sync(0xffffffffu, at >= 0);
                 if (lane == 0) {
                     if (!is_v) {
                         TileInfo &info = infos[n % kInfoSlots];
@@ -577,11 +654,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
                     mbar_arrive_expect_tx(&raw_full[slot], kv_group_bytes(DIM) * __popc(there));
                 }
                 __syncwarp();
-                if (page >= 0)
+                if (at >= 0)
                     bulk_copy_g2s(smem + L::kRawAt + slot * L::kRaw + lane * kv_group_bytes(DIM),
-                                  (is_v ? p.v_cache : p.k_cache) + kv_group_offset(page, head_kv, key % p.page_size, p.heads_kv,
-                                                                                   p.page_size / kKvGroup, DIM),
-                                  kv_group_bytes(DIM), &raw_full[slot], policy);
+                                  (is_v ? p.v_cache : p.k_cache) + at, kv_group_bytes(DIM), &raw_full[slot], policy);
+                if (!is_v) next = look_up(n + 1);
             }
             if (!ok) abort_flag = 1;
             // copies in flight end before the CTA does

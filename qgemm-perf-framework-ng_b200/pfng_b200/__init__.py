@@ -443,25 +443,42 @@ class KvPlan(typing.NamedTuple):
     counts: typing.Any     # [3] new tokens, pages wanted from the free list, new tokens without a page
 
 
-_value_formats = {}
+# These calls are made several times per layer and decode step, where the host's time counts: names are looked up
+# once, and the current stream is read without building a Stream object.
+_value_formats = {}  # torch dtype -> code, and code or name -> torch dtype
+
+
+def _formats() -> dict:
+    if not _value_formats:
+        import torch
+        for code, name, dtype in ((OUT_F32, "f32", torch.float32), (OUT_F16, "f16", torch.float16),
+                                  (OUT_BF16, "bf16", torch.bfloat16)):
+            _value_formats[dtype] = code
+            _value_formats[code] = _value_formats[name] = dtype
+    return _value_formats
 
 
 def _value_format(t) -> int:
     """Format code of a tensor's values (fp32, fp16 or bf16)."""
-    if not _value_formats:
-        import torch
-        _value_formats.update({torch.float32: OUT_F32, torch.float16: OUT_F16, torch.bfloat16: OUT_BF16})
-    if t.dtype not in _value_formats or t.stride(-1) != 1:
+    fmt = _formats().get(t.dtype)
+    if fmt is None or t.stride(-1) != 1:
         raise PfngError(ERR_INVALID_ARGUMENT, f"values of {t.dtype} with strides {tuple(t.stride())}")
-    return _value_formats[t.dtype]
+    return fmt
 
 
 def _value_tensor(fmt, rows: int, cols: int, device):
     import torch
-    fmt = _fmt(fmt)
-    if fmt not in (OUT_F32, OUT_F16, OUT_BF16):
+    dtype = _formats().get(fmt) if isinstance(fmt, (int, str)) else None
+    if dtype is None:
         raise PfngError(ERR_INVALID_ARGUMENT, f"out_format {fmt}")
-    return torch.empty((rows, cols), dtype=(torch.float32, torch.float16, torch.bfloat16)[fmt], device=device)
+    return torch.empty(rows, cols, dtype=dtype, device=device)
+
+
+def _raw_stream(stream, device) -> int:
+    if stream is not None:
+        return stream.cuda_stream
+    import torch
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if device.index is None else device.index)
 
 
 def kv_cache_bytes(num_pages: int, page_size: int, heads_kv: int, head_dim: int) -> int:
@@ -475,15 +492,13 @@ def kv_plan(kv_len, q_len, block_table, free_pages, page_size: int, max_tokens: 
     import torch
     n = kv_len.numel()
     if out is None:
-        dev = kv_len.device
-        out = KvPlan(torch.empty(n, dtype=torch.int32, device=dev), torch.empty(n + 1, dtype=torch.int32, device=dev),
-                     torch.empty(max_tokens, dtype=torch.int32, device=dev),
-                     torch.empty(max_tokens, dtype=torch.int64, device=dev),
-                     torch.empty(3, dtype=torch.int32, device=dev))
+        ints = torch.empty(2 * n + 4 + max_tokens, dtype=torch.int32, device=kv_len.device)
+        seq_len, cu_q, positions, counts = ints.split((n, n + 1, max_tokens, 3))
+        out = KvPlan(seq_len, cu_q, positions, torch.empty(max_tokens, dtype=torch.int64, device=kv_len.device), counts)
     _check(lib().pfng_b200_kv_plan(_ptr(kv_len), _ptr(q_len), n, _ptr(block_table), block_table.shape[1],
                                    _ptr(free_pages), free_pages.numel(), page_size, _ptr(out.seq_len), _ptr(out.cu_q),
                                    _ptr(out.positions), _ptr(out.slots), max_tokens, _ptr(out.counts),
-                                   _stream(stream)), "kv_plan")
+                                   _raw_stream(stream, kv_len.device)), "kv_plan")
     return out
 
 
@@ -502,13 +517,13 @@ def qk_norm_rope(x, positions, cos_sin, heads_q: int, heads_k: int, head_dim: in
     _check(lib().pfng_b200_qk_norm_rope(
         _ptr(x), _value_format(x), x.stride(0), _ptr(q_weight), _ptr(k_weight), eps, _ptr(positions), _ptr(cos_sin),
         cos_sin.shape[0], cos_sin.shape[1], 1 if interleaved else 0, _ptr(q_out), q_out.stride(0), _ptr(k_out),
-        k_out.stride(0), fmt, tokens, heads_q, heads_k, head_dim, _stream(stream)), "qk_norm_rope")
+        k_out.stride(0), fmt, tokens, heads_q, heads_k, head_dim, _raw_stream(stream, x.device)), "qk_norm_rope")
     return q_out, k_out
 
 
 def _cache_pages(cache, page_size: int, heads_kv: int, head_dim: int) -> int:
-    page = kv_cache_bytes(1, page_size, heads_kv, head_dim)
-    return cache.numel() // page if page else 0
+    page = heads_kv * page_size * (head_dim // 2 + head_dim // 16)
+    return cache.numel() // page if page > 0 else 0
 
 
 def kv_append_q4_0(k, v, slots, k_cache, v_cache, heads_kv: int, head_dim: int, page_size: int, stream=None) -> None:
@@ -517,7 +532,7 @@ def kv_append_q4_0(k, v, slots, k_cache, v_cache, heads_kv: int, head_dim: int, 
                 _cache_pages(v_cache, page_size, heads_kv, head_dim))
     _check(lib().pfng_b200_kv_append_q4_0(
         _ptr(k), k.stride(0), _value_format(k), _ptr(v), v.stride(0), _value_format(v), _ptr(slots), _ptr(k_cache),
-        _ptr(v_cache), pages, page_size, k.shape[0], heads_kv, head_dim, _stream(stream)), "kv_append_q4_0")
+        _ptr(v_cache), pages, page_size, k.shape[0], heads_kv, head_dim, _raw_stream(stream, k.device)), "kv_append_q4_0")
 
 
 def attention_q4_0(q, k_cache, v_cache, block_table, seq_len, cu_q, heads_q: int, heads_kv: int, head_dim: int,
@@ -536,8 +551,7 @@ def attention_q4_0(q, k_cache, v_cache, block_table, seq_len, cu_q, heads_q: int
         _ptr(q), q.stride(0), _value_format(q), _ptr(k_cache), _ptr(v_cache), pages, page_size, _ptr(block_table),
         block_table.shape[1], _ptr(seq_len), _ptr(cu_q), requests, tokens, max_q, max_kv, heads_q, heads_kv, head_dim,
         head_dim ** -0.5 if scale is None else scale, 1 if causal else 0, window, _ptr(out), out.stride(0),
-        _value_format(out), _ptr(lse), _ptr(ws), 0 if ws is None else ws.numel(), p, _stream(stream)),
-        "attention_q4_0")
+        _value_format(out), _ptr(lse), _ptr(ws), 0 if ws is None else ws.numel(), p, _raw_stream(stream, q.device)), "attention_q4_0")
     return out
 
 
