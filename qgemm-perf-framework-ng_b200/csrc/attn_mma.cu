@@ -11,8 +11,8 @@
 // other's softmax runs.  Roles (512 threads, one CTA per SM):
 //   warps 0-7    softmax, a warpgroup per row tile; they load Q, rescale O
 //                and write the output
-//   warps 8-11   dequantization: nibbles and scales of a tile -> fp16 operand
-//                rows in the 128-byte swizzled layout
+//   warps 8-11, 14, 15  dequantization: nibbles and scales of a tile -> fp16
+//                operand rows in the 128-byte swizzled layout
 //   warp 12      issues the MMAs
 //   warp 13      copies the tiles' groups from the pages (bulk copies, a ring
 //                of six raw K or V tiles)
@@ -40,7 +40,8 @@ namespace {
 constexpr int kTile = 128;       // rows of a row tile, keys of a key tile
 constexpr int kRows = 2 * kTile;
 constexpr int kThreads = 512;
-constexpr int kDequantWarps = 4;
+constexpr int kDequantWarps = 6;
+constexpr int kGroups = kTile / kKvGroup;  // 16-key groups of a unit: the tasks of the dequantizing warps
 constexpr int kRawSlots = 6;
 constexpr int kOperands = 3;     // dequantized K or V tiles: unit 2 n is K of key tile n, unit 2 n + 1 its V
 constexpr int kInfoSlots = 16;
@@ -249,8 +250,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
 
     if (tid == 0) {
         abort_flag = 0;
-        for (int i = 0; i < kRawSlots; ++i) mbar_init(&raw_full[i], 1), mbar_init(&raw_empty[i], kDequantWarps);
-        for (int i = 0; i < kOperands; ++i) mbar_init(&op_full[i], kDequantWarps), mbar_init(&op_empty[i], 1);
+        for (int i = 0; i < kRawSlots; ++i) mbar_init(&raw_full[i], 1), mbar_init(&raw_empty[i], kGroups);
+        for (int i = 0; i < kOperands; ++i) mbar_init(&op_full[i], kGroups), mbar_init(&op_empty[i], 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s_full[i], 1), mbar_init(&o_full[i], 1);
             mbar_init(&p_full[2 * i], 4), mbar_init(&p_full[2 * i + 1], 4);
@@ -270,7 +271,84 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(tmem_holder);
     const uint32_t base = smem_u32(smem);
 
-    // Registers: 512 threads x 128 at launch, 2 x 192 + 80 + 48 a thread of the
+    // ---------------- dequantization ----------------
+    // The tasks are the 16-key groups of the units in order, dealt to the
+    // warps in turn (8 groups a unit, 6 warps: every warp has the same share of
+    // a step).
+    const auto dequantize = [&](int first_task) {
+        uint32_t magic;
+        asm volatile("mov.b32 %0, 0x64006400;" : "=r"(magic));
+        constexpr int kPieces = DIM / 64;  // 16-byte pieces of a group's rows per lane
+        constexpr int kQuads = DIM / 32;   // pieces of a row
+        int g = first_task, slot = 0, buf = 0;
+        uint32_t raw_phase = 0, op_phase = 1;  // op_empty: the first round does not wait
+        for (int j = 0; j < 2 * count;) {
+            const int n = j >> 1;
+            const bool is_v = j & 1;
+            if (!wait_bar(&raw_full[slot], raw_phase, &abort_flag, mp.err, kErrWaitFull)) return false;
+            const uint8_t *raw = smem + L::kRawAt + slot * L::kRaw + g * kv_group_bytes(DIM);
+            TileInfo &info = infos[n % kInfoSlots];
+            const bool there = (info.groups >> g) & 1u;
+            const int keys = seq - (first + n) * kTile - g * kKvGroup;  // rows past the last key are zeros
+            uint4 words[kPieces];
+            uint32_t scales[kPieces][kBlocks / 2];
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) {
+                const int row = (i * 32 + lane) / kQuads, u = lane % kQuads;
+                words[i] = *reinterpret_cast<const uint4 *>(raw + row * kv_row_bytes(DIM) + 16 * u);
+#pragma unroll
+                for (int b = 0; b < kBlocks / 2; ++b) {
+                    scales[i][b] = *reinterpret_cast<const uint32_t *>(raw + kv_scale_offset(DIM) + row * (DIM / 16) + 4 * b);
+                    if (!there || row >= keys) scales[i][b] = 0;
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&raw_empty[slot]);
+            if (!wait_bar(&op_empty[buf], op_phase, &abort_flag, mp.err, kErrWaitEmpty)) return false;
+            uint8_t *to = smem + L::kKV + buf * L::kOperand;
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) {
+                const int row = g * kKvGroup + (i * 32 + lane) / kQuads, u = lane % kQuads;
+                uint32_t s[4];
+                if (is_v) {
+                    bool bad = false;
+#pragma unroll
+                    for (int b = 0; b < kBlocks / 2; ++b)
+                        bad |= (scales[i][b] & 0x7c00u) == 0x7c00u || (scales[i][b] & 0x7c000000u) == 0x7c000000u;
+                    if (bad) {
+#pragma unroll
+                        for (int b = 0; b < kBlocks / 2; ++b) scales[i][b] = 0;
+                        if (u == 0) atomicOr(&info.bad[row >> 5], 1u << (row & 31));
+                    }
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) s[x] = scales[i][kBlocks == 4 ? (x & 1) : 0];
+                } else {
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        const int b = x % kBlocks;
+                        s[x] = __byte_perm(scales[i][b / 2], 0, (b & 1) ? 0x3232 : 0x1010);
+                    }
+                }
+                const uint32_t w[4] = {words[i].x, words[i].y, words[i].z, words[i].w};
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+                    *reinterpret_cast<uint4 *>(to + operand_at(row, 4 * u + x)) = unpack_word(w[x], s[x], magic);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&op_full[buf]);
+            g += kDequantWarps;
+            if (g >= kGroups) {
+                g -= kGroups;
+                ++j;
+                if (++slot == kRawSlots) slot = 0, raw_phase ^= 1;
+                if (++buf == kOperands) buf = 0, op_phase ^= 1;
+            }
+        }
+        return true;
+    };
+
+    // Registers: 512 threads x 128 at launch, 2 x 192 + 2 x 64 a thread of the
     // four warpgroups after this.
     if (warp < 8) {
         // ---------------- softmax ----------------
@@ -469,90 +547,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
                     p.lse[token * p.heads_q + head] = none ? -INFINITY : (m + log2f(l)) / kLog2e;
             }
         }
-    } else if (warp < 12) {
-        // ---------------- dequantization ----------------
-        registers_down<80>();
-        const int t = tid - 256;
-        uint32_t magic;
-        asm volatile("mov.b32 %0, 0x64006400;" : "=r"(magic));
-        constexpr int kQuads = DIM / 32;  // 16-byte pieces of a row
-        constexpr int kLoads = kQuads * kTile / (32 * kDequantWarps);  // pieces of a thread
-        bool ok = true;
-        for (int j = 0; j < 2 * count; ++j) {
-            const int n = j >> 1, slot = j % kRawSlots, buf = j % kOperands;
-            const bool is_v = j & 1;
-            if (!wait_bar(&raw_full[slot], (j / kRawSlots) & 1, &abort_flag, mp.err, kErrWaitFull)) {
-                ok = false;
-                break;
-            }
-            const uint8_t *raw = smem + L::kRawAt + slot * L::kRaw;
-            TileInfo &info = infos[n % kInfoSlots];
-            const uint32_t groups = info.groups;
-            const int keys = seq - (first + n) * kTile;  // rows past the last key are zeros
-            // the whole tile into registers, so that its slot can be refilled
-            uint4 words[kLoads];
-            uint32_t scales[kLoads][kBlocks / 2];
-#pragma unroll
-            for (int i = 0; i < kLoads; ++i) {
-                const int idx = i * (32 * kDequantWarps) + t, row = idx / kQuads, u = idx % kQuads;
-                const uint8_t *gr = raw + (row / kKvGroup) * kv_group_bytes(DIM);
-                words[i] = *reinterpret_cast<const uint4 *>(gr + (row % kKvGroup) * kv_row_bytes(DIM) + 16 * u);
-#pragma unroll
-                for (int b = 0; b < kBlocks / 2; ++b)
-                    scales[i][b] = *reinterpret_cast<const uint32_t *>(gr + kv_scale_offset(DIM) +
-                                                                       (row % kKvGroup) * (DIM / 16) + 4 * b);
-            }
-#pragma unroll
-            for (int i = 0; i < kLoads; ++i) {
-                const int row = (i * (32 * kDequantWarps) + t) / kQuads;
-                const bool valid = row < keys && ((groups >> (row / kKvGroup)) & 1u);
-#pragma unroll
-                for (int b = 0; b < kBlocks / 2; ++b)
-                    if (!valid) scales[i][b] = 0;
-            }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&raw_empty[slot]);
-            if (j >= kOperands &&
-                !wait_bar(&op_empty[buf], ((j / kOperands) - 1) & 1, &abort_flag, mp.err, kErrWaitEmpty)) {
-                ok = false;
-                break;
-            }
-            uint8_t *to = smem + L::kKV + buf * L::kOperand;
-#pragma unroll
-            for (int i = 0; i < kLoads; ++i) {
-                const int idx = i * (32 * kDequantWarps) + t, row = idx / kQuads, u = idx % kQuads;
-                uint32_t s[4];
-                if (is_v) {
-                    bool bad = false;
-#pragma unroll
-                    for (int b = 0; b < kBlocks / 2; ++b)
-                        bad |= (scales[i][b] & 0x7c00u) == 0x7c00u || (scales[i][b] & 0x7c000000u) == 0x7c000000u;
-                    if (bad) {
-#pragma unroll
-                        for (int b = 0; b < kBlocks / 2; ++b) scales[i][b] = 0;
-                        if (u == 0) atomicOr(&info.bad[row >> 5], 1u << (row & 31));
-                    }
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) s[x] = scales[i][kBlocks == 4 ? (x & 1) : 0];
-                } else {
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        const int b = x % kBlocks;
-                        s[x] = __byte_perm(scales[i][b / 2], 0, (b & 1) ? 0x3232 : 0x1010);
-                    }
-                }
-                const uint32_t w[4] = {words[i].x, words[i].y, words[i].z, words[i].w};
-#pragma unroll
-                for (int x = 0; x < 4; ++x)
-                    *reinterpret_cast<uint4 *>(to + operand_at(row, 4 * u + x)) = unpack_word(w[x], s[x], magic);
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&op_full[buf]);
-        }
-        if (!ok) abort_flag = 1;
     } else {
-        registers_down<48>();
+        registers_down<64>();
         if (warp == 12) {
             // ---------------- MMA issue ----------------
             const uint32_t leader = elect_leader();
@@ -664,6 +660,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
             if (!ok || aborted(&abort_flag))
                 for (int x = max(j - kRawSlots, 0); x < j; ++x)
                     mbar_wait(&raw_full[x % kRawSlots], (x / kRawSlots) & 1, mp.err, kErrWaitFull);
+        } else if (!dequantize(warp < 12 ? warp - 8 : warp - 10)) {
+            abort_flag = 1;
         }
         __syncwarp();
     }
