@@ -31,10 +31,26 @@ PFNG_DEV void attn_visible(const AttnArgs &p, int seq, int q_len, int i, int &lo
     hi = p.causal ? min(pos + 1, seq) : seq;
 }
 
-// Page of key j of request r, -1 for an entry outside the cache.
-PFNG_DEV int attn_page(const AttnArgs &p, int64_t r, int j) {
-    const int page = p.table[r * p.max_pages + j / p.page_size];
-    return page >= 0 && page < p.num_pages ? page : -1;
+// Which page of a request holds key j, and the 16-token group within it.  The
+// division by the page size is a multiplication by ceil(2^32 / groups), which
+// is at most one too high for j < 2^30.
+PFNG_DEV int attn_page_index(const AttnArgs &p, int j, int &group) {
+    const int g = j / kKvGroup;
+    int page = static_cast<int>(__umulhi(static_cast<uint32_t>(g), p.page_magic));
+    if (p.page_groups == 1) page = g;
+    group = g - page * p.page_groups;
+    if (group < 0) --page, group += p.page_groups;
+    return page;
+}
+
+// First byte, within a cache, of the group that holds key j of request r for a
+// key head; -1 where the table's entry is outside the cache.
+template <int DIM>
+PFNG_DEV int64_t attn_group_at(const AttnArgs &p, int64_t r, int head_kv, int j) {
+    int group;
+    const int at = attn_page_index(p, j, group), page = p.table[r * p.max_pages + at];
+    if (page < 0 || page >= p.num_pages) return -1;
+    return page * p.page_bytes + (static_cast<int64_t>(head_kv) * p.page_groups + group) * kv_group_bytes(DIM);
 }
 
 }  // namespace pfng

@@ -623,14 +623,18 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
             int j = 0;
             // the pages of a key tile are looked up while the copies before it wait
             int64_t at = -1, next = -1;  // this lane's group in the caches
+            int run = 0, next_run = 0;   // groups that its copy takes: those of a page go in one
             const auto look_up = [&](int n) {
                 const int key = (first + n) * kTile + lane * kKvGroup;
-                if (n >= count || lane >= kTile / kKvGroup || key >= seq) return int64_t{-1};
-                const int page = attn_page(p, r, key);
-                return page < 0 ? int64_t{-1}
-                                : kv_group_offset(page, head_kv, key % p.page_size, p.heads_kv, p.page_size / kKvGroup, DIM);
+                next = -1;
+                if (n >= count || lane >= kGroups || key >= seq) return;
+                next = attn_group_at<DIM>(p, r, head_kv, key);
+                int in_page;
+                attn_page_index(p, key, in_page);
+                next_run = lane > 0 && in_page > 0
+                               ? 0 : min(min(kGroups - lane, p.page_groups - in_page), (seq - key + kKvGroup - 1) / kKvGroup);
             };
-            next = look_up(0);
+            look_up(0);
             for (; j < 2 * count; ++j) {
                 const int n = j >> 1, slot = j % kRawSlots;
                 const bool is_v = j & 1;
@@ -639,7 +643,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
                     ok = false;
                     break;
                 }
-                if (!is_v) at = next;
+                if (!is_v) at = next, run = next_run;
                 const uint32_t there = __ballot_sync(0xffffffffu, at >= 0);
                 if (lane == 0) {
                     if (!is_v) {
@@ -650,10 +654,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
                     mbar_arrive_expect_tx(&raw_full[slot], kv_group_bytes(DIM) * __popc(there));
                 }
                 __syncwarp();
-                if (at >= 0)
+                if (at >= 0 && run > 0)
                     bulk_copy_g2s(smem + L::kRawAt + slot * L::kRaw + lane * kv_group_bytes(DIM),
-                                  (is_v ? p.v_cache : p.k_cache) + at, kv_group_bytes(DIM), &raw_full[slot], policy);
-                if (!is_v) next = look_up(n + 1);
+                                  (is_v ? p.v_cache : p.k_cache) + at, run * kv_group_bytes(DIM), &raw_full[slot], policy);
+                if (!is_v) look_up(n + 1);
             }
             if (!ok) abort_flag = 1;
             // copies in flight end before the CTA does

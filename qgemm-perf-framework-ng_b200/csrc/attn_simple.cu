@@ -41,14 +41,16 @@ __global__ void __launch_bounds__(kWarps * 32) attn_simple_kernel(const AttnArgs
         q[i] = one[0];
     }
     __syncwarp();
-    const int groups = p.page_size / kKvGroup;
     float m = -INFINITY, l = 0.0f, o[8] = {};
     for (int base = lo & ~31; base < hi; base += 32) {
         const int j = base + lane;
-        int page = -1;
-        if (j >= lo && j < hi) page = attn_page(p, r, j);
-        const int offset = j % p.page_size, in_group = offset % kKvGroup;
-        const int64_t at = page < 0 ? 0 : kv_group_offset(page, head_kv, offset, p.heads_kv, groups, dim);
+        int page = -1, in_page = 0;
+        if (j >= lo && j < hi) {
+            page = p.table[r * p.max_pages + attn_page_index(p, j, in_page)];
+            if (page >= p.num_pages) page = -1;
+        }
+        const int in_group = j % kKvGroup;
+        const int64_t at = page < 0 ? 0 : kv_group_offset(page, head_kv, in_page * kKvGroup, p.heads_kv, p.page_groups, dim);
         float s = -INFINITY;
         if (page >= 0) {
             const uint8_t *group = p.k_cache + at;
@@ -88,7 +90,7 @@ __global__ void __launch_bounds__(kWarps * 32) attn_simple_kernel(const AttnArgs
             const float pc = __shfl_sync(0xffffffffu, e, c);
             const int64_t atc = __shfl_sync(0xffffffffu, at, c);
             if (!((present >> c) & 1u)) continue;
-            const int rc = (base + c) % p.page_size % kKvGroup;
+            const int rc = (base + c) % kKvGroup;
             const uint8_t *group = p.v_cache + atc;
             const uint8_t *bytes = group + rc * kv_row_bytes(dim);
             const uint16_t *scales = reinterpret_cast<const uint16_t *>(group + kv_scale_offset(dim)) + rc * blocks;

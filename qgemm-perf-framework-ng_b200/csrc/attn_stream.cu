@@ -32,13 +32,22 @@
 //     eight shuffles.  The rounding of d P to fp16 (2^-12 on average) is the
 //     only one between the cache and the fp32 output; M includes a power of two
 //     that follows the largest d and keeps d P in the middle of fp16's range.
+#include <algorithm>
+
 #include "attn.cuh"
 #include "pfng_tma.h"
 
 namespace pfng {
 namespace {
 
-constexpr int kUnit = 64;    // keys of a unit: one stage of a warp's ring
+#ifndef KU
+#define KU 64
+#define KW1 12
+#define KS1 2
+#define KW2 8
+#define KS2 3
+#endif
+constexpr int kUnit = KU;    // keys of a unit: one stage of a warp's ring
 // Warps of a CTA (one CTA per SM) and stages of a warp's ring.  The rings take
 // 221 KB either way; one row tile of 8 fits 168 registers, two need 255.
 // 8 requests of 60000..100000 keys, one token: 196 us with 12 warps, 230 with
@@ -46,7 +55,7 @@ constexpr int kUnit = 64;    // keys of a unit: one stage of a warp's ring
 // of 4000..32000 keys (12 rows): 131 us with 8 warps, 184 with 12.
 template <int NT>
 struct Config {
-    static constexpr int kWarps = NT == 1 ? 12 : 8, kThreads = 32 * kWarps, kStages = NT == 1 ? 2 : 3;
+    static constexpr int kWarps = NT == 1 ? KW1 : KW2, kThreads = 32 * kWarps, kStages = NT == 1 ? KS1 : KS2;
 };
 constexpr float kSlack = 6.0f;
 constexpr float kNoMax = -3.0e38f;  // the maximum before the first visible key
@@ -204,7 +213,8 @@ struct Pieces {
 
 // Position of a warp on the line.
 struct Cursor {
-    int64_t r, item;       // request, item number
+    int r;                 // request
+    int64_t item;          // item number
     int head, tile;        // key head and row tile of the item
     int first, count, at;  // units of the item, and the next one of them
     RequestShape shape;
@@ -283,40 +293,72 @@ PFNG_DEV Cursor seek(const AttnArgs &p, int64_t u) {
     return c;
 }
 
-// Bulk copies of a unit's groups into a stage; returns the groups that are
-// there (bit i: keys 16 i .. of the unit).
-template <int DIM>
-PFNG_DEV uint32_t fetch_unit(const AttnArgs &p, const Cursor &c, uint8_t *stage, uint64_t *bar, uint64_t policy) {
-    constexpr int kGroups = kUnit / kKvGroup;
-    constexpr uint32_t kBytes = kv_group_bytes(DIM);
-    const int lane = threadIdx.x & 31;
-    const int g = lane % kGroups;
-    const bool is_v = lane >= kGroups;
-    const int key = (c.first + c.at) * kUnit + g * kKvGroup;
-    const int page = lane < 2 * kGroups && key < c.shape.seq ? attn_page(p, c.r, key) : -1;
-    const uint32_t there = __ballot_sync(0xffffffffu, page >= 0) & ((1u << kGroups) - 1);
-    if (lane == 0) mbar_arrive_expect_tx(bar, 2 * kBytes * __popc(there));
-    __syncwarp();
-    if (page >= 0) {
-        const int64_t at = kv_group_offset(page, c.head, key % p.page_size, p.heads_kv, p.page_size / kKvGroup, DIM);
-        bulk_copy_g2s(stage + lane * kBytes, (is_v ? p.v_cache : p.k_cache) + at, kBytes, bar, policy);
+// The units to copy next, per lane: lane g < kUnit / 16 copies the unit's g-th
+// group of K, the next as many lanes those of V.  What does not change within an
+// item is computed once for it.
+struct Fetcher {
+    const int32_t *pages;  // the request's row of the block table
+    const uint8_t *base;   // this lane's cache, at the key head
+    int key, seq, left;    // this lane's next key, keys of the request, units left in the item
+    template <int DIM>
+    PFNG_DEV void open(const AttnArgs &p, const Cursor &c) {
+        constexpr int kGroups = kUnit / kKvGroup;
+        const int lane = threadIdx.x & 31;
+        pages = p.table + static_cast<int64_t>(c.r) * p.max_pages;
+        base = (lane >= kGroups ? p.v_cache : p.k_cache) +
+               static_cast<int64_t>(c.head) * p.page_groups * kv_group_bytes(DIM);
+        key = (c.first + c.at) * kUnit + (lane % kGroups) * kKvGroup;
+        seq = lane < 2 * kGroups ? c.shape.seq : 0;
+        left = c.count - c.at;
     }
-    return there;
-}
+    // Bulk copies of a unit into a stage; returns the groups that are there
+    // (bit i: keys 16 i .. of the unit).
+    template <int DIM>
+    PFNG_DEV uint32_t fetch(const AttnArgs &p, uint32_t stage, uint64_t *bar, uint64_t policy) {
+        constexpr int kGroups = kUnit / kKvGroup;
+        constexpr uint32_t kBytes = kv_group_bytes(DIM);
+        const int lane = threadIdx.x & 31;
+        int page = -1, group = 0;
+        if (key < seq) {
+            const int at = attn_page_index(p, key, group);
+            page = pages[at];
+            page = page < p.num_pages ? page : -1;
+        }
+        const uint32_t there = __ballot_sync(0xffffffffu, page >= 0) & ((1u << kGroups) - 1);
+        if (lane == 0) mbar_arrive_expect_tx(bar, 2 * kBytes * __popc(there));
+        __syncwarp();
+        // one copy for the groups of a page: a copy takes its operands from uniform
+        // registers, so lanes that copy at once do it one after the other
+        const int g = lane % kGroups;
+        if (page >= 0 && (g == 0 || group == 0)) {
+            const int run = min(min(kGroups - g, p.page_groups - group), (seq - key + kKvGroup - 1) / kKvGroup);
+            bulk_copy_g2s(stage + lane * kBytes, base + page * p.page_bytes + group * static_cast<int>(kBytes), run * kBytes,
+                          bar, policy);
+        }
+        key += kUnit;
+        --left;
+        return there;
+    }
+};
 
+// What a warp keeps in shared memory, so that its loop fits its registers.
+template <int DIM, int NT>
+struct WarpState {
+    float start[NT][4][DIM / 32][2];  // -8 2^-24 sum(q) per block, rows 2 q4 and 2 q4 + 1
+    int lo[NT * 8], hi[NT * 8];       // visible keys of the rows
+    Cursor ahead, at;                 // item to copy from, item at work
+};
 template <int DIM, int NT>
 struct RowTile {
     static constexpr int kBlocks = DIM / 32;
     uint32_t q[NT][kBlocks][4];   // B fragments: low nibbles (2), high nibbles / 16 (2)
-    float start[NT][kBlocks][2];  // -8 2^-24 sum(q) per block, of this thread's two rows
     float mul[NT][2];             // score = accumulator * mul, in log2 units
-    int lo[NT][2], hi[NT][2];     // visible keys of this thread's two rows
     int lo_max, hi_min;           // keys that every row sees
     int lo_min, hi_max;           // keys that some row sees
 };
 
 template <int DIM, int NT>
-PFNG_DEV void load_rows(const StreamParams &sp, const Cursor &c, RowTile<DIM, NT> &t) {
+PFNG_DEV void load_rows(const StreamParams &sp, const Cursor &c, RowTile<DIM, NT> &t, WarpState<DIM, NT> &w) {
     const AttnArgs &p = sp.a;
     const int lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
     const int group = p.heads_q / p.heads_kv;
@@ -382,7 +424,7 @@ PFNG_DEV void load_rows(const StreamParams &sp, const Cursor &c, RowTile<DIM, NT
             const int from = (2 * q4 + x) * 4;  // a lane that loaded row 2 q4 + x
 #pragma unroll
             for (int b = 0; b < DIM / 32; ++b)
-                t.start[n][b][x] = -8.0f * 0x1p-24f * __shfl_sync(0xffffffffu, sum[b], from);
+                w.start[n][q4][b][x] = -8.0f * 0x1p-24f * __shfl_sync(0xffffffffu, sum[b], from);
             t.mul[n][x] = __shfl_sync(0xffffffffu, mul, from);
             const int rr = (c.tile * NT + n) * 8 + 2 * q4 + x;
             int lo = 0, hi = 0;
@@ -392,7 +434,7 @@ PFNG_DEV void load_rows(const StreamParams &sp, const Cursor &c, RowTile<DIM, NT
                 t.lo_max = max(t.lo_max, lo), t.hi_min = min(t.hi_min, hi);
                 t.lo_min = min(t.lo_min, lo), t.hi_max = max(t.hi_max, hi);
             }
-            t.lo[n][x] = lo, t.hi[n][x] = hi;
+            w.lo[n * 8 + 2 * q4 + x] = lo, w.hi[n * 8 + 2 * q4 + x] = hi;
         }
     }
 #pragma unroll
@@ -402,6 +444,7 @@ PFNG_DEV void load_rows(const StreamParams &sp, const Cursor &c, RowTile<DIM, NT
         t.lo_min = min(t.lo_min, __shfl_xor_sync(0xffffffffu, t.lo_min, o));
         t.hi_max = max(t.hi_max, __shfl_xor_sync(0xffffffffu, t.hi_max, o));
     }
+    __syncwarp();
 }
 
 template <int DIM, int NT>
@@ -433,8 +476,8 @@ PFNG_DEV int key_of_row(int r) { return (r & 8) | ((r & 7) >> 1) | ((r & 1) << 2
 // their groups; MASKED: some row does not see all of them.  magic: 0x64006400,
 // 1024 in both halves.
 template <int DIM, int NT, bool MASKED>
-PFNG_DEV void attend16(const RowTile<DIM, NT> &t, RowSums<DIM, NT> &s, uint32_t kg, uint32_t vg, int key0,
-                       uint32_t magic) {
+PFNG_DEV void attend16(const RowTile<DIM, NT> &t, const WarpState<DIM, NT> &w, RowSums<DIM, NT> &s, uint32_t kg,
+                       uint32_t vg, int key0, uint32_t magic) {
     constexpr int kBlocks = DIM / 32, kRow = DIM / 2, kScaleRow = DIM / 16, kScales = kv_scale_offset(DIM);
     const int lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
     const int ka = key_of_row(g), kb = ka + 8;  // this thread's keys (accumulator rows g and g + 8)
@@ -453,7 +496,15 @@ PFNG_DEV void attend16(const RowTile<DIM, NT> &t, RowSums<DIM, NT> &s, uint32_t 
         wa[0] = x.x, wa[1] = x.y, wb[0] = y.x, wb[1] = y.y;
         da[0] = lds32(ks + kScales), db[0] = lds32(ks + kScales + 8 * kScaleRow);
     }
-    float sc[NT][4] = {};
+    float sc[NT][4] = {}, start[NT][kBlocks][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int b = 0; b < kBlocks; b += 2) {
+            const uint4 x = lds128(smem_u32(&w.start[n][q4][b][0]));
+            start[n][b][0] = __uint_as_float(x.x), start[n][b][1] = __uint_as_float(x.y);
+            start[n][b + 1][0] = __uint_as_float(x.z), start[n][b + 1][1] = __uint_as_float(x.w);
+        }
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b) {
         const uint32_t a8 = wa[b] >> 8, b8 = wb[b] >> 8;
@@ -466,10 +517,10 @@ PFNG_DEV void attend16(const RowTile<DIM, NT> &t, RowSums<DIM, NT> &s, uint32_t 
                     t.q[n][b][1]);
             mma_f16(c, wa[b] & 0x00F000F0u, wb[b] & 0x00F000F0u, a8 & 0x00F000F0u, b8 & 0x00F000F0u, t.q[n][b][2],
                     t.q[n][b][3]);
-            sc[n][0] = fmaf(fa, c[0] + t.start[n][b][0], sc[n][0]);
-            sc[n][1] = fmaf(fa, c[1] + t.start[n][b][1], sc[n][1]);
-            sc[n][2] = fmaf(fb, c[2] + t.start[n][b][0], sc[n][2]);
-            sc[n][3] = fmaf(fb, c[3] + t.start[n][b][1], sc[n][3]);
+            sc[n][0] = fmaf(fa, c[0] + start[n][b][0], sc[n][0]);
+            sc[n][1] = fmaf(fa, c[1] + start[n][b][1], sc[n][1]);
+            sc[n][2] = fmaf(fb, c[2] + start[n][b][0], sc[n][2]);
+            sc[n][3] = fmaf(fb, c[3] + start[n][b][1], sc[n][3]);
         }
     }
     // V: this thread's keys are q4 + 4 i (operand rows 2 q4, 2 q4 + 1, + 8, + 9)
@@ -497,7 +548,8 @@ PFNG_DEV void attend16(const RowTile<DIM, NT> &t, RowSums<DIM, NT> &s, uint32_t 
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int key = key0 + (i < 2 ? ka : kb);
-                sc[n][i] = key >= t.lo[n][i & 1] && key < t.hi[n][i & 1] ? sc[n][i] * t.mul[n][i & 1] : -INFINITY;
+                const int row = n * 8 + 2 * q4 + (i & 1);
+                sc[n][i] = key >= w.lo[row] && key < w.hi[row] ? sc[n][i] * t.mul[n][i & 1] : -INFINITY;
             }
     } else {
 #pragma unroll
@@ -576,15 +628,15 @@ PFNG_DEV void attend16(const RowTile<DIM, NT> &t, RowSums<DIM, NT> &s, uint32_t 
         uint32_t p0[NT], p1[NT];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            float w[4];
+            float dp[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = sc[n][i] * d[i];
+            for (int i = 0; i < 4; ++i) dp[i] = sc[n][i] * d[i];
             if constexpr (MASKED) {  // 0 times an infinite scale is 0 where the row does not see the key
 #pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] = sc[n][i] == 0.0f ? 0.0f : w[i];
+                for (int i = 0; i < 4; ++i) dp[i] = sc[n][i] == 0.0f ? 0.0f : dp[i];
             }
-            p0[n] = h2(__floats2half2_rn(w[0], w[1]));
-            p1[n] = h2(__floats2half2_rn(w[2], w[3]));
+            p0[n] = h2(__floats2half2_rn(dp[0], dp[1]));
+            p1[n] = h2(__floats2half2_rn(dp[2], dp[3]));
         }
         // low nibbles: 1024 + n - 1032; high ones: (1024 + 16 n) / 16 - 72
         const auto low = [&](uint32_t z) { return h2(__hadd2(as_h2(and_or<0x000F000Fu>(z, magic)), minus1032)); };
@@ -651,6 +703,7 @@ __global__ void __launch_bounds__(Config<NT>::kThreads, 1) attn_stream_kernel(co
     constexpr int kWarps = Config<NT>::kWarps, kThreads = Config<NT>::kThreads, kStages = Config<NT>::kStages;
     extern __shared__ __align__(128) uint8_t ring[];
     __shared__ __align__(8) uint64_t bars[kWarps][kStages];
+    __shared__ __align__(16) WarpState<DIM, NT> states[kWarps];
     const AttnArgs &p = sp.a;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     constexpr uint32_t kHalf = (kUnit / kKvGroup) * kv_group_bytes(DIM);
@@ -668,12 +721,20 @@ __global__ void __launch_bounds__(Config<NT>::kThreads, 1) attn_stream_kernel(co
     const int64_t begin = pieces.start(worker), end = pieces.start(worker + 1);
     if (begin == end) return;
 
-    uint8_t *mine = ring + warp * kStages * 2 * kHalf;
+    const uint32_t ring_at = smem_u32(ring) + warp * kStages * 2 * kHalf;
     const uint64_t policy = l2_policy_evict_first();
     constexpr int kGroups = kUnit / kKvGroup;
     constexpr uint32_t kGroupMask = (1u << kGroups) - 1;
-    Cursor ahead = seek<NT>(p, begin), at = ahead;
-    int64_t fetched = begin;
+    WarpState<DIM, NT> &state = states[warp];
+    Fetcher fetcher;
+    {
+        const Cursor c = seek<NT>(p, begin);
+        if (lane == 0) state.ahead = state.at = c;
+        __syncwarp();
+        fetcher.open<DIM>(p, c);
+    }
+    int left = static_cast<int>(end - begin), to_fetch = left;  // units
+    int key0 = (state.at.first + state.at.at) * kUnit, in_item = state.at.count - state.at.at;
     int fetch_stage = 0, stage = 0;
     uint32_t there = 0, phase = 0;  // groups present: kGroups bits a stage
 
@@ -683,60 +744,81 @@ __global__ void __launch_bounds__(Config<NT>::kThreads, 1) attn_stream_kernel(co
     uint32_t magic;
     asm volatile("mov.b32 %0, 0x64006400;" : "=r"(magic));
 #pragma unroll 1
-    for (int64_t u = begin; u < end; ++u) {
+    while (left > 0) {
 #pragma unroll 1
-        while (fetched < end && fetched < u + kStages) {
-            const uint32_t bits = fetch_unit<DIM>(p, ahead, mine + fetch_stage * 2 * kHalf, &bars[warp][fetch_stage], policy);
+        while (to_fetch > 0 && left - to_fetch < kStages) {
+            const uint32_t bits = fetcher.fetch<DIM>(p, ring_at + fetch_stage * 2 * kHalf, &bars[warp][fetch_stage], policy);
             there = (there & ~(kGroupMask << (kGroups * fetch_stage))) | bits << (kGroups * fetch_stage);
-            ++fetched;
+            --to_fetch;
             if (++fetch_stage == kStages) fetch_stage = 0;
-            if (++ahead.at == ahead.count) next_item<NT>(p, ahead);
+            if (fetcher.left == 0 && to_fetch > 0) {
+                Cursor c = state.ahead;
+                next_item<NT>(p, c);
+                __syncwarp();
+                if (lane == 0) state.ahead = c;
+                __syncwarp();
+                fetcher.open<DIM>(p, c);
+            }
         }
         if (!opened) {
-            load_rows<DIM, NT>(sp, at, tile);
+            load_rows<DIM, NT>(sp, state.at, tile, state);
             clear(sums);
             opened = true;
-            whole = at.at == 0;
+            whole = state.at.at == 0;
         }
         ok = mbar_wait(&bars[warp][stage], phase, sp.err, kErrWaitFull);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        const uint32_t k = smem_u32(mine) + stage * 2 * kHalf, v = k + kHalf;
-        const int key0 = (at.first + at.at) * kUnit;
+        const uint32_t k = ring_at + stage * 2 * kHalf, v = k + kHalf;
 #pragma unroll 1
         for (int i = 0; i < kGroups; ++i) {
             const int key = key0 + i * kKvGroup;
             if (!((there >> (kGroups * stage + i)) & 1u) || key >= tile.hi_max || key + kKvGroup <= tile.lo_min) continue;
             if (key >= tile.lo_max && key + kKvGroup <= tile.hi_min)
-                attend16<DIM, NT, false>(tile, sums, k + i * kv_group_bytes(DIM), v + i * kv_group_bytes(DIM), key, magic);
+                attend16<DIM, NT, false>(tile, state, sums, k + i * kv_group_bytes(DIM), v + i * kv_group_bytes(DIM), key,
+                                         magic);
             else
-                attend16<DIM, NT, true>(tile, sums, k + i * kv_group_bytes(DIM), v + i * kv_group_bytes(DIM), key, magic);
+                attend16<DIM, NT, true>(tile, state, sums, k + i * kv_group_bytes(DIM), v + i * kv_group_bytes(DIM), key,
+                                        magic);
         }
         __syncwarp();
         if (++stage == kStages) stage = 0, phase ^= 1;
-        if (++at.at == at.count || u + 1 == end) {
-            whole = whole && at.at == at.count;
-            store_rows<DIM, NT>(sp, at, sums, whole, worker + at.item);
+        --left, --in_item;
+        key0 += kUnit;
+        if (in_item == 0 || left == 0) {
+            Cursor c = state.at;
+            whole = whole && in_item == 0;
+            store_rows<DIM, NT>(sp, c, sums, whole, worker + c.item);
             opened = false;
-            if (at.at == at.count) next_item<NT>(p, at);
+            if (in_item == 0) {
+                next_item<NT>(p, c);
+                __syncwarp();
+                if (lane == 0) state.at = c;
+                __syncwarp();
+                key0 = c.first * kUnit;
+                in_item = c.count;
+            }
         }
     }
     if (!ok)  // copies in flight end before the CTA does
         for (int i = 0; i < kStages; ++i) mbar_wait(&bars[warp][i], i >= stage ? phase : phase ^ 1, sp.err, kErrWaitFull);
 }
 
-// Joins the pieces of an item: weights 2^(m_i - max m) in line order.
-constexpr int kJoinThreads = 128;
+// Joins the pieces of an item: weights 2^(m_i - max m), the pieces in a fixed
+// order.  A CTA per query row of a row tile, its warps on every fourth piece.
+constexpr int kJoinWarps = 4, kJoinThreads = 32 * kJoinWarps;
 template <int DIM, int NT>
-__global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const StreamParams sp, int64_t workers) {
+__global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const StreamParams sp, int64_t workers, int rows) {
+    __shared__ float part[kJoinWarps][DIM + 1];
     const AttnArgs &p = sp.a;
-    const int64_t r = blockIdx.x / p.heads_kv;
-    const int head_kv = static_cast<int>(blockIdx.x % p.heads_kv);
+    const int i = static_cast<int>(blockIdx.x % rows);  // row within its tile
+    const int64_t rest = blockIdx.x / rows;
+    const int64_t r = rest / p.heads_kv;
+    const int head_kv = static_cast<int>(rest % p.heads_kv);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int64_t units, before, item;
     line_totals<NT, kJoinThreads>(p, r, units, before, item);
     const Pieces pieces(units, workers);
-    pdl_wait();
     const RequestShape shape = request_shape<NT>(p, r);
     const int group = p.heads_q / p.heads_kv;
     int64_t per_head = 0;
@@ -747,45 +829,53 @@ __global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const StreamPar
     }
     before += head_kv * per_head;
     item += static_cast<int64_t>(head_kv) * shape.tiles;
+    pdl_wait();
     for (int t = 0; t < shape.tiles; ++t, ++item) {
         int first, count;
         tile_units<NT>(p, shape, t, first, count);
         const int64_t u0 = before, u1 = before + count;
         before = u1;
+        const int row = t * 8 * NT + i;
         const int64_t w0 = pieces.worker_of(u0), w1 = pieces.worker_of(u1 - 1);
-        if (w0 == w1) continue;  // written by its one piece
-        for (int i = warp; i < 8 * NT; i += kJoinThreads / 32) {
-            const int row = t * 8 * NT + i;
-            if (row >= shape.rows) break;
-            float m = kNoMax;
-            for (int64_t w = w0 + lane; w <= w1; w += 32)
-                m = fmaxf(m, sp.part_ml[(w + item) * (8 * NT) + i].x);
+        if (w0 == w1 || row >= shape.rows) continue;  // written by its one piece
+        const auto slot = [&](int64_t w) { return (w + item) * (8 * NT) + i; };
+        float m = kNoMax;
+        for (int64_t w = w0 + lane; w <= w1; w += 32) m = fmaxf(m, sp.part_ml[slot(w)].x);
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-            constexpr int kPer = DIM / 32;
-            float acc[kPer] = {}, l = 0.0f;
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        constexpr int kPer = DIM / 32;
+        float acc[kPer] = {}, l = 0.0f;
 #pragma unroll 4
-            for (int64_t w = w0; w <= w1; ++w) {
-                const int64_t at = (w + item) * (8 * NT) + i;
-                const float2 ml = sp.part_ml[at];
-                const float f = exp2_approx(ml.x - m);
-                l += ml.y * f;
+        for (int64_t w = w0 + warp; w <= w1; w += kJoinWarps) {
+            const float2 ml = sp.part_ml[slot(w)];
+            const float f = exp2_approx(ml.x - m);
+            l += ml.y * f;
+            const float *o = sp.part_o + slot(w) * DIM;
 #pragma unroll
-                for (int x = 0; x < kPer; ++x) acc[x] += f * sp.part_o[at * DIM + lane * kPer + x];
-            }
-            const bool none = m == kNoMax && l == 0.0f;
-            const float f = none ? 0.0f : 1.0f / l;
-            const int64_t token = p.cu_q[r] + row / group, head = static_cast<int64_t>(head_kv) * group + row % group;
-#pragma unroll
-            for (int x = 0; x < kPer; ++x) {
-                const float v[1] = {acc[x] * f};
-                store_values<1>(p.out_format, p.out, token * p.ldo + head * DIM + lane * kPer + x, v);
-            }
-            if (p.lse && lane == 0)
-                p.lse[token * p.heads_q + head] = none ? -INFINITY : (m + log2f(l)) / kLog2e;
+            for (int x = 0; x < kPer; ++x) acc[x] += f * o[lane + 32 * x];
         }
+#pragma unroll
+        for (int x = 0; x < kPer; ++x) part[warp][lane + 32 * x] = acc[x];
+        if (lane == 0) part[warp][DIM] = l;
+        __syncthreads();
+        l = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kJoinWarps; ++w) l += part[w][DIM];
+        const bool none = m == kNoMax && l == 0.0f;
+        const float f = none ? 0.0f : 1.0f / l;
+        const int64_t token = p.cu_q[r] + row / group, head = static_cast<int64_t>(head_kv) * group + row % group;
+        if (static_cast<int>(threadIdx.x) < DIM) {
+            float v[1] = {0.0f};
+#pragma unroll
+            for (int w = 0; w < kJoinWarps; ++w) v[0] += part[w][threadIdx.x];
+            v[0] *= f;
+            store_values<1>(p.out_format, p.out, token * p.ldo + head * DIM + threadIdx.x, v);
+        }
+        if (p.lse && threadIdx.x == 0) p.lse[token * p.heads_q + head] = none ? -INFINITY : (m + log2f(l)) / kLog2e;
+        __syncthreads();
     }
 }
+static_assert(kJoinThreads >= 128, "a thread per dimension");
 
 int64_t max_rows(const AttnArgs &p) { return p.max_q * (p.heads_q / p.heads_kv); }
 int row_tiles_of_8(const AttnArgs &p) { return max_rows(p) <= 8 ? 1 : 2; }
@@ -809,7 +899,8 @@ cudaError_t launch(const StreamParams &sp, cudaStream_t s) {
     attn_stream_kernel<DIM, NT><<<static_cast<unsigned>(grid), Config<NT>::kThreads, smem, s>>>(sp);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(sp.a.requests * sp.a.heads_kv));
+    const int rows = static_cast<int>(std::min<int64_t>(8 * NT, max_rows(sp.a)));
+    cfg.gridDim = dim3(static_cast<unsigned>(sp.a.requests * sp.a.heads_kv * rows));
     cfg.blockDim = dim3(kJoinThreads);
     cfg.stream = s;
     cudaLaunchAttribute attr{};
@@ -817,13 +908,13 @@ cudaError_t launch(const StreamParams &sp, cudaStream_t s) {
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, attn_join_kernel<DIM, NT>, sp, workers(sp.a));
+    return cudaLaunchKernelEx(&cfg, attn_join_kernel<DIM, NT>, sp, workers(sp.a), rows);
 }
 
 }  // namespace
 
 bool attn_stream_supported(const AttnArgs &p) {
-    return (p.head_dim == 64 || p.head_dim == 128) && p.requests * p.heads_kv < 0x7fffffff;
+    return (p.head_dim == 64 || p.head_dim == 128) && p.requests * p.heads_kv * 16 < 0x7fffffff;
 }
 
 size_t attn_stream_workspace(const AttnArgs &p) {

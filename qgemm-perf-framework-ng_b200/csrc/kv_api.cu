@@ -179,6 +179,9 @@ int pfng_b200_attention_q4_0(const void *q, int64_t ldq, int q_format, const voi
     a.window = window, a.page_size = static_cast<int>(page_size), a.causal = causal != 0, a.scale = scale;
     a.heads_q = static_cast<int>(heads_q), a.heads_kv = static_cast<int>(heads_kv);
     a.head_dim = static_cast<int>(head_dim);
+    a.page_groups = static_cast<int>(page_size / 16);
+    a.page_magic = static_cast<uint32_t>(((int64_t{1} << 32) + a.page_groups - 1) / a.page_groups);
+    a.page_bytes = static_cast<int64_t>(pfng_b200_kv_cache_bytes(1, page_size, heads_kv, head_dim));
     const int resolved = resolve_attention(a, path);
     if (resolved < 0) return PFNG_B200_ERR_UNSUPPORTED;
     if ((st = device_status()) != PFNG_B200_OK) return st;

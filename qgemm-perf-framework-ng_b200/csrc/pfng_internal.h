@@ -181,7 +181,10 @@ struct AttnArgs {
     int64_t num_pages, max_pages, requests, tokens;
     int64_t max_q, max_kv;  // upper bounds of the requests' new tokens and keys
     int64_t window;
-    int page_size, heads_q, heads_kv, head_dim, causal;
+    int page_size, page_groups;  // tokens and 16-token groups of a page
+    uint32_t page_magic;         // ceil(2^32 / page_groups), for page_groups > 1
+    int64_t page_bytes;          // bytes of a page of K (and of V), all key heads
+    int heads_q, heads_kv, head_dim, causal;
     float scale;
 };
 cudaError_t launch_attn_simple(const AttnArgs &args, cudaStream_t s);
