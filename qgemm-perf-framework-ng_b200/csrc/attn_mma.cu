@@ -232,7 +232,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
     const int64_t rest = blockIdx.x % (p.requests * p.heads_kv);
     const int64_t r = rest / p.heads_kv;
     const int head_kv = static_cast<int>(rest % p.heads_kv);
-    const int group = p.heads_q / p.heads_kv;
+    const int group = p.group;
     int all;
     const int rows = attn_new_tokens(p, r, all) * group;
     const int row0 = tile * kRows;
@@ -686,7 +686,7 @@ cudaError_t launch(const MmaParams &mp, int64_t grid, cudaStream_t s) {
     return cudaGetLastError();
 }
 
-int64_t row_blocks(const AttnArgs &p) { return (p.max_q * (p.heads_q / p.heads_kv) + kRows - 1) / kRows; }
+int64_t row_blocks(const AttnArgs &p) { return (p.max_q * p.group + kRows - 1) / kRows; }
 
 }  // namespace
 

@@ -20,7 +20,7 @@ __global__ void __launch_bounds__(kWarps * 32) attn_simple_kernel(const AttnArgs
     const int dim = p.head_dim, blocks = dim / 32;
     const int64_t row = static_cast<int64_t>(blockIdx.x) * kWarps + warp;
     const int64_t token = row / p.heads_q;
-    const int head = static_cast<int>(row % p.heads_q), head_kv = head / (p.heads_q / p.heads_kv);
+    const int head = static_cast<int>(row % p.heads_q), head_kv = head / p.group;
     if (token >= p.tokens || token < p.cu_q[0] || token >= p.cu_q[p.requests]) return;
     // the request of this token: last one whose first token is at or before it
     int64_t a = 0, b = p.requests;

@@ -40,14 +40,7 @@
 namespace pfng {
 namespace {
 
-#ifndef KU
-#define KU 64
-#define KW1 12
-#define KS1 2
-#define KW2 8
-#define KS2 3
-#endif
-constexpr int kUnit = KU;    // keys of a unit: one stage of a warp's ring
+constexpr int kUnit = 64;    // keys of a unit: one stage of a warp's ring
 // Warps of a CTA (one CTA per SM) and stages of a warp's ring.  The rings take
 // 221 KB either way; one row tile of 8 fits 168 registers, two need 255.
 // 8 requests of 60000..100000 keys, one token: 196 us with 12 warps, 230 with
@@ -55,19 +48,13 @@ constexpr int kUnit = KU;    // keys of a unit: one stage of a warp's ring
 // of 4000..32000 keys (12 rows): 131 us with 8 warps, 184 with 12.
 template <int NT>
 struct Config {
-    static constexpr int kWarps = NT == 1 ? KW1 : KW2, kThreads = 32 * kWarps, kStages = NT == 1 ? KS1 : KS2;
+    static constexpr int kWarps = NT == 1 ? 12 : 8, kThreads = 32 * kWarps, kStages = NT == 1 ? 2 : 3;
+    static constexpr int kStep = 2;  // groups whose scores are computed before their O
 };
 constexpr float kSlack = 6.0f;
 constexpr float kNoMax = -3.0e38f;  // the maximum before the first visible key
 constexpr float kLog2e = 1.4426950408889634f;
 
-struct StreamParams {
-    AttnArgs a;
-    float *part_o;     // [slots][rows][dim]: unnormalised outputs of pieces
-    float2 *part_ml;   // [slots][rows]: maximum (log2) and sum
-    int vec_q;         // rows of q allow 4-value loads
-    int *err;
-};
 
 PFNG_DEV void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, "
@@ -150,14 +137,14 @@ template <int NT>
 PFNG_DEV RequestShape request_shape(const AttnArgs &p, int64_t r) {
     RequestShape s;
     s.seq = attn_seq_len(p, r);
-    s.rows = attn_new_tokens(p, r, s.all) * (p.heads_q / p.heads_kv);
+    s.rows = attn_new_tokens(p, r, s.all) * (p.group);
     s.tiles = (s.rows + 8 * NT - 1) / (8 * NT);
     return s;
 }
 // Units [first, first + count) of row tile `tile`.
 template <int NT>
 PFNG_DEV void tile_units(const AttnArgs &p, const RequestShape &s, int tile, int &first, int &count) {
-    const int group = p.heads_q / p.heads_kv;
+    const int group = p.group;
     int lo, hi, lo2, hi2;
     attn_visible(p, s.seq, s.all, tile * 8 * NT / group, lo, hi2);
     attn_visible(p, s.seq, s.all, (min(tile * 8 * NT + 8 * NT, s.rows) - 1) / group, lo2, hi);
@@ -176,28 +163,34 @@ PFNG_DEV int64_t request_units(const AttnArgs &p, int64_t r) {
     return sum * p.heads_kv;
 }
 
-// Sum over all requests of (units, items), and over the requests before `r`,
-// by all threads of a CTA.
+// Units of all requests, by all threads of a CTA.
 template <int NT, int THREADS>
-PFNG_DEV void line_totals(const AttnArgs &p, int64_t r, int64_t &units, int64_t &units_before, int64_t &items_before) {
-    __shared__ int64_t sums[THREADS / 32][3];
-    int64_t u = 0, ub = 0, ib = 0;
-    for (int64_t i = threadIdx.x; i < p.requests; i += THREADS) {
-        const int64_t n = request_units<NT>(p, i);
-        u += n;
-        if (i < r) ub += n, ib += static_cast<int64_t>(request_shape<NT>(p, i).tiles) * p.heads_kv;
-    }
+PFNG_DEV int64_t line_units(const AttnArgs &p) {
+    __shared__ int64_t sums[THREADS / 32];
+    int64_t u = 0;
+    for (int64_t i = threadIdx.x; i < p.requests; i += THREADS) u += request_units<NT>(p, i);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        u += __shfl_xor_sync(0xffffffffu, u, o);
-        ub += __shfl_xor_sync(0xffffffffu, ub, o);
-        ib += __shfl_xor_sync(0xffffffffu, ib, o);
-    }
-    if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5][0] = u, sums[threadIdx.x >> 5][1] = ub, sums[threadIdx.x >> 5][2] = ib;
+    for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
+    if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = u;
     __syncthreads();
-    units = units_before = items_before = 0;
-    for (int w = 0; w < THREADS / 32; ++w) units += sums[w][0], units_before += sums[w][1], items_before += sums[w][2];
+    u = 0;
+    for (int w = 0; w < THREADS / 32; ++w) u += sums[w];
+    return u;
 }
+
+// Where a request starts on the line, for the kernel that joins the pieces.
+struct LineStart {
+    int64_t units, items;  // before the request
+};
+
+struct StreamParams {
+    AttnArgs a;
+    float *part_o;     // [slots][rows][dim]: unnormalised outputs of pieces
+    float2 *part_ml;   // [slots][rows]: maximum (log2) and sum
+    LineStart *starts; // [requests + 1]: written by worker 0
+    int vec_q;         // rows of q allow 4-value loads
+    int *err;
+};
 
 // The line cut into `workers` pieces of each or each + 1 units, the longer
 // ones first.
@@ -243,15 +236,17 @@ PFNG_DEV void next_item(const AttnArgs &p, Cursor &c) {
     }
     tile_units<NT>(p, c.shape, c.tile, c.first, c.count);
 }
-// Cursor at unit `u` of the line, by one warp.
+// Cursor at unit `u` of the line, by one warp.  With `starts` it goes through
+// the whole line and writes where each request starts (and the totals).
 template <int NT>
-PFNG_DEV Cursor seek(const AttnArgs &p, int64_t u) {
+PFNG_DEV Cursor seek(const AttnArgs &p, int64_t u, LineStart *starts) {
     const int lane = threadIdx.x & 31;
     Cursor c;
     c.item = 0;
-    int64_t before = 0;
-    c.r = p.requests;
-    for (int64_t base = 0; base < p.requests; base += 32) {
+    int64_t before = 0, line = 0, line_items = 0;
+    bool found = false;
+    c.r = static_cast<int>(p.requests);
+    for (int64_t base = 0; base < p.requests && (!found || starts); base += 32) {
         const int64_t i = base + lane;
         int64_t n = i < p.requests ? request_units<NT>(p, i) : 0;
         int64_t items = i < p.requests ? static_cast<int64_t>(request_shape<NT>(p, i).tiles) * p.heads_kv : 0;
@@ -261,17 +256,19 @@ PFNG_DEV Cursor seek(const AttnArgs &p, int64_t u) {
             const int64_t x = __shfl_up_sync(0xffffffffu, n, o), y = __shfl_up_sync(0xffffffffu, items, o);
             if (lane >= o) n += x, items += y;
         }
-        const uint32_t past = __ballot_sync(0xffffffffu, before + n > u);
-        if (past) {
+        if (starts && i < p.requests) starts[i] = {line + n - own, line_items + items - own_items};
+        const uint32_t past = __ballot_sync(0xffffffffu, line + n > u);
+        if (past && !found) {
             const int k = __ffs(past) - 1;
-            c.r = base + k;
-            before += __shfl_sync(0xffffffffu, n - own, k);
-            c.item += __shfl_sync(0xffffffffu, items - own_items, k);
-            break;
+            found = true;
+            c.r = static_cast<int>(base) + k;
+            before = line + __shfl_sync(0xffffffffu, n - own, k);
+            c.item = line_items + __shfl_sync(0xffffffffu, items - own_items, k);
         }
-        before += __shfl_sync(0xffffffffu, n, 31);
-        c.item += __shfl_sync(0xffffffffu, items, 31);
+        line += __shfl_sync(0xffffffffu, n, 31);
+        line_items += __shfl_sync(0xffffffffu, items, 31);
     }
+    if (starts && lane == 0) starts[p.requests] = {line, line_items};
     open_request<NT>(p, c);
     if (c.r >= p.requests) return c;
     int64_t left = u - before;
@@ -361,7 +358,7 @@ template <int DIM, int NT>
 PFNG_DEV void load_rows(const StreamParams &sp, const Cursor &c, RowTile<DIM, NT> &t, WarpState<DIM, NT> &w) {
     const AttnArgs &p = sp.a;
     const int lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
-    const int group = p.heads_q / p.heads_kv;
+    const int group = p.group;
     t.lo_max = 0, t.hi_min = 0x7fffffff, t.lo_min = 0x7fffffff, t.hi_max = 0;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -472,106 +469,114 @@ PFNG_DEV void clear(RowSums<DIM, NT> &s) {
 // a warp read neighbouring rows of shared memory.
 PFNG_DEV int key_of_row(int r) { return (r & 8) | ((r & 7) >> 1) | ((r & 1) << 2); }
 
-// 16 keys: key0 is the first one's number, kg and vg the shared addresses of
-// their groups; MASKED: some row does not see all of them.  magic: 0x64006400,
-// 1024 in both halves.
-template <int DIM, int NT, bool MASKED>
-PFNG_DEV void attend16(const RowTile<DIM, NT> &t, const WarpState<DIM, NT> &w, RowSums<DIM, NT> &s, uint32_t kg,
-                       uint32_t vg, int key0, uint32_t magic) {
+// kGroups groups of 16 keys: key0 is the first key's number, kg and vg the
+// shared addresses of the groups; MASKED: some row does not see some of the
+// keys.  magic: 0x64006400, 1024 in both halves.
+// All scores first, then one look at maximum and scales, then all of O: a few
+// long runs of independent instructions, which the pipes (ALU for the nibbles,
+// FMA, tensor cores, shuffles) overlap.
+template <int DIM, int NT, int kGroups, bool MASKED>
+PFNG_DEV void attend(const RowTile<DIM, NT> &t, const WarpState<DIM, NT> &w, RowSums<DIM, NT> &s, uint32_t kg,
+                     uint32_t vg, int key0, uint32_t magic) {
     constexpr int kBlocks = DIM / 32, kRow = DIM / 2, kScaleRow = DIM / 16, kScales = kv_scale_offset(DIM);
+    constexpr int kGroup = kv_group_bytes(DIM);
     const int lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
-    const int ka = key_of_row(g), kb = ka + 8;  // this thread's keys (accumulator rows g and g + 8)
+    const int ka = key_of_row(g), kb = ka + 8;  // this thread's keys of a group (accumulator rows g and g + 8)
 
     // ---- scores ----
-    uint32_t wa[kBlocks], wb[kBlocks], da[kBlocks / 2], db[kBlocks / 2];
-    const uint32_t kw = kg + ka * kRow + q4 * 4 * kBlocks, ks = kg + ka * kScaleRow;
-    if constexpr (kBlocks == 4) {
-        const uint4 x = lds128(kw), y = lds128(kw + 8 * kRow);
-        wa[0] = x.x, wa[1] = x.y, wa[2] = x.z, wa[3] = x.w;
-        wb[0] = y.x, wb[1] = y.y, wb[2] = y.z, wb[3] = y.w;
-        const uint2 u = lds64(ks + kScales), v = lds64(ks + kScales + 8 * kScaleRow);
-        da[0] = u.x, da[1] = u.y, db[0] = v.x, db[1] = v.y;
-    } else {
-        const uint2 x = lds64(kw), y = lds64(kw + 8 * kRow);
-        wa[0] = x.x, wa[1] = x.y, wb[0] = y.x, wb[1] = y.y;
-        da[0] = lds32(ks + kScales), db[0] = lds32(ks + kScales + 8 * kScaleRow);
-    }
-    float sc[NT][4] = {}, start[NT][kBlocks][2];
+    float sc[kGroups][NT][4];
+    {
+        float start[NT][kBlocks][2];
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int b = 0; b < kBlocks; b += 2) {
-            const uint4 x = lds128(smem_u32(&w.start[n][q4][b][0]));
-            start[n][b][0] = __uint_as_float(x.x), start[n][b][1] = __uint_as_float(x.y);
-            start[n][b + 1][0] = __uint_as_float(x.z), start[n][b + 1][1] = __uint_as_float(x.w);
-        }
+            for (int b = 0; b < kBlocks; b += 2) {
+                const uint4 x = lds128(smem_u32(&w.start[n][q4][b][0]));
+                start[n][b][0] = __uint_as_float(x.x), start[n][b][1] = __uint_as_float(x.y);
+                start[n][b + 1][0] = __uint_as_float(x.z), start[n][b + 1][1] = __uint_as_float(x.w);
+            }
 #pragma unroll
-    for (int b = 0; b < kBlocks; ++b) {
-        const uint32_t a8 = wa[b] >> 8, b8 = wb[b] >> 8;
-        const float fa = (b & 1) ? high_half(da[b / 2]) : low_half(da[b / 2]);
-        const float fb = (b & 1) ? high_half(db[b / 2]) : low_half(db[b / 2]);
+        for (int j = 0; j < kGroups; ++j) {
+            uint32_t wa[kBlocks], wb[kBlocks], da[kBlocks / 2], db[kBlocks / 2];
+            const uint32_t kw = kg + ka * kRow + q4 * 4 * kBlocks + j * kGroup;
+            const uint32_t ks = kg + ka * kScaleRow + kScales + j * kGroup;
+            if constexpr (kBlocks == 4) {
+                const uint4 x = lds128(kw), y = lds128(kw + 8 * kRow);
+                wa[0] = x.x, wa[1] = x.y, wa[2] = x.z, wa[3] = x.w;
+                wb[0] = y.x, wb[1] = y.y, wb[2] = y.z, wb[3] = y.w;
+                const uint2 u = lds64(ks), v = lds64(ks + 8 * kScaleRow);
+                da[0] = u.x, da[1] = u.y, db[0] = v.x, db[1] = v.y;
+            } else {
+                const uint2 x = lds64(kw), y = lds64(kw + 8 * kRow);
+                wa[0] = x.x, wa[1] = x.y, wb[0] = y.x, wb[1] = y.y;
+                da[0] = lds32(ks), db[0] = lds32(ks + 8 * kScaleRow);
+            }
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            mma_f16(c, wa[b] & 0x000F000Fu, wb[b] & 0x000F000Fu, a8 & 0x000F000Fu, b8 & 0x000F000Fu, t.q[n][b][0],
-                    t.q[n][b][1]);
-            mma_f16(c, wa[b] & 0x00F000F0u, wb[b] & 0x00F000F0u, a8 & 0x00F000F0u, b8 & 0x00F000F0u, t.q[n][b][2],
-                    t.q[n][b][3]);
-            sc[n][0] = fmaf(fa, c[0] + start[n][b][0], sc[n][0]);
-            sc[n][1] = fmaf(fa, c[1] + start[n][b][1], sc[n][1]);
-            sc[n][2] = fmaf(fb, c[2] + start[n][b][0], sc[n][2]);
-            sc[n][3] = fmaf(fb, c[3] + start[n][b][1], sc[n][3]);
-        }
-    }
-    // V: this thread's keys are q4 + 4 i (operand rows 2 q4, 2 q4 + 1, + 8, + 9)
-    uint32_t v[4][kBlocks / 2], dv[4][kBlocks / 2];
-    const uint32_t vw = vg + q4 * kRow + g * 2 * kBlocks, vs = vg + q4 * kScaleRow;
+            for (int n = 0; n < NT; ++n) sc[j][n][0] = sc[j][n][1] = sc[j][n][2] = sc[j][n][3] = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if constexpr (kBlocks == 4) {
-            const uint2 x = lds64(vw + 4 * i * kRow), y = lds64(vs + kScales + 4 * i * kScaleRow);
-            v[i][0] = x.x, v[i][1] = x.y, dv[i][0] = y.x, dv[i][1] = y.y;
-        } else {
-            v[i][0] = lds32(vw + 4 * i * kRow), dv[i][0] = lds32(vs + kScales + 4 * i * kScaleRow);
+            for (int b = 0; b < kBlocks; ++b) {
+                const uint32_t a8 = wa[b] >> 8, b8 = wb[b] >> 8;
+                const float fa = (b & 1) ? high_half(da[b / 2]) : low_half(da[b / 2]);
+                const float fb = (b & 1) ? high_half(db[b / 2]) : low_half(db[b / 2]);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    mma_f16(c, wa[b] & 0x000F000Fu, wb[b] & 0x000F000Fu, a8 & 0x000F000Fu, b8 & 0x000F000Fu, t.q[n][b][0],
+                            t.q[n][b][1]);
+                    mma_f16(c, wa[b] & 0x00F000F0u, wb[b] & 0x00F000F0u, a8 & 0x00F000F0u, b8 & 0x00F000F0u, t.q[n][b][2],
+                            t.q[n][b][3]);
+                    sc[j][n][0] = fmaf(fa, c[0] + start[n][b][0], sc[j][n][0]);
+                    sc[j][n][1] = fmaf(fa, c[1] + start[n][b][1], sc[j][n][1]);
+                    sc[j][n][2] = fmaf(fb, c[2] + start[n][b][0], sc[j][n][2]);
+                    sc[j][n][3] = fmaf(fb, c[3] + start[n][b][1], sc[j][n][3]);
+                }
+            }
         }
     }
-    if constexpr (MASKED) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {  // a key that no row sees may be anything: its scales are not looked at
-            const int key = key0 + q4 + 4 * i;
-            const bool seen = key >= t.lo_min && key < t.hi_max;
-#pragma unroll
-            for (int j = 0; j < kBlocks / 2; ++j) dv[i][j] = seen ? dv[i][j] : 0;
-        }
+    for (int j = 0; j < kGroups; ++j)
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int key = key0 + (i < 2 ? ka : kb);
-                const int row = n * 8 + 2 * q4 + (i & 1);
-                sc[n][i] = key >= w.lo[row] && key < w.hi[row] ? sc[n][i] * t.mul[n][i & 1] : -INFINITY;
+                sc[j][n][i] *= t.mul[n][i & 1];
+                if constexpr (MASKED) {
+                    const int key = key0 + j * kKvGroup + (i < 2 ? ka : kb), row = n * 8 + 2 * q4 + (i & 1);
+                    if (!(key >= w.lo[row] && key < w.hi[row])) sc[j][n][i] = -INFINITY;
+                }
             }
-    } else {
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sc[n][i] *= t.mul[n][i & 1];
-    }
 
     // ---- maximum, renewed when a score or a scale passes its limit ----
-    uint32_t d2 = larger(dv[0][0], dv[1][0]);
-    d2 = larger(larger(d2, dv[2][0]), dv[3][0]);
-    if constexpr (kBlocks == 4) {
-        d2 = larger(larger(d2, dv[0][1]), dv[1][1]);
-        d2 = larger(larger(d2, dv[2][1]), dv[3][1]);
+    // V scales of the groups, in words of two: read once, kWords / 32 a lane
+    float d_top;
+    {
+        constexpr int kGroupWords = kKvGroup * kScaleRow / 4, kWords = kGroups * kGroupWords;
+        uint32_t d2 = 0;
+#pragma unroll
+        for (int i = 0; i < (kWords + 31) / 32; ++i) {
+            const int at = (i * 32 + lane) % kWords, j = at / kGroupWords, in_group = at % kGroupWords;
+            uint32_t x = lds32(vg + kScales + j * kGroup + 4 * in_group);
+            if constexpr (MASKED) {  // a key that no row sees may be anything: its scales are not looked at
+                const int key = key0 + j * kKvGroup + 4 * in_group / kScaleRow;
+                if (!(key >= t.lo_min && key < t.hi_max)) x = 0;
+            }
+            d2 = i == 0 ? x : larger(d2, x);
+        }
+        d_top = fmaxf(fabsf(low_half(d2)), fabsf(high_half(d2)));
     }
-    float over = sc[0][0] - s.m[0][0];
+    float tops[NT][2];
+    bool past = d_top > s.d_limit;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) over = fmaxf(over, sc[n][i] - s.m[n][i & 1]);
-    float d_top = fmaxf(fabsf(low_half(d2)), fabsf(high_half(d2)));
-    if (__any_sync(0xffffffffu, over > s.limit || d_top > s.d_limit)) {
+        for (int x = 0; x < 2; ++x) {
+            float top = fmaxf(sc[0][n][x], sc[0][n][x + 2]);
+#pragma unroll
+            for (int j = 1; j < kGroups; ++j) top = fmaxf(top, fmaxf(sc[j][n][x], sc[j][n][x + 2]));
+            tops[n][x] = top;
+            past |= top > s.m[n][x] + s.limit;
+        }
+    if (__any_sync(0xffffffffu, past)) {
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) d_top = fmaxf(d_top, __shfl_xor_sync(0xffffffffu, d_top, o));
         float up = s.limit - kSlack;  // log2 of the power of two that P carries
@@ -586,7 +591,7 @@ PFNG_DEV void attend16(const RowTile<DIM, NT> &t, const WarpState<DIM, NT> &w, R
             float f[2];
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-                float top = fmaxf(sc[n][x], sc[n][x + 2]);
+                float top = tops[n][x];
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
                 top = fmaxf(top - up, s.m[n][x]);
@@ -601,55 +606,73 @@ PFNG_DEV void attend16(const RowTile<DIM, NT> &t, const WarpState<DIM, NT> &w, R
             }
         }
     }
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sc[n][i] = exp2_approx(sc[n][i] - s.m[n][i & 1]);
-        s.l[n][0] += sc[n][0] + sc[n][2];
-        s.l[n][1] += sc[n][1] + sc[n][3];
-    }
 
     // ---- O^T += V^T (d P) ----
-    // P of this thread's four keys, query row g
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        rows_to_columns(sc[n][0], sc[n][1]);
-        rows_to_columns(sc[n][2], sc[n][3]);
-    }
     const __half2 minus1032 = __float2half2_rn(-1032.0f), minus72 = __float2half2_rn(-72.0f),
                   sixteenth = __float2half2_rn(0.0625f);
 #pragma unroll
-    for (int b = 0; b < kBlocks; ++b) {
-        const uint32_t sel = (b & 1) ? 0x7632u : 0x5410u;
-        const uint32_t x = __byte_perm(v[0][b / 2], v[1][b / 2], sel), y = __byte_perm(v[2][b / 2], v[3][b / 2], sel);
-        float d[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) d[i] = (b & 1) ? high_half(dv[i][b / 2]) : low_half(dv[i][b / 2]);
-        uint32_t p0[NT], p1[NT];
+    for (int j = 0; j < kGroups; ++j) {
+        // P of this thread's four keys q4 + 4 i (operand rows 2 q4, 2 q4 + 1, + 8, + 9), query row g
+        float pr[NT][4];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            float dp[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) dp[i] = sc[n][i] * d[i];
-            if constexpr (MASKED) {  // 0 times an infinite scale is 0 where the row does not see the key
-#pragma unroll
-                for (int i = 0; i < 4; ++i) dp[i] = sc[n][i] == 0.0f ? 0.0f : dp[i];
-            }
-            p0[n] = h2(__floats2half2_rn(dp[0], dp[1]));
-            p1[n] = h2(__floats2half2_rn(dp[2], dp[3]));
+            for (int i = 0; i < 4; ++i) pr[n][i] = exp2_approx(sc[j][n][i] - s.m[n][i & 1]);
+            s.l[n][0] += pr[n][0] + pr[n][2];
+            s.l[n][1] += pr[n][1] + pr[n][3];
+            rows_to_columns(pr[n][0], pr[n][1]);
+            rows_to_columns(pr[n][2], pr[n][3]);
         }
-        // low nibbles: 1024 + n - 1032; high ones: (1024 + 16 n) / 16 - 72
-        const auto low = [&](uint32_t z) { return h2(__hadd2(as_h2(and_or<0x000F000Fu>(z, magic)), minus1032)); };
-        const auto high = [&](uint32_t z) {
-            return h2(__hfma2(as_h2(and_or<0x00F000F0u>(z, magic)), sixteenth, minus72));
-        };
-        const uint32_t x8 = x >> 8, y8 = y >> 8;
-        const uint32_t a0 = low(x), a1 = high(x), a2 = low(y), a3 = high(y);
-        const uint32_t b0 = low(x8), b1 = high(x8), b2 = low(y8), b3 = high(y8);
+        uint32_t v[4][kBlocks / 2], dv[4][kBlocks / 2];
+        const uint32_t vw = vg + q4 * kRow + g * 2 * kBlocks + j * kGroup, vs = vg + q4 * kScaleRow + kScales + j * kGroup;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            mma_f16(s.o[n][2 * b], a0, a1, a2, a3, p0[n], p1[n]);
-            mma_f16(s.o[n][2 * b + 1], b0, b1, b2, b3, p0[n], p1[n]);
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (kBlocks == 4) {
+                const uint2 x = lds64(vw + 4 * i * kRow), y = lds64(vs + 4 * i * kScaleRow);
+                v[i][0] = x.x, v[i][1] = x.y, dv[i][0] = y.x, dv[i][1] = y.y;
+            } else {
+                v[i][0] = lds32(vw + 4 * i * kRow), dv[i][0] = lds32(vs + 4 * i * kScaleRow);
+            }
+            if constexpr (MASKED) {
+                const int key = key0 + j * kKvGroup + q4 + 4 * i;
+                const bool seen = key >= t.lo_min && key < t.hi_max;
+#pragma unroll
+                for (int x = 0; x < kBlocks / 2; ++x) dv[i][x] = seen ? dv[i][x] : 0;
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) {
+            const uint32_t sel = (b & 1) ? 0x7632u : 0x5410u;
+            const uint32_t x = __byte_perm(v[0][b / 2], v[1][b / 2], sel), y = __byte_perm(v[2][b / 2], v[3][b / 2], sel);
+            float d[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) d[i] = (b & 1) ? high_half(dv[i][b / 2]) : low_half(dv[i][b / 2]);
+            uint32_t p0[NT], p1[NT];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                float dp[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    dp[i] = pr[n][i] * d[i];
+                    // 0 times an infinite scale is 0 where the row does not see the key
+                    if constexpr (MASKED) dp[i] = pr[n][i] == 0.0f ? 0.0f : dp[i];
+                }
+                p0[n] = h2(__floats2half2_rn(dp[0], dp[1]));
+                p1[n] = h2(__floats2half2_rn(dp[2], dp[3]));
+            }
+            // low nibbles: 1024 + n - 1032; high ones: (1024 + 16 n) / 16 - 72
+            const auto low = [&](uint32_t z) { return h2(__hadd2(as_h2(and_or<0x000F000Fu>(z, magic)), minus1032)); };
+            const auto high = [&](uint32_t z) {
+                return h2(__hfma2(as_h2(and_or<0x00F000F0u>(z, magic)), sixteenth, minus72));
+            };
+            const uint32_t x8 = x >> 8, y8 = y >> 8;
+            const uint32_t a0 = low(x), a1 = high(x), a2 = low(y), a3 = high(y);
+            const uint32_t b0 = low(x8), b1 = high(x8), b2 = low(y8), b3 = high(y8);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                mma_f16(s.o[n][2 * b], a0, a1, a2, a3, p0[n], p1[n]);
+                mma_f16(s.o[n][2 * b + 1], b0, b1, b2, b3, p0[n], p1[n]);
+            }
         }
     }
 }
@@ -660,7 +683,7 @@ template <int DIM, int NT>
 PFNG_DEV void store_rows(const StreamParams &sp, const Cursor &c, RowSums<DIM, NT> &s, bool whole, int64_t slot) {
     const AttnArgs &p = sp.a;
     const int lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
-    const int group = p.heads_q / p.heads_kv;
+    const int group = p.group;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -700,7 +723,7 @@ PFNG_DEV void store_rows(const StreamParams &sp, const Cursor &c, RowSums<DIM, N
 
 template <int DIM, int NT>
 __global__ void __launch_bounds__(Config<NT>::kThreads, 1) attn_stream_kernel(const StreamParams sp) {
-    constexpr int kWarps = Config<NT>::kWarps, kThreads = Config<NT>::kThreads, kStages = Config<NT>::kStages;
+    constexpr int kWarps = Config<NT>::kWarps, kThreads = Config<NT>::kThreads, kStages = Config<NT>::kStages, kStep = Config<NT>::kStep;
     extern __shared__ __align__(128) uint8_t ring[];
     __shared__ __align__(8) uint64_t bars[kWarps][kStages];
     __shared__ __align__(16) WarpState<DIM, NT> states[kWarps];
@@ -711,15 +734,14 @@ __global__ void __launch_bounds__(Config<NT>::kThreads, 1) attn_stream_kernel(co
         for (int i = 0; i < kStages; ++i) mbar_init(&bars[warp][i], 1);
         fence_mbar_init();
     }
-    int64_t units, none0, none1;
-    line_totals<NT, kThreads>(p, 0, units, none0, none1);  // synchronises
+    const int64_t units = line_units<NT, kThreads>(p);  // synchronises
     pdl_trigger();
     const int64_t workers = static_cast<int64_t>(gridDim.x) * kWarps;
     // a short line goes to the first warp of every SM, then to the second
     const int64_t worker = static_cast<int64_t>(warp) * gridDim.x + blockIdx.x;
     const Pieces pieces(units, workers);
     const int64_t begin = pieces.start(worker), end = pieces.start(worker + 1);
-    if (begin == end) return;
+    if (begin == end && worker > 0) return;  // worker 0 has a unit wherever there is one
 
     const uint32_t ring_at = smem_u32(ring) + warp * kStages * 2 * kHalf;
     const uint64_t policy = l2_policy_evict_first();
@@ -728,7 +750,8 @@ __global__ void __launch_bounds__(Config<NT>::kThreads, 1) attn_stream_kernel(co
     WarpState<DIM, NT> &state = states[warp];
     Fetcher fetcher;
     {
-        const Cursor c = seek<NT>(p, begin);
+        const Cursor c = seek<NT>(p, begin, worker == 0 ? sp.starts : nullptr);
+        if (begin == end) return;
         if (lane == 0) state.ahead = state.at = c;
         __syncwarp();
         fetcher.open<DIM>(p, c);
@@ -770,16 +793,20 @@ __global__ void __launch_bounds__(Config<NT>::kThreads, 1) attn_stream_kernel(co
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         const uint32_t k = ring_at + stage * 2 * kHalf, v = k + kHalf;
+        const uint32_t bits = (there >> (kGroups * stage)) & kGroupMask;
+        if (bits == kGroupMask && key0 >= tile.lo_max && key0 + kUnit <= tile.hi_min) {
 #pragma unroll 1
-        for (int i = 0; i < kGroups; ++i) {
-            const int key = key0 + i * kKvGroup;
-            if (!((there >> (kGroups * stage + i)) & 1u) || key >= tile.hi_max || key + kKvGroup <= tile.lo_min) continue;
-            if (key >= tile.lo_max && key + kKvGroup <= tile.hi_min)
-                attend16<DIM, NT, false>(tile, state, sums, k + i * kv_group_bytes(DIM), v + i * kv_group_bytes(DIM), key,
-                                         magic);
-            else
-                attend16<DIM, NT, true>(tile, state, sums, k + i * kv_group_bytes(DIM), v + i * kv_group_bytes(DIM), key,
-                                        magic);
+            for (int i = 0; i < kGroups; i += kStep)
+                attend<DIM, NT, kStep, false>(tile, state, sums, k + i * kv_group_bytes(DIM), v + i * kv_group_bytes(DIM),
+                                              key0 + i * kKvGroup, magic);
+        } else {
+#pragma unroll 1
+            for (int i = 0; i < kGroups; ++i) {
+                const int key = key0 + i * kKvGroup;
+                if (((bits >> i) & 1u) && key < tile.hi_max && key + kKvGroup > tile.lo_min)
+                    attend<DIM, NT, 1, true>(tile, state, sums, k + i * kv_group_bytes(DIM), v + i * kv_group_bytes(DIM), key,
+                                             magic);
+            }
         }
         __syncwarp();
         if (++stage == kStages) stage = 0, phase ^= 1;
@@ -816,20 +843,18 @@ __global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const StreamPar
     const int64_t r = rest / p.heads_kv;
     const int head_kv = static_cast<int>(rest % p.heads_kv);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int64_t units, before, item;
-    line_totals<NT, kJoinThreads>(p, r, units, before, item);
-    const Pieces pieces(units, workers);
     const RequestShape shape = request_shape<NT>(p, r);
-    const int group = p.heads_q / p.heads_kv;
+    const int group = p.group;
     int64_t per_head = 0;
     for (int t = 0; t < shape.tiles; ++t) {
         int first, count;
         tile_units<NT>(p, shape, t, first, count);
         per_head += count;
     }
-    before += head_kv * per_head;
-    item += static_cast<int64_t>(head_kv) * shape.tiles;
     pdl_wait();
+    const LineStart start = sp.starts[r];
+    const Pieces pieces(sp.starts[p.requests].units, workers);
+    int64_t before = start.units + head_kv * per_head, item = start.items + static_cast<int64_t>(head_kv) * shape.tiles;
     for (int t = 0; t < shape.tiles; ++t, ++item) {
         int first, count;
         tile_units<NT>(p, shape, t, first, count);
@@ -877,7 +902,7 @@ __global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const StreamPar
 }
 static_assert(kJoinThreads >= 128, "a thread per dimension");
 
-int64_t max_rows(const AttnArgs &p) { return p.max_q * (p.heads_q / p.heads_kv); }
+int64_t max_rows(const AttnArgs &p) { return p.max_q * (p.group); }
 int row_tiles_of_8(const AttnArgs &p) { return max_rows(p) <= 8 ? 1 : 2; }
 int64_t max_items(const AttnArgs &p) {
     const int64_t tile = 8 * row_tiles_of_8(p);
@@ -918,7 +943,8 @@ bool attn_stream_supported(const AttnArgs &p) {
 }
 
 size_t attn_stream_workspace(const AttnArgs &p) {
-    return static_cast<size_t>(slots(p)) * (8 * row_tiles_of_8(p)) * (p.head_dim + 2) * sizeof(float) + 256;
+    return static_cast<size_t>(slots(p)) * (8 * row_tiles_of_8(p)) * (p.head_dim + 2) * sizeof(float) +
+           static_cast<size_t>(p.requests + 1) * sizeof(LineStart) + 256;
 }
 
 cudaError_t launch_attn_stream(const AttnArgs &p, void *workspace, int *err, cudaStream_t s) {
@@ -927,6 +953,7 @@ cudaError_t launch_attn_stream(const AttnArgs &p, void *workspace, int *err, cud
     const int64_t rows = slots(p) * 8 * row_tiles_of_8(p);
     sp.part_o = static_cast<float *>(workspace);
     sp.part_ml = reinterpret_cast<float2 *>(sp.part_o + rows * p.head_dim);
+    sp.starts = reinterpret_cast<LineStart *>(sp.part_ml + rows);
     const uintptr_t at = reinterpret_cast<uintptr_t>(p.q);
     sp.vec_q = p.ldq % 4 == 0 && at % (p.q_format == kOutF32 ? 16 : 8) == 0;
     sp.err = err;

@@ -36,7 +36,7 @@ int resolve_attention(const AttnArgs &a, int path) {
     const bool stream = attn_stream_supported(a), mma = attn_mma_supported(a);
     if (path == PFNG_B200_PATH_AUTO) {
         // up to 16 query rows per key head are one tile of the streaming kernel
-        const bool few = a.max_q * (a.heads_q / a.heads_kv) <= 16;
+        const bool few = a.max_q * a.group <= 16;
         if (few && stream) return PFNG_B200_PATH_GEMV;
         return mma ? PFNG_B200_PATH_MMA : PFNG_B200_PATH_SIMPLE;
     }
@@ -142,6 +142,7 @@ size_t pfng_b200_attention_q4_0_workspace_size(int64_t requests, int64_t tokens,
     AttnArgs a{};
     a.requests = requests, a.tokens = tokens, a.max_q = max_q, a.max_kv = max_kv;
     a.heads_q = static_cast<int>(heads_q), a.heads_kv = static_cast<int>(heads_kv);
+    a.group = a.heads_q / a.heads_kv;
     a.head_dim = static_cast<int>(head_dim);
     const int resolved = resolve_attention(a, path);
     return resolved < 0 ? 0 : attention_workspace(a, resolved);
@@ -178,6 +179,7 @@ int pfng_b200_attention_q4_0(const void *q, int64_t ldq, int q_format, const voi
     a.requests = requests, a.tokens = tokens, a.max_q = max_q, a.max_kv = max_kv;
     a.window = window, a.page_size = static_cast<int>(page_size), a.causal = causal != 0, a.scale = scale;
     a.heads_q = static_cast<int>(heads_q), a.heads_kv = static_cast<int>(heads_kv);
+    a.group = a.heads_q / a.heads_kv;
     a.head_dim = static_cast<int>(head_dim);
     a.page_groups = static_cast<int>(page_size / 16);
     a.page_magic = static_cast<uint32_t>(((int64_t{1} << 32) + a.page_groups - 1) / a.page_groups);

@@ -184,7 +184,7 @@ struct AttnArgs {
     int page_size, page_groups;  // tokens and 16-token groups of a page
     uint32_t page_magic;         // ceil(2^32 / page_groups), for page_groups > 1
     int64_t page_bytes;          // bytes of a page of K (and of V), all key heads
-    int heads_q, heads_kv, head_dim, causal;
+    int heads_q, heads_kv, group, head_dim, causal;  // group = heads_q / heads_kv
     float scale;
 };
 cudaError_t launch_attn_simple(const AttnArgs &args, cudaStream_t s);
