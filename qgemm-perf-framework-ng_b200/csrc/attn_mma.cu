@@ -210,6 +210,54 @@ PFNG_DEV uint4 unpack_word(uint32_t w, uint32_t scale, uint32_t magic) {
                       h2(__hmul2(__hfma2(as_h2(and_or<0x00F000F0u>(w8, magic)), sixteenth, minus72), s)));
 }
 
+// One query row into its row of the Q operand, by one thread: scaled by a power
+// of two (and the sign of the softmax scale), in the order of K's words.
+// Returns the factor from accumulators to scores in log2 units.
+template <int DIM, int FMT>
+PFNG_DEV float load_q(const MmaParams &mp, int64_t at, bool live, uint8_t *to, int row) {
+    const AttnArgs &p = mp.a;
+    constexpr int kBlocks = DIM / 32;
+    RawValues<FMT, 4> x[DIM / 4];  // the whole row: one latency
+#pragma unroll
+    for (int c = 0; c < DIM / 4; ++c) x[c].zero();
+    if (live && mp.vec_q) {
+#pragma unroll
+        for (int c = 0; c < DIM / 4; ++c) x[c].load(p.q, at + 4 * c);
+    } else if (live) {
+#pragma unroll
+        for (int c = 0; c < DIM / 4; ++c)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                RawValues<FMT, 1> one;
+                one.load(p.q, at + 4 * c + j);
+                if constexpr (FMT == kOutF32) x[c].w[j] = one.w[0];
+                else x[c].w[j / 2] |= one.w[0] << (16 * (j & 1));
+            }
+    }
+    float top = 0.0f;
+#pragma unroll
+    for (int c = 0; c < DIM / 4; ++c)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) top = fmaxf(top, fabsf(x[c][j]));
+    int e = 0;
+    if (top > 0.0f && top < INFINITY) e = exponent_of(top) - 13;
+    const float up0 = power_of_two(-(e / 2)) * (p.scale < 0.0f ? -1.0f : 1.0f), up1 = power_of_two(-(e - e / 2));
+#pragma unroll
+    for (int c = 0; c < DIM / 8; ++c) {
+        const int t = c / kBlocks, b = c % kBlocks;
+        float v[2][4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[h][j] = x[8 * b + 4 * h + t][j] * up0 * up1;
+        *reinterpret_cast<uint4 *>(to + operand_at(row, c)) =
+            make_uint4(h2(__floats2half2_rn(v[0][0], v[0][2])), h2(__floats2half2_rn(v[0][1], v[0][3])),
+                       h2(__floats2half2_rn(v[1][0], v[1][2])), h2(__floats2half2_rn(v[1][1], v[1][3])));
+    }
+    // a floor keeps -inf * mul at -inf for a scale of 0
+    return fmaxf(fabsf(p.scale) * kLog2e * power_of_two(e / 2) * power_of_two(e - e / 2), 1e-35f);
+}
+
 template <int DIM>
 __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams mp) {
     using L = Layout<DIM>;
@@ -364,54 +412,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
             float mul;
             {  // Q: largest value of the row into [2^13, 2^14), sign of the softmax scale included
                 const int64_t at = token * p.ldq + head * DIM;
-                float top = 0.0f;
-#pragma unroll 4
-                for (int c = 0; c < DIM / 4; ++c) {
-                    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                    if (live) {
-                        if (mp.vec_q) {
-                            load_values<4>(p.q_format, p.q, at + 4 * c, v);
-                        } else {
-                            for (int j = 0; j < 4; ++j) {
-                                float one[1];
-                                load_values<1>(p.q_format, p.q, at + 4 * c + j, one);
-                                v[j] = one[0];
-                            }
-                        }
-                    }
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) top = fmaxf(top, fabsf(v[j]));
-                }
-                int e = 0;
-                if (top > 0.0f && top < INFINITY) e = exponent_of(top) - 13;
-                const float up0 = power_of_two(-(e / 2)) * (p.scale < 0.0f ? -1.0f : 1.0f),
-                            up1 = power_of_two(-(e - e / 2));
-                // a floor keeps -inf * mul at -inf for a scale of 0
-                mul = fmaxf(fabsf(p.scale) * kLog2e * power_of_two(e / 2) * power_of_two(e - e / 2), 1e-35f);
-#pragma unroll 2
-                for (int c = 0; c < DIM / 8; ++c) {
-                    const int t = c / kBlocks, b = c % kBlocks;
-                    float v[2][4] = {};
-                    if (live) {
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            if (mp.vec_q) {
-                                load_values<4>(p.q_format, p.q, at + 32 * b + 16 * h + 4 * t, v[h]);
-                            } else {
-                                for (int j = 0; j < 4; ++j) {
-                                    float one[1];
-                                    load_values<1>(p.q_format, p.q, at + 32 * b + 16 * h + 4 * t + j, one);
-                                    v[h][j] = one[0];
-                                }
-                            }
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) v[h][j] = v[h][j] * up0 * up1;
-                        }
-                    }
-                    *reinterpret_cast<uint4 *>(smem + L::kQ + i * L::kOperand + operand_at(in_tile, c)) = make_uint4(
-                        h2(__floats2half2_rn(v[0][0], v[0][2])), h2(__floats2half2_rn(v[0][1], v[0][3])),
-                        h2(__floats2half2_rn(v[1][0], v[1][2])), h2(__floats2half2_rn(v[1][1], v[1][3])));
-                }
+                uint8_t *to = smem + L::kQ + i * L::kOperand;
+                if (p.q_format == kOutF32)
+                    mul = load_q<DIM, kOutF32>(mp, at, live, to, in_tile);
+                else if (p.q_format == kOutF16)
+                    mul = load_q<DIM, kOutF16>(mp, at, live, to, in_tile);
+                else
+                    mul = load_q<DIM, kOutBF16>(mp, at, live, to, in_tile);
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(q_full);
