@@ -210,52 +210,73 @@ PFNG_DEV uint4 unpack_word(uint32_t w, uint32_t scale, uint32_t magic) {
                       h2(__hmul2(__hfma2(as_h2(and_or<0x00F000F0u>(w8, magic)), sixteenth, minus72), s)));
 }
 
-// One query row into its row of the Q operand, by one thread: scaled by a power
-// of two (and the sign of the softmax scale), in the order of K's words.
-// Returns the factor from accumulators to scores in log2 units.
+// The 32 query rows of a warp into their rows of the Q operand: scaled by a
+// power of two each (and the sign of the softmax scale), in the order of K's
+// words.  DIM / 8 lanes read a row, eight values each, so that a load covers
+// whole lines (a row per lane took 15000 cycles for a CTA's rows).  Returns,
+// for the row of this lane, the factor from accumulators to scores in log2
+// units.  row: the warp's first row; `at`, `live`: where this lane's row is.
 template <int DIM, int FMT>
 PFNG_DEV float load_q(const MmaParams &mp, int64_t at, bool live, uint8_t *to, int row) {
     const AttnArgs &p = mp.a;
-    constexpr int kBlocks = DIM / 32;
-    RawValues<FMT, 4> x[DIM / 4];  // the whole row: one latency
+    constexpr int kLanes = DIM / 8, kAtOnce = 32 / kLanes, kSteps = 32 / kAtOnce, kBatch = FMT == kOutF32 ? 4 : 8;
+    const int lane = threadIdx.x & 31, sub = lane % kLanes, part = lane / kLanes;
+    float mul = 0.0f;
+#pragma unroll 1
+    for (int step0 = 0; step0 < kSteps; step0 += kBatch) {
+        RawValues<FMT, 8> x[kBatch];
 #pragma unroll
-    for (int c = 0; c < DIM / 4; ++c) x[c].zero();
-    if (live && mp.vec_q) {
+        for (int k = 0; k < kBatch; ++k) {
+            const int mine = (step0 + k) * kAtOnce + part;  // of the warp's rows
+            const int64_t from = __shfl_sync(0xffffffffu, at, mine) + 8 * sub;
+            x[k].zero();
+            if (!__shfl_sync(0xffffffffu, static_cast<int>(live), mine)) continue;
+            if (mp.vec_q) {
+                x[k].load(p.q, from);
+            } else {
 #pragma unroll
-        for (int c = 0; c < DIM / 4; ++c) x[c].load(p.q, at + 4 * c);
-    } else if (live) {
+                for (int j = 0; j < 8; ++j) {
+                    RawValues<FMT, 1> one;
+                    one.load(p.q, from + j);
+                    if constexpr (FMT == kOutF32) x[k].w[j] = one.w[0];
+                    else x[k].w[j / 2] |= one.w[0] << (16 * (j & 1));
+                }
+            }
+        }
 #pragma unroll
-        for (int c = 0; c < DIM / 4; ++c)
+        for (int k = 0; k < kBatch; ++k) {
+            float top = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[k][j]));
+#pragma unroll
+            for (int o = 1; o < kLanes; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            // largest value into [2^13, 2^14)
+            int e = 0;
+            if (top > 0.0f && top < INFINITY) e = exponent_of(top) - 13;
+            const float up0 = power_of_two(-(e / 2)) * (p.scale < 0.0f ? -1.0f : 1.0f), up1 = power_of_two(-(e - e / 2));
+            // a floor keeps -inf * mul at -inf for a scale of 0
+            const float row_mul = fmaxf(fabsf(p.scale) * kLog2e * power_of_two(e / 2) * power_of_two(e - e / 2), 1e-35f);
+            uint32_t h[4];
+            // values 0, 2 and 1, 3 of each four in a register
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                RawValues<FMT, 1> one;
-                one.load(p.q, at + 4 * c + j);
-                if constexpr (FMT == kOutF32) x[c].w[j] = one.w[0];
-                else x[c].w[j / 2] |= one.w[0] << (16 * (j & 1));
+                const int v = 4 * (j >> 1) + (j & 1);
+                h[j] = h2(__floats2half2_rn(x[k][v] * up0 * up1, x[k][v + 2] * up0 * up1));
             }
+            // chunk t of a block: values 4 t .. and 16 + 4 t ..; this lane has values 8 (sub % 4) .. of its
+            // block: t = 0, 1 are made by lanes 0 and 2 of the four, t = 2, 3 by lanes 1 and 3
+            const bool upper = sub & 2;
+            const uint32_t r0 = __shfl_xor_sync(0xffffffffu, upper ? h[0] : h[2], 2);
+            const uint32_t r1 = __shfl_xor_sync(0xffffffffu, upper ? h[1] : h[3], 2);
+            const int t = 2 * (sub & 1) + (upper ? 1 : 0), c = t * (DIM / 32) + sub / 4;
+            *reinterpret_cast<uint4 *>(to + operand_at(row + (step0 + k) * kAtOnce + part, c)) =
+                upper ? make_uint4(r0, r1, h[2], h[3]) : make_uint4(h[0], h[1], r0, r1);
+            // the lane that owns a row takes its factor
+            const float m = __shfl_sync(0xffffffffu, row_mul, (lane % kAtOnce) * kLanes);
+            if (lane / kAtOnce == step0 + k) mul = m;
+        }
     }
-    float top = 0.0f;
-#pragma unroll
-    for (int c = 0; c < DIM / 4; ++c)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) top = fmaxf(top, fabsf(x[c][j]));
-    int e = 0;
-    if (top > 0.0f && top < INFINITY) e = exponent_of(top) - 13;
-    const float up0 = power_of_two(-(e / 2)) * (p.scale < 0.0f ? -1.0f : 1.0f), up1 = power_of_two(-(e - e / 2));
-#pragma unroll
-    for (int c = 0; c < DIM / 8; ++c) {
-        const int t = c / kBlocks, b = c % kBlocks;
-        float v[2][4];
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[h][j] = x[8 * b + 4 * h + t][j] * up0 * up1;
-        *reinterpret_cast<uint4 *>(to + operand_at(row, c)) =
-            make_uint4(h2(__floats2half2_rn(v[0][0], v[0][2])), h2(__floats2half2_rn(v[0][1], v[0][3])),
-                       h2(__floats2half2_rn(v[1][0], v[1][2])), h2(__floats2half2_rn(v[1][1], v[1][3])));
-    }
-    // a floor keeps -inf * mul at -inf for a scale of 0
-    return fmaxf(fabsf(p.scale) * kLog2e * power_of_two(e / 2) * power_of_two(e - e / 2), 1e-35f);
+    return mul;
 }
 
 template <int DIM>
@@ -414,11 +435,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
                 const int64_t at = token * p.ldq + head * DIM;
                 uint8_t *to = smem + L::kQ + i * L::kOperand;
                 if (p.q_format == kOutF32)
-                    mul = load_q<DIM, kOutF32>(mp, at, live, to, in_tile);
+                    mul = load_q<DIM, kOutF32>(mp, at, live, to, (warp & 3) * 32);
                 else if (p.q_format == kOutF16)
-                    mul = load_q<DIM, kOutF16>(mp, at, live, to, in_tile);
+                    mul = load_q<DIM, kOutF16>(mp, at, live, to, (warp & 3) * 32);
                 else
-                    mul = load_q<DIM, kOutBF16>(mp, at, live, to, in_tile);
+                    mul = load_q<DIM, kOutBF16>(mp, at, live, to, (warp & 3) * 32);
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(q_full);
@@ -510,45 +531,68 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
             const float f = none ? 0.0f : 1.0f / l;
             if (ok) {
                 const int64_t at = token * p.ldo + head * DIM;
+                // Through shared memory (this row tile's Q, which no MMA reads any more), so that a store covers
+                // whole lines: rows of DIM / 4 pieces of four values, piece x of row y at x ^ y.
+                const int size = p.out_format == kOutF32 ? 4 : 2, rows_at_once = 64 / size;
+                constexpr int kPieces = DIM / 4;
+                uint8_t *mine = smem + L::kQ + i * L::kOperand + (warp & 3) * (L::kOperand / 4);
 #pragma unroll 1
-                for (int c = 0; c < DIM / 32; ++c) {
-                    uint32_t o[32] = {};
-                    if (count > 0) {
-                        tmem_ld32(o_at + 32 * c, o);
-                        tmem_wait_ld<32>(o);
-                    }
-                    if (!live) continue;
+                for (int row1 = 0; row1 < 32; row1 += rows_at_once) {
+                    const int y = lane - row1;
+                    const bool staged = mp.vec_out && y >= 0 && y < rows_at_once;
+#pragma unroll 1
+                    for (int c = 0; c < DIM / 32; ++c) {
+                        uint32_t o[32] = {};
+                        if (count > 0) {
+                            tmem_ld32(o_at + 32 * c, o);
+                            tmem_wait_ld<32>(o);
+                        }
 #pragma unroll
-                    for (int b = 0; b < kBlocks; ++b)
+                        for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
-                        for (int h = 0; h < 2; ++h)
+                            for (int h = 0; h < 2; ++h)
 #pragma unroll
-                            for (int x = 0; x < (kBlocks == 4 ? 1 : 2); ++x) {
-                                // words of a V row: (g, pair of blocks); element (b & 1) + 2 e + 4 h of a word is
-                                // dimension 2 g + e + 16 h of block b
-                                float v[4];
-                                int dim;
-                                if constexpr (kBlocks == 4) {
-                                    dim = 32 * b + 16 * h + 4 * c;
+                                for (int x = 0; x < (kBlocks == 4 ? 1 : 2); ++x) {
+                                    // words of a V row: (g, pair of blocks); element (b & 1) + 2 e + 4 h of a word is
+                                    // dimension 2 g + e + 16 h of block b
+                                    float v[4];
+                                    int dim;
+                                    if constexpr (kBlocks == 4) {
+                                        dim = 32 * b + 16 * h + 4 * c;
 #pragma unroll
-                                    for (int j = 0; j < 4; ++j)
-                                        v[j] = __uint_as_float(o[(2 * (j >> 1) + (b >> 1)) * 8 + (b & 1) + 2 * (j & 1) + 4 * h]) * f;
-                                } else {
-                                    dim = 32 * b + 16 * h + 8 * c + 4 * x;
+                                        for (int j = 0; j < 4; ++j)
+                                            v[j] = __uint_as_float(o[(2 * (j >> 1) + (b >> 1)) * 8 + (b & 1) + 2 * (j & 1) + 4 * h]) * f;
+                                    } else {
+                                        dim = 32 * b + 16 * h + 8 * c + 4 * x;
 #pragma unroll
-                                    for (int j = 0; j < 4; ++j)
-                                        v[j] = __uint_as_float(o[(2 * x + (j >> 1)) * 8 + b + 2 * (j & 1) + 4 * h]) * f;
-                                }
-                                if (mp.vec_out) {
-                                    store_values<4>(p.out_format, p.out, at + dim, v);
-                                } else {
-#pragma unroll
-                                    for (int j = 0; j < 4; ++j) {
-                                        const float one[1] = {v[j]};
-                                        store_values<1>(p.out_format, p.out, at + dim + j, one);
+                                        for (int j = 0; j < 4; ++j)
+                                            v[j] = __uint_as_float(o[(2 * x + (j >> 1)) * 8 + b + 2 * (j & 1) + 4 * h]) * f;
+                                    }
+                                    if (staged) {
+                                        store_values<4>(p.out_format, mine, (y * kPieces + ((dim / 4) ^ (y % kPieces))) * 4, v);
+                                    } else if (!mp.vec_out && live && row1 == 0) {
+                                        for (int j = 0; j < 4; ++j) {
+                                            const float one[1] = {v[j]};
+                                            store_values<1>(p.out_format, p.out, at + dim + j, one);
+                                        }
                                     }
                                 }
-                            }
+                    }
+                    __syncwarp();
+                    if (mp.vec_out) {
+                        for (int idx = lane; idx < rows_at_once * kPieces; idx += 32) {
+                            const int z = idx / kPieces, x = idx % kPieces, from = (z * kPieces + (x ^ (z % kPieces))) * 4;
+                            const int64_t to = __shfl_sync(0xffffffffu, at, row1 + z) + 4 * x;
+                            if (!__shfl_sync(0xffffffffu, static_cast<int>(live), row1 + z)) continue;
+                            if (size == 4)
+                                *reinterpret_cast<uint4 *>(static_cast<float *>(p.out) + to) =
+                                    *reinterpret_cast<const uint4 *>(mine + from * 4);
+                            else
+                                *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + to) =
+                                    *reinterpret_cast<const uint2 *>(mine + from * 2);
+                        }
+                    }
+                    __syncwarp();
                 }
                 if (live && p.lse)
                     p.lse[token * p.heads_q + head] = none ? -INFINITY : (m + log2f(l)) / kLog2e;
@@ -707,7 +751,7 @@ cudaError_t launch_attn_mma(const AttnArgs &p, int *err, cudaStream_t s) {
     const auto wide = [](const void *x, int64_t ld, int fmt) {
         return ld % 4 == 0 && reinterpret_cast<uintptr_t>(x) % (fmt == kOutF32 ? 16 : 8) == 0;
     };
-    mp.vec_q = wide(p.q, p.ldq, p.q_format);
+    mp.vec_q = p.ldq % 8 == 0 && reinterpret_cast<uintptr_t>(p.q) % 16 == 0;
     mp.vec_out = wide(p.out, p.ldo, p.out_format);
     mp.tiles = static_cast<int>(row_blocks(p));
     mp.err = err;
