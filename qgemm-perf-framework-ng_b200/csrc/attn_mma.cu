@@ -7,19 +7,21 @@
 //   S_i = Q_i K^T          tcgen05.mma, both operands in shared memory, S in TMEM
 //   P_i = 2^(S_i - m)      one thread per row: TMEM -> registers -> TMEM (fp16)
 //   O_i += P_i V           tcgen05.mma, P from TMEM, V from shared memory
-// for i = 0, 1 in turn, so that the tensor cores work on one tile while the
-// other's softmax runs.  Roles (512 threads, one CTA per SM):
+// for i = 0, 1, by 64 keys: S of a row tile has two buffers of 64 columns (P
+// goes over its S), so the MMAs of 64 keys run while the softmax is at the 64
+// before them.  Roles (512 threads, one CTA per SM):
 //   warps 0-7    softmax, a warpgroup per row tile; they load Q, rescale O
 //                and write the output
-//   warps 8-11, 14, 15  dequantization: nibbles and scales of a tile -> fp16
-//                operand rows in the 128-byte swizzled layout
+//   warp 8       copies the tiles' groups from the pages (bulk copies, a ring
+//                of raw K or V tiles)
 //   warp 12      issues the MMAs
-//   warp 13      copies the tiles' groups from the pages (bulk copies, a ring
-//                of six raw K or V tiles)
+//   warps 9-11, 13-15  dequantization: nibbles and scales of a tile -> fp16
+//                operand rows in the 128-byte swizzled layout; none of them on
+//                the scheduler that the MMA warp shares with two softmax warps
 // One dequantization serves 256 rows: 13 instructions per 8 values.  Bounds per
 // 256 x 128 step, in cycles: 2048 of MMA, 2048 of exponentials (16 per cycle and
-// SM), about 2300 of shared memory (operands read by the MMAs, dequantized
-// tiles written).
+// SM), about 2800 of shared memory (Q, K and V read by the MMAs: 256 KB; tiles
+// dequantized: 100 KB; at 128 bytes a cycle).
 //
 // Precision: d (n - 8) is rounded to fp16 (2^-12 on average), P to fp16 with
 // the row's largest at 2^8..2^15 (so that small ones stay normal numbers);
@@ -42,14 +44,15 @@ constexpr int kRows = 2 * kTile;
 constexpr int kThreads = 512;
 constexpr int kDequantWarps = 6;
 constexpr int kGroups = kTile / kKvGroup;  // 16-key groups of a unit: the tasks of the dequantizing warps
-constexpr int kRawSlots = 6;
-constexpr int kOperands = 3;     // dequantized K or V tiles: unit 2 n is K of key tile n, unit 2 n + 1 its V
+constexpr int kStep = 64;        // keys of an S buffer
+constexpr int kRawSlots = 3;
+constexpr int kOperands = 4;     // dequantized K or V tiles: unit 2 n is K of key tile n, unit 2 n + 1 its V
 constexpr int kInfoSlots = 16;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNoMax = -3.0e38f;
 constexpr float kLift = 8.0f;    // log2 of P at a renewed maximum
 constexpr float kSlack = 7.0f;   // a score may pass the maximum by this before it is renewed
-constexpr uint32_t kTmemCols = 512;  // S0 S1 (P over S) at 0 and 128, O0 O1 at 256 and 384
+constexpr uint32_t kTmemCols = 512;  // S_i at 128 i + 64 buffer (P over S), O_i at 256 + 128 i
 
 // What the softmax needs to know about a key tile beyond its numbers.
 struct TileInfo {
@@ -66,7 +69,7 @@ struct Layout {
     static constexpr uint32_t kRawAt = kKV + kOperands * kOperand;  // [kRawSlots]
     static constexpr uint32_t kInfo = kRawAt + kRawSlots * kRaw;
     static constexpr uint32_t kBars = kInfo + ((kInfoSlots * sizeof(TileInfo) + 7) & ~7u);
-    static constexpr uint32_t kNumBars = 2 * kRawSlots + 2 * kOperands + 2 + 4 + 2 + 2;
+    static constexpr uint32_t kNumBars = 2 * kRawSlots + 2 * kOperands + 4 + 4 + 2 + 2;
     static constexpr uint32_t kBytes = kBars + 8 * kNumBars + 16 + 1024;
 };
 
@@ -156,11 +159,6 @@ PFNG_DEV void tmem_wait_ld(uint32_t *x) {
     }
 }
 PFNG_DEV void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-template <int N>
-PFNG_DEV void registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N>
-PFNG_DEV void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
-
 PFNG_DEV float exp2_approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -288,7 +286,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::kBars);
     uint64_t *raw_full = bars, *raw_empty = raw_full + kRawSlots;
     uint64_t *op_full = raw_empty + kRawSlots, *op_empty = op_full + kOperands;
-    uint64_t *s_full = op_empty + kOperands, *p_full = s_full + 2, *o_full = p_full + 4;
+    uint64_t *s_full = op_empty + kOperands, *p_full = s_full + 4, *o_full = p_full + 4;  // [row tile][buffer]; o_full: every O += P V
     uint64_t *q_full = o_full + 2, *mma_done = q_full + 1;
     uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(bars + L::kNumBars);
     TileInfo *infos = reinterpret_cast<TileInfo *>(smem + L::kInfo);
@@ -322,7 +320,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
         for (int i = 0; i < kRawSlots; ++i) mbar_init(&raw_full[i], 1), mbar_init(&raw_empty[i], kGroups);
         for (int i = 0; i < kOperands; ++i) mbar_init(&op_full[i], kGroups), mbar_init(&op_empty[i], 1);
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&s_full[i], 1), mbar_init(&o_full[i], 1);
+            mbar_init(&o_full[i], 1);
+            mbar_init(&s_full[2 * i], 1), mbar_init(&s_full[2 * i + 1], 1);
             mbar_init(&p_full[2 * i], 4), mbar_init(&p_full[2 * i + 1], 4);
 
         }
@@ -417,11 +416,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
         return true;
     };
 
-    // Registers: 512 threads x 128 at launch, 2 x 192 + 2 x 64 a thread of the
-    // four warpgroups after this.
     if (warp < 8) {
         // ---------------- softmax ----------------
-        registers_up<192>();
         const int i = warp >> 2;  // row tile
         const int in_tile = (warp & 3) * 32 + lane, row = row0 + i * kTile + in_tile;
         const bool live = row < rows;
@@ -457,30 +453,34 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
                         if (((info.bad[c >> 5] >> (c & 31)) & 1u) && key0 + c >= lo && key0 + c < hi)
                             l = __int_as_float(0x7fffffff);
             };
-            for (int n = 0; n < count; ++n) {
-                if (!wait_bar(&s_full[i], n & 1, &abort_flag, mp.err, kErrWaitFull)) {
+            const int steps = count * (kTile / kStep);
+#pragma unroll 1
+            for (int u = 0; u < steps; ++u) {
+                const int n = u >> 1, buf = u & 1;
+                if (!wait_bar(&s_full[2 * i + buf], (u >> 1) & 1, &abort_flag, mp.err, kErrWaitFull)) {
                     ok = false;
                     break;
                 }
                 tc_fence_after();
-                const uint32_t groups = infos[n % kInfoSlots].groups;
-                if (n > 0) bad_keys(n - 1);  // V of the last tile is complete: this tile's MMA came after its own
-                const int from = lo - (first + n) * kTile, to = hi - (first + n) * kTile;
-                const bool masked = __any_sync(0xffffffffu, from > 0 || to < kTile) || groups != 0xffu;
-                uint32_t s[kTile];
-#pragma unroll
-                for (int c = 0; c < kTile; c += 32) tmem_ld32(s_at + c, s + c);
-                tmem_wait_ld<kTile>(s);
+                const uint32_t at = s_at + kStep * buf;
+                uint32_t s[kStep];
+                tmem_ld32(at, s);
+                tmem_ld32(at + 32, s + 32);
+                const uint32_t groups = (infos[n % kInfoSlots].groups >> (buf * (kStep / kKvGroup))) & 0xfu;
+                if (u > 0 && buf == 0) bad_keys(n - 1);  // this S came after O += P V of 64 keys before the last
+                const int from = lo - first * kTile - u * kStep, to = hi - first * kTile - u * kStep;
+                const bool masked = __any_sync(0xffffffffu, from > 0 || to < kStep) || groups != 0xfu;
+                tmem_wait_ld<kStep>(s);
                 if (masked) {  // what a row does not see is -inf
 #pragma unroll
-                    for (int c = 0; c < kTile; ++c)
+                    for (int c = 0; c < kStep; ++c)
                         if (!(c >= from && c < to && ((groups >> (c / kKvGroup)) & 1u))) s[c] = 0xff800000u;
                 }
                 float tops[4];
 #pragma unroll
                 for (int x = 0; x < 4; ++x) tops[x] = -INFINITY;
 #pragma unroll
-                for (int x = 0; x < kTile; x += 8)
+                for (int x = 0; x < kStep; x += 8)
 #pragma unroll
                     for (int y = 0; y < 4; ++y)
                         tops[y] = fmaxf(fmaxf(tops[y], __uint_as_float(s[x + y])), __uint_as_float(s[x + y + 4]));
@@ -490,7 +490,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
                     const float f = exp2_approx(m - m_new);
                     m = m_new;
                     l *= f;
-                    if (n > 0) {
+                    if (u > 0) {  // O of the 64 keys before this has to be complete
+                        ok = wait_bar(&o_full[i], (u - 1) & 1, &abort_flag, mp.err, kErrWaitFull);
+                        if (!ok) break;
+                        tc_fence_after();
 #pragma unroll 1
                         for (int c = 0; c < DIM; c += 32) {
                             uint32_t o[32];
@@ -504,25 +507,22 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
                 }
                 float sum[4] = {};
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {  // by halves of the keys: their part of O += P V can start
-#pragma unroll
-                    for (int x = 64 * h; x < 64 * h + 64; x += 2) {
-                        const float u = exp2_approx(fmaf(__uint_as_float(s[x]), mul, -m));
-                        const float w = exp2_approx(fmaf(__uint_as_float(s[x + 1]), mul, -m));
-                        sum[x & 2] += u;
-                        sum[(x & 2) + 1] += w;
-                        s[x / 2] = h2(__floats2half2_rn(u, w));
-                    }
-                    tmem_st32(s_at + 32 * h, s + 32 * h);  // P over S
-                    tmem_wait_st();
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&p_full[2 * i + h]);
+                for (int x = 0; x < kStep; x += 2) {
+                    const float v = exp2_approx(fmaf(__uint_as_float(s[x]), mul, -m));
+                    const float w = exp2_approx(fmaf(__uint_as_float(s[x + 1]), mul, -m));
+                    sum[x & 2] += v;
+                    sum[(x & 2) + 1] += w;
+                    s[x / 2] = h2(__floats2half2_rn(v, w));
                 }
+                tmem_st32(at, s);  // P over S
                 l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[2 * i + buf]);
             }
             if (ok && count > 0) {
-                ok = wait_bar(&o_full[i], 0, &abort_flag, mp.err, kErrWaitFull);
+                ok = wait_bar(&o_full[i], (steps - 1) & 1, &abort_flag, mp.err, kErrWaitFull);
                 if (ok) bad_keys(count - 1);
             }
             if (!ok) abort_flag = 1;
@@ -599,7 +599,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
             }
         }
     } else {
-        registers_down<64>();
         if (warp == 12) {
             // ---------------- MMA issue ----------------
             const uint32_t leader = elect_leader();
@@ -607,18 +606,19 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
             // little more than wait.  Descriptors differ by their address
             // field, in the low word, only.  (A thread per row tile measured
             // 13 % slower: MMAs of two accumulators then alternate.)
-            constexpr uint32_t kIdescS = idesc_f16(kTile, false), kIdescO = idesc_f16(DIM, true);
+            constexpr uint32_t kIdescS = idesc_f16(kStep, false), kIdescO = idesc_f16(DIM, true);
             constexpr uint32_t kHalf = (kTile * 128) >> 4, kBuf = L::kOperand >> 4;
             const uint64_t q_desc = sw128_desc(base + L::kQ);
             const uint64_t k_desc = sw128_desc(base + L::kKV), v_desc0 = v_desc(base + L::kKV);
             bool ok = count > 0;
-            const auto scores = [&](int i, uint32_t buf) {  // S_i = Q_i K^T
-                const uint64_t q = q_desc + i * kBuf, k = k_desc + buf * kBuf;
+            // S of row tile i for half h of the key tile in operand buffer `op`
+            const auto scores = [&](int i, int h, uint32_t op) {
+                const uint64_t q = q_desc + i * kBuf, k = k_desc + op * kBuf + h * ((kStep * 128) >> 4);
 #pragma unroll
                 for (int x = 0; x < DIM / 16; ++x)
-                    umma_f16_ss(leader, tmem + i * kTile, q + (x >> 2) * kHalf + (x & 3) * 2, k + (x >> 2) * kHalf + (x & 3) * 2,
-                                kIdescS, x > 0);
-                umma_commit_by(leader, &s_full[i]);
+                    umma_f16_ss(leader, tmem + i * kTile + h * kStep, q + (x >> 2) * kHalf + (x & 3) * 2,
+                                k + (x >> 2) * kHalf + (x & 3) * 2, kIdescS, x > 0);
+                umma_commit_by(leader, &s_full[2 * i + h]);
             };
             const auto ready = [&](uint64_t *bar, uint32_t parity) {
                 return __all_sync(0xffffffffu, mbar_test_wait(bar, parity) ||
@@ -627,8 +627,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
             if (ok) ok = ready(q_full, 0) && ready(&op_full[0], 0);
             if (ok) {
                 tc_fence_after();
-                scores(0, 0);
-                if (row_tiles > 1) scores(1, 0);
+#pragma unroll 1
+                for (int h = 0; h < 2; ++h)
+                    for (int i = 0; i < row_tiles; ++i) scores(i, h, 0);
                 umma_commit_by(leader, &op_empty[0]);
             }
             uint32_t vb = 1, v_phase = 0;  // buffer of V(n); K(n + 1) is in the one after it
@@ -636,38 +637,35 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
             for (int n = 0; n < count && ok; ++n) {
                 const uint32_t kb = vb + 1 == kOperands ? 0 : vb + 1, k_phase = vb + 1 == kOperands ? v_phase ^ 1 : v_phase;
                 const bool more = n + 1 < count;
-                const uint64_t v = v_desc0 + vb * kBuf;
-                ok = ready(&op_full[vb], v_phase);
 #pragma unroll 1
-                for (int i = 0; i < row_tiles && ok; ++i) {
-#pragma unroll
-                    for (int h = 0; h < 2 && ok; ++h) {  // O_i += P_i V, by halves of the keys
+                for (int h = 0; h < 2 && ok; ++h) {
+                    const uint64_t v = v_desc0 + vb * kBuf + h * ((kStep * 128) >> 4);
+                    if (h == 0) ok = ready(&op_full[vb], v_phase);
+#pragma unroll 1
+                    for (int i = 0; i < row_tiles && ok; ++i) {
                         ok = ready(&p_full[2 * i + h], n & 1);
-                        tc_fence_after();
                         if (!ok) break;
+                        tc_fence_after();
 #pragma unroll
-                        for (int x = 4 * h; x < 4 * h + 4; ++x)
-                            umma_f16_ts(leader, tmem + 256 + i * kTile, tmem + i * kTile + 8 * x, v + x * (2048 >> 4), kIdescO,
-                                        n > 0 || x > 0);
-                    }
-                    if (!ok) break;
-                    if (i == row_tiles - 1) umma_commit_by(leader, &op_empty[vb]);
-                    if (!more) {
+                        for (int x = 0; x < kStep / 16; ++x)  // O_i += P_i V
+                            umma_f16_ts(leader, tmem + 256 + i * kTile, tmem + i * kTile + h * kStep + 8 * x,
+                                        v + x * (2048 >> 4), kIdescO, n > 0 || h > 0 || x > 0);
                         umma_commit_by(leader, &o_full[i]);
-                        continue;
+                        if (!more) continue;
+                        if (h == 0 && i == 0) ok = ready(&op_full[kb], k_phase);
+                        if (ok) scores(i, h, kb);
                     }
-                    if (i == 0) ok = ready(&op_full[kb], k_phase);
-                    if (!ok) break;
-                    scores(i, kb);
-                    if (i == row_tiles - 1) umma_commit_by(leader, &op_empty[kb]);
                 }
+                if (!ok) break;
+                umma_commit_by(leader, &op_empty[vb]);
+                if (more) umma_commit_by(leader, &op_empty[kb]);
                 vb = kb + 1 == kOperands ? 0 : kb + 1;
                 v_phase = kb + 1 == kOperands ? k_phase ^ 1 : k_phase;
             }
             if (!ok && count > 0) abort_flag = 1;
             umma_commit_by(leader, mma_done);  // TMEM is freed at the end: no MMA may be in flight
             if (!mbar_wait(mma_done, 0, mp.err, kErrWaitFull)) abort_flag = 1;
-        } else if (warp == 13) {
+        } else if (warp == 8) {
             // ---------------- copies from the pages ----------------
             const uint64_t policy = l2_policy_evict_normal();
             bool ok = true;
@@ -715,7 +713,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
             if (!ok || aborted(&abort_flag))
                 for (int x = max(j - kRawSlots, 0); x < j; ++x)
                     mbar_wait(&raw_full[x % kRawSlots], (x / kRawSlots) & 1, mp.err, kErrWaitFull);
-        } else if (!dequantize(warp < 12 ? warp - 8 : warp - 10)) {
+        } else if (!dequantize(warp < 12 ? warp - 9 : warp - 10)) {
             abort_flag = 1;
         }
         __syncwarp();
