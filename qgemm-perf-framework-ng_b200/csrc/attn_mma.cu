@@ -7,21 +7,19 @@
 //   S_i = Q_i K^T          tcgen05.mma, both operands in shared memory, S in TMEM
 //   P_i = 2^(S_i - m)      one thread per row: TMEM -> registers -> TMEM (fp16)
 //   O_i += P_i V           tcgen05.mma, P from TMEM, V from shared memory
-// for i = 0, 1, by 64 keys: S of a row tile has two buffers of 64 columns (P
-// goes over its S), so the MMAs of 64 keys run while the softmax is at the 64
-// before them.  Roles (512 threads, one CTA per SM):
+// for i = 0, 1 in turn, so that the tensor cores work on one tile while the
+// other's softmax runs.  Roles (512 threads, one CTA per SM):
 //   warps 0-7    softmax, a warpgroup per row tile; they load Q, rescale O
 //                and write the output
-//   warp 8       copies the tiles' groups from the pages (bulk copies, a ring
-//                of raw K or V tiles)
+//   warps 8-11, 14, 15  dequantization: nibbles and scales of a tile -> fp16
+//                operand rows in the 128-byte swizzled layout
 //   warp 12      issues the MMAs
-//   warps 9-11, 13-15  dequantization: nibbles and scales of a tile -> fp16
-//                operand rows in the 128-byte swizzled layout; none of them on
-//                the scheduler that the MMA warp shares with two softmax warps
+//   warp 13      copies the tiles' groups from the pages (bulk copies, a ring
+//                of six raw K or V tiles)
 // One dequantization serves 256 rows: 13 instructions per 8 values.  Bounds per
 // 256 x 128 step, in cycles: 2048 of MMA, 2048 of exponentials (16 per cycle and
-// SM), about 2800 of shared memory (Q, K and V read by the MMAs: 256 KB; tiles
-// dequantized: 100 KB; at 128 bytes a cycle).
+// SM), about 2300 of shared memory (operands read by the MMAs, dequantized
+// tiles written).
 //
 // Precision: d (n - 8) is rounded to fp16 (2^-12 on average), P to fp16 with
 // the row's largest at 2^8..2^15 (so that small ones stay normal numbers);
@@ -32,6 +30,8 @@
 // The order of a head's dimensions within the operands is the order in which
 // a cache row's words unpack (8 values a word); Q is stored in the same order,
 // and the output is written back through the inverse of V's.
+#include <algorithm>
+
 #include "attn.cuh"
 #include "pfng_tc.cuh"
 #include "pfng_tma.h"
@@ -44,15 +44,14 @@ constexpr int kRows = 2 * kTile;
 constexpr int kThreads = 512;
 constexpr int kDequantWarps = 6;
 constexpr int kGroups = kTile / kKvGroup;  // 16-key groups of a unit: the tasks of the dequantizing warps
-constexpr int kStep = 64;        // keys of an S buffer
-constexpr int kRawSlots = 3;
-constexpr int kOperands = 4;     // dequantized K or V tiles: unit 2 n is K of key tile n, unit 2 n + 1 its V
+constexpr int kRawSlots = 6;
+constexpr int kOperands = 3;     // dequantized K or V tiles: unit 2 n is K of key tile n, unit 2 n + 1 its V
 constexpr int kInfoSlots = 16;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNoMax = -3.0e38f;
 constexpr float kLift = 8.0f;    // log2 of P at a renewed maximum
 constexpr float kSlack = 7.0f;   // a score may pass the maximum by this before it is renewed
-constexpr uint32_t kTmemCols = 512;  // S_i at 128 i + 64 buffer (P over S), O_i at 256 + 128 i
+constexpr uint32_t kTmemCols = 512;  // S0 S1 (P over S) at 0 and 128, O0 O1 at 256 and 384
 
 // What the softmax needs to know about a key tile beyond its numbers.
 struct TileInfo {
@@ -69,14 +68,17 @@ struct Layout {
     static constexpr uint32_t kRawAt = kKV + kOperands * kOperand;  // [kRawSlots]
     static constexpr uint32_t kInfo = kRawAt + kRawSlots * kRaw;
     static constexpr uint32_t kBars = kInfo + ((kInfoSlots * sizeof(TileInfo) + 7) & ~7u);
-    static constexpr uint32_t kNumBars = 2 * kRawSlots + 2 * kOperands + 4 + 4 + 2 + 2;
+    static constexpr uint32_t kNumBars = 2 * kRawSlots + 2 * kOperands + 2 + 4 + 2 + 2;
     static constexpr uint32_t kBytes = kBars + 8 * kNumBars + 16 + 1024;
 };
 
 struct MmaParams {
     AttnArgs a;
-    int vec_q, vec_out;
-    int tiles;  // blocks of kRows per request and key head in the grid
+    int vec_q, vec_out;  // rows allow 16-byte accesses
+    int tiles;           // blocks of kRows per request and key head in the grid
+    int splits;          // pieces that the keys of a block are cut into
+    float *part_o;       // splits > 1: [block][split][kRows][dim] unnormalised outputs
+    float2 *part_ml;     // and [block][split][kRows] reference (log2) and sum
     int *err;
 };
 
@@ -159,6 +161,11 @@ PFNG_DEV void tmem_wait_ld(uint32_t *x) {
     }
 }
 PFNG_DEV void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+template <int N>
+PFNG_DEV void registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+PFNG_DEV void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
 PFNG_DEV float exp2_approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -277,6 +284,74 @@ PFNG_DEV float load_q(const MmaParams &mp, int64_t at, bool live, uint8_t *to, i
     return mul;
 }
 
+// The O rows of a warp, times f of each row, from TMEM to memory in format FMT.
+// Through shared memory (`mine`, 64 DIM bytes), so that a store covers whole
+// lines: rows of 16-byte pieces, piece x of row y at x ^ y.  `at`, `live`: where
+// this lane's row goes; zeros where there is no O (`have`).
+template <int DIM, int FMT>
+PFNG_DEV void write_rows(void *out, int64_t at, bool live, bool wide, float f, uint32_t o_at, bool have, uint8_t *mine) {
+    constexpr int kBlocks = DIM / 32, kSize = FMT == kOutF32 ? 4 : 2, kAtOnce = 64 / kSize, kPieces = DIM * kSize / 16;
+    const int lane = threadIdx.x & 31;
+    const uint32_t rows_live = __ballot_sync(0xffffffffu, live);
+#pragma unroll 1
+    for (int row1 = 0; row1 < 32; row1 += kAtOnce) {
+        const int y = lane - row1;
+        const bool staged = wide && y >= 0 && y < kAtOnce, direct = !wide && live && row1 == 0;
+#pragma unroll 1
+        for (int c = 0; c < DIM / 32; ++c) {
+            uint32_t o[32] = {};
+            if (have) {
+                tmem_ld32(o_at + 32 * c, o);
+                tmem_wait_ld<32>(o);
+            }
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int x = 0; x < (kBlocks == 4 ? 1 : 2); ++x) {
+                        // words of a V row: (g, pair of blocks); element (b & 1) + 2 e + 4 h of a word is
+                        // dimension 2 g + e + 16 h of block b
+                        float v[4];
+                        int dim;
+                        if constexpr (kBlocks == 4) {
+                            dim = 32 * b + 16 * h + 4 * c;
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                v[j] = __uint_as_float(o[(2 * (j >> 1) + (b >> 1)) * 8 + (b & 1) + 2 * (j & 1) + 4 * h]) * f;
+                        } else {
+                            dim = 32 * b + 16 * h + 8 * c + 4 * x;
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                v[j] = __uint_as_float(o[(2 * x + (j >> 1)) * 8 + b + 2 * (j & 1) + 4 * h]) * f;
+                        }
+                        if (staged) {
+                            const int piece = dim * kSize / 16, in_piece = dim * kSize % 16;
+                            store_values<4>(FMT, mine + (y * kPieces + (piece ^ (y % kPieces))) * 16 + in_piece, 0, v);
+                        }
+                        if (direct) {
+#pragma unroll 1
+                            for (int j = 0; j < 4; ++j) {
+                                const float one[1] = {j == 0 ? v[0] : j == 1 ? v[1] : j == 2 ? v[2] : v[3]};
+                                store_values<1>(FMT, out, at + dim + j, one);
+                            }
+                        }
+                    }
+        }
+        __syncwarp();
+        if (wide) {
+#pragma unroll 4
+            for (int idx = lane; idx < kAtOnce * kPieces; idx += 32) {
+                const int z = idx / kPieces, x = idx % kPieces;
+                const int64_t to = __shfl_sync(0xffffffffu, at, row1 + z) * kSize + 16 * x;
+                const uint4 piece = *reinterpret_cast<const uint4 *>(mine + (z * kPieces + (x ^ (z % kPieces))) * 16);
+                if ((rows_live >> (row1 + z)) & 1u) *reinterpret_cast<uint4 *>(static_cast<uint8_t *>(out) + to) = piece;
+            }
+        }
+        __syncwarp();
+    }
+}
+
 template <int DIM>
 __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams mp) {
     using L = Layout<DIM>;
@@ -286,7 +361,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::kBars);
     uint64_t *raw_full = bars, *raw_empty = raw_full + kRawSlots;
     uint64_t *op_full = raw_empty + kRawSlots, *op_empty = op_full + kOperands;
-    uint64_t *s_full = op_empty + kOperands, *p_full = s_full + 4, *o_full = p_full + 4;  // [row tile][buffer]; o_full: every O += P V
+    uint64_t *s_full = op_empty + kOperands, *p_full = s_full + 2, *o_full = p_full + 4;
     uint64_t *q_full = o_full + 2, *mma_done = q_full + 1;
     uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(bars + L::kNumBars);
     TileInfo *infos = reinterpret_cast<TileInfo *>(smem + L::kInfo);
@@ -295,10 +370,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
     const AttnArgs &p = mp.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     // the last row tiles see the most keys: they come first
-    const int tile = mp.tiles - 1 - static_cast<int>(blockIdx.x / (p.requests * p.heads_kv));
-    const int64_t rest = blockIdx.x % (p.requests * p.heads_kv);
-    const int64_t r = rest / p.heads_kv;
-    const int head_kv = static_cast<int>(rest % p.heads_kv);
+    const uint32_t per_tile = static_cast<uint32_t>(p.requests * p.heads_kv * mp.splits);
+    const int tile = mp.tiles - 1 - static_cast<int>(blockIdx.x / per_tile);
+    const uint32_t rest = blockIdx.x % per_tile;
+    const int split = static_cast<int>(rest % mp.splits), head_kv = static_cast<int>(rest / mp.splits % p.heads_kv);
+    const int64_t r = rest / (static_cast<uint32_t>(mp.splits) * p.heads_kv);
     const int group = p.group;
     int all;
     const int rows = attn_new_tokens(p, r, all) * group;
@@ -313,15 +389,19 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
         attn_visible(p, seq, all, (min(row0 + kRows, rows) - 1) / group, lo2, hi);
         first = max(lo, 0) / kTile;
         count = hi > first * kTile ? (hi + kTile - 1) / kTile - first : 0;
+        // this CTA's piece of them
+        const int begin = static_cast<int>(static_cast<int64_t>(count) * split / mp.splits);
+        count = static_cast<int>(static_cast<int64_t>(count) * (split + 1) / mp.splits) - begin;
+        first += begin;
     }
+    pdl_trigger();
 
     if (tid == 0) {
         abort_flag = 0;
         for (int i = 0; i < kRawSlots; ++i) mbar_init(&raw_full[i], 1), mbar_init(&raw_empty[i], kGroups);
         for (int i = 0; i < kOperands; ++i) mbar_init(&op_full[i], kGroups), mbar_init(&op_empty[i], 1);
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&o_full[i], 1);
-            mbar_init(&s_full[2 * i], 1), mbar_init(&s_full[2 * i + 1], 1);
+            mbar_init(&s_full[i], 1), mbar_init(&o_full[i], 1);
             mbar_init(&p_full[2 * i], 4), mbar_init(&p_full[2 * i + 1], 4);
 
         }
@@ -416,8 +496,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
         return true;
     };
 
+    // Registers: 512 threads x 128 at launch, 2 x 192 + 2 x 64 a thread of the
+    // four warpgroups after this.
     if (warp < 8) {
         // ---------------- softmax ----------------
+        registers_up<192>();
         const int i = warp >> 2;  // row tile
         const int in_tile = (warp & 3) * 32 + lane, row = row0 + i * kTile + in_tile;
         const bool live = row < rows;
@@ -453,34 +536,30 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
                         if (((info.bad[c >> 5] >> (c & 31)) & 1u) && key0 + c >= lo && key0 + c < hi)
                             l = __int_as_float(0x7fffffff);
             };
-            const int steps = count * (kTile / kStep);
-#pragma unroll 1
-            for (int u = 0; u < steps; ++u) {
-                const int n = u >> 1, buf = u & 1;
-                if (!wait_bar(&s_full[2 * i + buf], (u >> 1) & 1, &abort_flag, mp.err, kErrWaitFull)) {
+            for (int n = 0; n < count; ++n) {
+                if (!wait_bar(&s_full[i], n & 1, &abort_flag, mp.err, kErrWaitFull)) {
                     ok = false;
                     break;
                 }
                 tc_fence_after();
-                const uint32_t at = s_at + kStep * buf;
-                uint32_t s[kStep];
-                tmem_ld32(at, s);
-                tmem_ld32(at + 32, s + 32);
-                const uint32_t groups = (infos[n % kInfoSlots].groups >> (buf * (kStep / kKvGroup))) & 0xfu;
-                if (u > 0 && buf == 0) bad_keys(n - 1);  // this S came after O += P V of 64 keys before the last
-                const int from = lo - first * kTile - u * kStep, to = hi - first * kTile - u * kStep;
-                const bool masked = __any_sync(0xffffffffu, from > 0 || to < kStep) || groups != 0xfu;
-                tmem_wait_ld<kStep>(s);
+                const uint32_t groups = infos[n % kInfoSlots].groups;
+                if (n > 0) bad_keys(n - 1);  // V of the last tile is complete: this tile's MMA came after its own
+                const int from = lo - (first + n) * kTile, to = hi - (first + n) * kTile;
+                const bool masked = __any_sync(0xffffffffu, from > 0 || to < kTile) || groups != 0xffu;
+                uint32_t s[kTile];
+#pragma unroll
+                for (int c = 0; c < kTile; c += 32) tmem_ld32(s_at + c, s + c);
+                tmem_wait_ld<kTile>(s);
                 if (masked) {  // what a row does not see is -inf
 #pragma unroll
-                    for (int c = 0; c < kStep; ++c)
+                    for (int c = 0; c < kTile; ++c)
                         if (!(c >= from && c < to && ((groups >> (c / kKvGroup)) & 1u))) s[c] = 0xff800000u;
                 }
                 float tops[4];
 #pragma unroll
                 for (int x = 0; x < 4; ++x) tops[x] = -INFINITY;
 #pragma unroll
-                for (int x = 0; x < kStep; x += 8)
+                for (int x = 0; x < kTile; x += 8)
 #pragma unroll
                     for (int y = 0; y < 4; ++y)
                         tops[y] = fmaxf(fmaxf(tops[y], __uint_as_float(s[x + y])), __uint_as_float(s[x + y + 4]));
@@ -490,10 +569,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
                     const float f = exp2_approx(m - m_new);
                     m = m_new;
                     l *= f;
-                    if (u > 0) {  // O of the 64 keys before this has to be complete
-                        ok = wait_bar(&o_full[i], (u - 1) & 1, &abort_flag, mp.err, kErrWaitFull);
-                        if (!ok) break;
-                        tc_fence_after();
+                    if (n > 0) {
 #pragma unroll 1
                         for (int c = 0; c < DIM; c += 32) {
                             uint32_t o[32];
@@ -507,98 +583,51 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
                 }
                 float sum[4] = {};
 #pragma unroll
-                for (int x = 0; x < kStep; x += 2) {
-                    const float v = exp2_approx(fmaf(__uint_as_float(s[x]), mul, -m));
-                    const float w = exp2_approx(fmaf(__uint_as_float(s[x + 1]), mul, -m));
-                    sum[x & 2] += v;
-                    sum[(x & 2) + 1] += w;
-                    s[x / 2] = h2(__floats2half2_rn(v, w));
+                for (int h = 0; h < 2; ++h) {  // by halves of the keys: their part of O += P V can start
+#pragma unroll
+                    for (int x = 64 * h; x < 64 * h + 64; x += 2) {
+                        const float u = exp2_approx(fmaf(__uint_as_float(s[x]), mul, -m));
+                        const float w = exp2_approx(fmaf(__uint_as_float(s[x + 1]), mul, -m));
+                        sum[x & 2] += u;
+                        sum[(x & 2) + 1] += w;
+                        s[x / 2] = h2(__floats2half2_rn(u, w));
+                    }
+                    tmem_st32(s_at + 32 * h, s + 32 * h);  // P over S
+                    tmem_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&p_full[2 * i + h]);
                 }
-                tmem_st32(at, s);  // P over S
                 l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                tmem_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[2 * i + buf]);
             }
             if (ok && count > 0) {
-                ok = wait_bar(&o_full[i], (steps - 1) & 1, &abort_flag, mp.err, kErrWaitFull);
+                ok = wait_bar(&o_full[i], 0, &abort_flag, mp.err, kErrWaitFull);
                 if (ok) bad_keys(count - 1);
             }
             if (!ok) abort_flag = 1;
             tc_fence_after();
-            const bool none = l == 0.0f;
+            const bool none = l == 0.0f, have = count > 0;
             const float f = none ? 0.0f : 1.0f / l;
-            if (ok) {
+            // this row tile's Q is read by no MMA any more
+            uint8_t *mine = smem + L::kQ + i * L::kOperand + (warp & 3) * (L::kOperand / 4);
+            if (ok && mp.splits > 1) {
+                const int64_t slot = static_cast<int64_t>(blockIdx.x) * kRows + i * kTile + in_tile;
+                write_rows<DIM, kOutF32>(mp.part_o, slot * DIM, live, true, 1.0f, o_at, have, mine);
+                if (live) mp.part_ml[slot] = make_float2(m, l);
+            } else if (ok) {
                 const int64_t at = token * p.ldo + head * DIM;
-                // Through shared memory (this row tile's Q, which no MMA reads any more), so that a store covers
-                // whole lines: rows of DIM / 4 pieces of four values, piece x of row y at x ^ y.
-                const int size = p.out_format == kOutF32 ? 4 : 2, rows_at_once = 64 / size;
-                constexpr int kPieces = DIM / 4;
-                uint8_t *mine = smem + L::kQ + i * L::kOperand + (warp & 3) * (L::kOperand / 4);
-#pragma unroll 1
-                for (int row1 = 0; row1 < 32; row1 += rows_at_once) {
-                    const int y = lane - row1;
-                    const bool staged = mp.vec_out && y >= 0 && y < rows_at_once;
-#pragma unroll 1
-                    for (int c = 0; c < DIM / 32; ++c) {
-                        uint32_t o[32] = {};
-                        if (count > 0) {
-                            tmem_ld32(o_at + 32 * c, o);
-                            tmem_wait_ld<32>(o);
-                        }
-#pragma unroll
-                        for (int b = 0; b < kBlocks; ++b)
-#pragma unroll
-                            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                                for (int x = 0; x < (kBlocks == 4 ? 1 : 2); ++x) {
-                                    // words of a V row: (g, pair of blocks); element (b & 1) + 2 e + 4 h of a word is
-                                    // dimension 2 g + e + 16 h of block b
-                                    float v[4];
-                                    int dim;
-                                    if constexpr (kBlocks == 4) {
-                                        dim = 32 * b + 16 * h + 4 * c;
-#pragma unroll
-                                        for (int j = 0; j < 4; ++j)
-                                            v[j] = __uint_as_float(o[(2 * (j >> 1) + (b >> 1)) * 8 + (b & 1) + 2 * (j & 1) + 4 * h]) * f;
-                                    } else {
-                                        dim = 32 * b + 16 * h + 8 * c + 4 * x;
-#pragma unroll
-                                        for (int j = 0; j < 4; ++j)
-                                            v[j] = __uint_as_float(o[(2 * x + (j >> 1)) * 8 + b + 2 * (j & 1) + 4 * h]) * f;
-                                    }
-                                    if (staged) {
-                                        store_values<4>(p.out_format, mine, (y * kPieces + ((dim / 4) ^ (y % kPieces))) * 4, v);
-                                    } else if (!mp.vec_out && live && row1 == 0) {
-                                        for (int j = 0; j < 4; ++j) {
-                                            const float one[1] = {v[j]};
-                                            store_values<1>(p.out_format, p.out, at + dim + j, one);
-                                        }
-                                    }
-                                }
-                    }
-                    __syncwarp();
-                    if (mp.vec_out) {
-                        for (int idx = lane; idx < rows_at_once * kPieces; idx += 32) {
-                            const int z = idx / kPieces, x = idx % kPieces, from = (z * kPieces + (x ^ (z % kPieces))) * 4;
-                            const int64_t to = __shfl_sync(0xffffffffu, at, row1 + z) + 4 * x;
-                            if (!__shfl_sync(0xffffffffu, static_cast<int>(live), row1 + z)) continue;
-                            if (size == 4)
-                                *reinterpret_cast<uint4 *>(static_cast<float *>(p.out) + to) =
-                                    *reinterpret_cast<const uint4 *>(mine + from * 4);
-                            else
-                                *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + to) =
-                                    *reinterpret_cast<const uint2 *>(mine + from * 2);
-                        }
-                    }
-                    __syncwarp();
-                }
+                if (p.out_format == kOutF32)
+                    write_rows<DIM, kOutF32>(p.out, at, live, mp.vec_out, f, o_at, have, mine);
+                else if (p.out_format == kOutF16)
+                    write_rows<DIM, kOutF16>(p.out, at, live, mp.vec_out, f, o_at, have, mine);
+                else
+                    write_rows<DIM, kOutBF16>(p.out, at, live, mp.vec_out, f, o_at, have, mine);
                 if (live && p.lse)
                     p.lse[token * p.heads_q + head] = none ? -INFINITY : (m + log2f(l)) / kLog2e;
             }
         }
     } else {
+        registers_down<64>();
         if (warp == 12) {
             // ---------------- MMA issue ----------------
             const uint32_t leader = elect_leader();
@@ -606,19 +635,18 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
             // little more than wait.  Descriptors differ by their address
             // field, in the low word, only.  (A thread per row tile measured
             // 13 % slower: MMAs of two accumulators then alternate.)
-            constexpr uint32_t kIdescS = idesc_f16(kStep, false), kIdescO = idesc_f16(DIM, true);
+            constexpr uint32_t kIdescS = idesc_f16(kTile, false), kIdescO = idesc_f16(DIM, true);
             constexpr uint32_t kHalf = (kTile * 128) >> 4, kBuf = L::kOperand >> 4;
             const uint64_t q_desc = sw128_desc(base + L::kQ);
             const uint64_t k_desc = sw128_desc(base + L::kKV), v_desc0 = v_desc(base + L::kKV);
             bool ok = count > 0;
-            // S of row tile i for half h of the key tile in operand buffer `op`
-            const auto scores = [&](int i, int h, uint32_t op) {
-                const uint64_t q = q_desc + i * kBuf, k = k_desc + op * kBuf + h * ((kStep * 128) >> 4);
+            const auto scores = [&](int i, uint32_t buf) {  // S_i = Q_i K^T
+                const uint64_t q = q_desc + i * kBuf, k = k_desc + buf * kBuf;
 #pragma unroll
                 for (int x = 0; x < DIM / 16; ++x)
-                    umma_f16_ss(leader, tmem + i * kTile + h * kStep, q + (x >> 2) * kHalf + (x & 3) * 2,
-                                k + (x >> 2) * kHalf + (x & 3) * 2, kIdescS, x > 0);
-                umma_commit_by(leader, &s_full[2 * i + h]);
+                    umma_f16_ss(leader, tmem + i * kTile, q + (x >> 2) * kHalf + (x & 3) * 2, k + (x >> 2) * kHalf + (x & 3) * 2,
+                                kIdescS, x > 0);
+                umma_commit_by(leader, &s_full[i]);
             };
             const auto ready = [&](uint64_t *bar, uint32_t parity) {
                 return __all_sync(0xffffffffu, mbar_test_wait(bar, parity) ||
@@ -627,9 +655,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
             if (ok) ok = ready(q_full, 0) && ready(&op_full[0], 0);
             if (ok) {
                 tc_fence_after();
-#pragma unroll 1
-                for (int h = 0; h < 2; ++h)
-                    for (int i = 0; i < row_tiles; ++i) scores(i, h, 0);
+                scores(0, 0);
+                if (row_tiles > 1) scores(1, 0);
                 umma_commit_by(leader, &op_empty[0]);
             }
             uint32_t vb = 1, v_phase = 0;  // buffer of V(n); K(n + 1) is in the one after it
@@ -637,28 +664,31 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
             for (int n = 0; n < count && ok; ++n) {
                 const uint32_t kb = vb + 1 == kOperands ? 0 : vb + 1, k_phase = vb + 1 == kOperands ? v_phase ^ 1 : v_phase;
                 const bool more = n + 1 < count;
+                const uint64_t v = v_desc0 + vb * kBuf;
+                ok = ready(&op_full[vb], v_phase);
 #pragma unroll 1
-                for (int h = 0; h < 2 && ok; ++h) {
-                    const uint64_t v = v_desc0 + vb * kBuf + h * ((kStep * 128) >> 4);
-                    if (h == 0) ok = ready(&op_full[vb], v_phase);
-#pragma unroll 1
-                    for (int i = 0; i < row_tiles && ok; ++i) {
-                        ok = ready(&p_full[2 * i + h], n & 1);
-                        if (!ok) break;
-                        tc_fence_after();
+                for (int i = 0; i < row_tiles && ok; ++i) {
 #pragma unroll
-                        for (int x = 0; x < kStep / 16; ++x)  // O_i += P_i V
-                            umma_f16_ts(leader, tmem + 256 + i * kTile, tmem + i * kTile + h * kStep + 8 * x,
-                                        v + x * (2048 >> 4), kIdescO, n > 0 || h > 0 || x > 0);
-                        umma_commit_by(leader, &o_full[i]);
-                        if (!more) continue;
-                        if (h == 0 && i == 0) ok = ready(&op_full[kb], k_phase);
-                        if (ok) scores(i, h, kb);
+                    for (int h = 0; h < 2 && ok; ++h) {  // O_i += P_i V, by halves of the keys
+                        ok = ready(&p_full[2 * i + h], n & 1);
+                        tc_fence_after();
+                        if (!ok) break;
+#pragma unroll
+                        for (int x = 4 * h; x < 4 * h + 4; ++x)
+                            umma_f16_ts(leader, tmem + 256 + i * kTile, tmem + i * kTile + 8 * x, v + x * (2048 >> 4), kIdescO,
+                                        n > 0 || x > 0);
                     }
+                    if (!ok) break;
+                    if (i == row_tiles - 1) umma_commit_by(leader, &op_empty[vb]);
+                    if (!more) {
+                        umma_commit_by(leader, &o_full[i]);
+                        continue;
+                    }
+                    if (i == 0) ok = ready(&op_full[kb], k_phase);
+                    if (!ok) break;
+                    scores(i, kb);
+                    if (i == row_tiles - 1) umma_commit_by(leader, &op_empty[kb]);
                 }
-                if (!ok) break;
-                umma_commit_by(leader, &op_empty[vb]);
-                if (more) umma_commit_by(leader, &op_empty[kb]);
                 vb = kb + 1 == kOperands ? 0 : kb + 1;
                 v_phase = kb + 1 == kOperands ? k_phase ^ 1 : k_phase;
             }
@@ -726,35 +756,112 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
     }
 }
 
+// Joins the pieces of a block of rows: weights 2^(m_i - max m), pieces in order;
+// a warp per row.
+constexpr int kJoinWarps = 8;
 template <int DIM>
-cudaError_t launch(const MmaParams &mp, int64_t grid, cudaStream_t s) {
-    const cudaError_t e = cudaFuncSetAttribute(attn_mma_kernel<DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               static_cast<int>(Layout<DIM>::kBytes));
-    if (e != cudaSuccess) return e;
-    attn_mma_kernel<DIM><<<static_cast<unsigned>(grid), kThreads, Layout<DIM>::kBytes, s>>>(mp);
-    return cudaGetLastError();
+__global__ void __launch_bounds__(32 * kJoinWarps) attn_mma_join_kernel(const MmaParams mp) {
+    const AttnArgs &p = mp.a;
+    const int lane = threadIdx.x & 31;
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * kJoinWarps + (threadIdx.x >> 5);
+    const int64_t block = at / kRows;  // (tile, request, key head), as in the grid
+    const int in_block = static_cast<int>(at % kRows);
+    const int64_t per_tile = p.requests * p.heads_kv;
+    const int tile = mp.tiles - 1 - static_cast<int>(block / per_tile);
+    const int64_t r = block % per_tile / p.heads_kv;
+    const int head_kv = static_cast<int>(block % p.heads_kv);
+    int all;
+    const int rows = attn_new_tokens(p, r, all) * p.group, row = tile * kRows + in_block;
+    pdl_wait();
+    if (tile < 0 || row >= rows) return;
+    const int64_t slot0 = block * mp.splits * kRows + in_block;
+    float m = kNoMax;
+    for (int s = lane; s < mp.splits; s += 32) m = fmaxf(m, mp.part_ml[slot0 + static_cast<int64_t>(s) * kRows].x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    float l = 0.0f, acc[DIM / 32] = {};
+#pragma unroll 4
+    for (int s = 0; s < mp.splits; ++s) {
+        const int64_t slot = slot0 + static_cast<int64_t>(s) * kRows;
+        const float2 ml = mp.part_ml[slot];
+        const float f = exp2_approx(ml.x - m);
+        l += ml.y * f;
+#pragma unroll
+        for (int x = 0; x < DIM / 32; ++x) acc[x] += f * mp.part_o[slot * DIM + lane + 32 * x];
+    }
+    const bool none = l == 0.0f;
+    const float f = none ? 0.0f : 1.0f / l;
+    const int64_t token = p.cu_q[r] + row / p.group, head = static_cast<int64_t>(head_kv) * p.group + row % p.group;
+#pragma unroll
+    for (int x = 0; x < DIM / 32; ++x) {
+        const float v[1] = {acc[x] * f};
+        store_values<1>(p.out_format, p.out, token * p.ldo + head * DIM + lane + 32 * x, v);
+    }
+    if (p.lse && lane == 0) p.lse[token * p.heads_q + head] = none ? -INFINITY : (m + log2f(l)) / kLog2e;
 }
 
 int64_t row_blocks(const AttnArgs &p) { return (p.max_q * p.group + kRows - 1) / kRows; }
+int64_t blocks_of(const AttnArgs &p) { return row_blocks(p) * p.requests * p.heads_kv; }
+// Pieces per block of rows, none shorter than kMinTiles key tiles.  Few blocks:
+// as many pieces as make one wave of CTAs (10 blocks over 16000 keys: 55 us with
+// 14 pieces, 74 with 29, a second wave that is not full).  Where no two pieces
+// per block fit one wave, three waves even out ragged lengths (96 blocks over
+// 1000..4000 keys: 86 us with 1 piece, 65 with 3, 60 with 4); from three waves
+// of blocks on there is nothing to cut.
+constexpr int kMinTiles = 4;
+int splits_of(const AttnArgs &p) {
+    const int64_t sms = device_sm_count(), blocks = blocks_of(p);
+    const int64_t want = sms / blocks >= 2 ? sms / blocks : 3 * sms / blocks;
+    const int64_t most = (p.max_kv + kTile - 1) / kTile / kMinTiles;
+    return static_cast<int>(std::max<int64_t>(1, std::min(want, most)));
+}
+
+template <int DIM>
+cudaError_t launch(const MmaParams &mp, cudaStream_t s) {
+    cudaError_t e = cudaFuncSetAttribute(attn_mma_kernel<DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         static_cast<int>(Layout<DIM>::kBytes));
+    if (e != cudaSuccess) return e;
+    const int64_t blocks = blocks_of(mp.a);
+    attn_mma_kernel<DIM><<<static_cast<unsigned>(blocks * mp.splits), kThreads, Layout<DIM>::kBytes, s>>>(mp);
+    if ((e = cudaGetLastError()) != cudaSuccess || mp.splits == 1) return e;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(blocks * (kRows / kJoinWarps)));
+    cfg.blockDim = dim3(32 * kJoinWarps);
+    cfg.stream = s;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, attn_mma_join_kernel<DIM>, mp);
+}
 
 }  // namespace
 
 bool attn_mma_supported(const AttnArgs &p) {
-    return (p.head_dim == 64 || p.head_dim == 128) && row_blocks(p) * p.requests * p.heads_kv < 0x7fffffff;
+    return (p.head_dim == 64 || p.head_dim == 128) && blocks_of(p) * (kRows / kJoinWarps) < 0x7fffffff;
 }
 
-cudaError_t launch_attn_mma(const AttnArgs &p, int *err, cudaStream_t s) {
+size_t attn_mma_workspace(const AttnArgs &p) {
+    const int splits = splits_of(p);
+    if (splits == 1) return 0;
+    return static_cast<size_t>(blocks_of(p)) * splits * kRows * (p.head_dim + 2) * sizeof(float) + 256;
+}
+
+cudaError_t launch_attn_mma(const AttnArgs &p, void *workspace, int *err, cudaStream_t s) {
     MmaParams mp{};
     mp.a = p;
     const auto wide = [](const void *x, int64_t ld, int fmt) {
-        return ld % 4 == 0 && reinterpret_cast<uintptr_t>(x) % (fmt == kOutF32 ? 16 : 8) == 0;
+        return ld % (fmt == kOutF32 ? 4 : 8) == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
     };
-    mp.vec_q = p.ldq % 8 == 0 && reinterpret_cast<uintptr_t>(p.q) % 16 == 0;
+    mp.vec_q = wide(p.q, p.ldq, p.q_format);
     mp.vec_out = wide(p.out, p.ldo, p.out_format);
     mp.tiles = static_cast<int>(row_blocks(p));
+    mp.splits = splits_of(p);
+    mp.part_o = static_cast<float *>(workspace);
+    mp.part_ml = reinterpret_cast<float2 *>(mp.part_o + blocks_of(p) * mp.splits * kRows * p.head_dim);
     mp.err = err;
-    const int64_t grid = row_blocks(p) * p.requests * p.heads_kv;
-    return p.head_dim == 128 ? launch<128>(mp, grid, s) : launch<64>(mp, grid, s);
+    return p.head_dim == 128 ? launch<128>(mp, s) : launch<64>(mp, s);
 }
 
 }  // namespace pfng

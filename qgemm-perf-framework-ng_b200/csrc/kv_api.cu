@@ -35,8 +35,14 @@ int check_attention(int64_t requests, int64_t tokens, int64_t heads_q, int64_t h
 int resolve_attention(const AttnArgs &a, int path) {
     const bool stream = attn_stream_supported(a), mma = attn_mma_supported(a);
     if (path == PFNG_B200_PATH_AUTO) {
-        // up to 16 query rows per key head are one tile of the streaming kernel
-        const bool few = a.max_q * a.group <= 16;
+        // Query rows per key head.  Up to 16 are one row tile of the streaming
+        // kernel.  Up to 32 (two tiles, each reading the cache) it still wins
+        // unless there are so few (request, key head) pairs that the MMA
+        // kernel can cut the keys of each into four pieces and more: 32 rows,
+        // 8 x 8 pairs, 16000 keys 131 us against 200; 1 x 8 pairs, 8000 keys
+        // 51 against 33.  With 64 rows the MMA kernel wins (232 against 200).
+        const int64_t rows = a.max_q * a.group, pairs = a.requests * a.heads_kv;
+        const bool few = rows <= 16 || (rows <= 32 && 4 * pairs > device_sm_count());
         if (few && stream) return PFNG_B200_PATH_GEMV;
         return mma ? PFNG_B200_PATH_MMA : PFNG_B200_PATH_SIMPLE;
     }
@@ -46,7 +52,9 @@ int resolve_attention(const AttnArgs &a, int path) {
 }
 
 size_t attention_workspace(const AttnArgs &a, int resolved) {
-    return resolved == PFNG_B200_PATH_GEMV ? attn_stream_workspace(a) : 0;
+    return resolved == PFNG_B200_PATH_GEMV  ? attn_stream_workspace(a)
+           : resolved == PFNG_B200_PATH_MMA ? attn_mma_workspace(a)
+                                            : 0;
 }
 
 }  // namespace
@@ -192,7 +200,7 @@ int pfng_b200_attention_q4_0(const void *q, int64_t ldq, int q_format, const voi
     if (need > 0 && !aligned(workspace, 256)) return PFNG_B200_ERR_ALIGNMENT;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (resolved == PFNG_B200_PATH_GEMV) return status_of(launch_attn_stream(a, workspace, device_error_word(), s));
-    if (resolved == PFNG_B200_PATH_MMA) return status_of(launch_attn_mma(a, device_error_word(), s));
+    if (resolved == PFNG_B200_PATH_MMA) return status_of(launch_attn_mma(a, workspace, device_error_word(), s));
     return status_of(launch_attn_simple(a, s));
 }
 

@@ -193,7 +193,8 @@ bool attn_stream_supported(const AttnArgs &args);
 size_t attn_stream_workspace(const AttnArgs &args);
 // attn_mma.cu -- many query rows per key head
 bool attn_mma_supported(const AttnArgs &args);
-cudaError_t launch_attn_mma(const AttnArgs &args, int *err, cudaStream_t s);
+size_t attn_mma_workspace(const AttnArgs &args);
+cudaError_t launch_attn_mma(const AttnArgs &args, void *workspace, int *err, cudaStream_t s);
 cudaError_t launch_attn_stream(const AttnArgs &args, void *workspace, int *err, cudaStream_t s);
 
 // shard.cu
