@@ -1,0 +1,106 @@
+"""The attention half of a decoder layer on quantized weights and a quantized cache: a prompt step, then decode steps.
+
+    python examples/quantized_attention.py [--steps 4] [--requests 3] [--hidden 1024] [--heads 8] [--kv-heads 2]
+
+Per step: kv_plan once; then, for the layer, the Q/K/V projection (q4_0 weights), qk_norm_rope, kv_append_q4_0 into the
+pages that the plan gave, attention_q4_0 over them, and the output projection.  Synthetic weights and activations.  The
+last step's attention is compared with a plain one in 64 bits over the values that the cache holds.
+"""
+import argparse
+import pathlib
+import sys
+
+ROOT = pathlib.Path(__file__).resolve().parent.parent
+sys.path.insert(0, str(ROOT / "qgemm-perf-framework-ng_b200"))
+import torch  # noqa: E402
+
+import pfng_b200 as pb  # noqa: E402
+
+
+class Layer:
+    """Weights of one attention layer, and its q4_0 cache."""
+
+    def __init__(self, hidden, heads, kv_heads, dim, pages, page_size, seed=0):
+        g = torch.Generator("cuda").manual_seed(seed)
+        self.heads, self.kv_heads, self.dim, self.page_size = heads, kv_heads, dim, page_size
+        self.rows = (heads + 2 * kv_heads) * dim
+        scale = hidden ** -0.5
+        self.w_qkv = pb.quantize_q4_0(torch.randn(self.rows, hidden, generator=g, device="cuda") * scale)
+        self.w_out = pb.quantize_q4_0(torch.randn(hidden, heads * dim, generator=g, device="cuda") * scale)
+        self.q_norm = 1 + 0.1 * torch.randn(dim, generator=g, device="cuda")
+        self.k_norm = 1 + 0.1 * torch.randn(dim, generator=g, device="cuda")
+        size = pb.kv_cache_bytes(pages, page_size, kv_heads, dim)
+        self.k_cache = torch.zeros(size, dtype=torch.uint8, device="cuda")
+        self.v_cache = torch.zeros(size, dtype=torch.uint8, device="cuda")
+
+    def step(self, x, plan, table, cos_sin, max_q, max_kv):
+        """Activations x [tokens][hidden] (fp32) -> (output projection [tokens][hidden], q, attention output)."""
+        hidden = x.shape[1]
+        qkv = pb.compute("q4_0", self.w_qkv, x, self.rows)
+        q, k = pb.qk_norm_rope(qkv, plan.positions, cos_sin, self.heads, self.kv_heads, self.dim, q_weight=self.q_norm,
+                               k_weight=self.k_norm)
+        v = qkv[:, (self.heads + self.kv_heads) * self.dim:]
+        pb.kv_append_q4_0(k, v, plan.slots, self.k_cache, self.v_cache, self.kv_heads, self.dim, self.page_size)
+        a = pb.attention_q4_0(q, self.k_cache, self.v_cache, table, plan.seq_len, plan.cu_q, self.heads, self.kv_heads,
+                              self.dim, self.page_size, max_q=max_q, max_kv=max_kv, out_format="f32")
+        return pb.compute("q4_0", self.w_out, a, hidden), q, a
+
+
+def rope_table(max_pos, dim):
+    inv = 10000.0 ** (-torch.arange(0, dim, 2, dtype=torch.float64) / dim)
+    angle = torch.arange(max_pos, dtype=torch.float64)[:, None] * inv
+    return torch.cat([angle.cos(), angle.sin()], 1).float().cuda()
+
+
+def run(steps=4, requests=3, hidden=1024, heads=8, kv_heads=2, dim=128, page_size=16, max_len=512, seed=0):
+    """Runs a prompt step and `steps` decode steps; returns what a check of the last one needs."""
+    pages = requests * (max_len // page_size) + 1
+    layer = Layer(hidden, heads, kv_heads, dim, pages, page_size, seed)
+    g = torch.Generator("cuda").manual_seed(seed + 1)
+    table = torch.full((requests, max_len // page_size), -1, dtype=torch.int32, device="cuda")
+    free = torch.randperm(pages, device="cuda").to(torch.int32)
+    cos_sin = rope_table(max_len, dim)
+    kv_len = torch.zeros(requests, dtype=torch.int32, device="cuda")
+    lengths, taken = [37 + 50 * r for r in range(requests)], 0  # what the scheduler knows on the host
+    for step in range(steps + 1):
+        new = lengths if step == 0 else [1] * requests
+        held = [n + step for n in lengths]
+        q_len = torch.tensor(new, dtype=torch.int32, device="cuda")
+        plan = pb.kv_plan(kv_len, q_len, table, free[taken:], page_size, sum(new))
+        x = torch.randn(sum(new), hidden, generator=g, device="cuda")
+        out, q, a = layer.step(x, plan, table, cos_sin, max_q=max(new), max_kv=max(held))
+        taken = sum(-(-n // page_size) for n in held)
+        kv_len = plan.seq_len
+    return layer, table, held, q, a, out
+
+
+def check(layer, table, held, q, a):
+    """Largest difference of the last step's attention from the plain one, and the largest value."""
+    sys.path.insert(0, str(ROOT / "tests"))
+    import kv_plain
+    pages = pb._cache_pages(layer.k_cache, layer.page_size, layer.kv_heads, layer.dim)
+    k = kv_plain.values(layer.k_cache, pages, layer.page_size, layer.kv_heads, layer.dim, True)
+    v = kv_plain.values(layer.v_cache, pages, layer.page_size, layer.kv_heads, layer.dim, False)
+    shape = (len(held), layer.heads, layer.dim)
+    want = kv_plain.attention(q.cpu().double().reshape(shape), k, v, table.tolist(), held, list(range(len(held) + 1)),
+                              layer.page_size, layer.dim ** -0.5, True, 0)[0]
+    return float((a.cpu().double().reshape(shape) - want).abs().max()), float(want.abs().max())
+
+
+def main():
+    ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
+    ap.add_argument("--steps", type=int, default=4)
+    ap.add_argument("--requests", type=int, default=3)
+    ap.add_argument("--hidden", type=int, default=1024)
+    ap.add_argument("--heads", type=int, default=8)
+    ap.add_argument("--kv-heads", type=int, default=2)
+    args = ap.parse_args()
+    layer, table, held, q, a, out = run(args.steps, args.requests, args.hidden, args.heads, args.kv_heads)
+    pb.check_kernel_error()
+    off, size = check(layer, table, held, q, a)
+    print(f"{args.steps} decode steps after a prompt step, lengths {held}: attention differs by {off:.2e} at most "
+          f"(values up to {size:.2f}); output {tuple(out.shape)}")
+
+
+if __name__ == "__main__":
+    main()

@@ -458,16 +458,18 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
             for (int i = 0; i < kPieces; ++i) {
                 const int row = g * kKvGroup + (i * 32 + lane) / kQuads, u = lane % kQuads;
                 uint32_t s[4];
+                // scales that are not finite: of V 0 and the key marked, as 0 * inf would reach the rows that do
+                // not see it; of K NaN, which is masked with the score
+                bool bad = false;
+#pragma unroll
+                for (int b = 0; b < kBlocks / 2; ++b)
+                    bad |= (scales[i][b] & 0x7c00u) == 0x7c00u || (scales[i][b] & 0x7c000000u) == 0x7c000000u;
+                if (bad) {
+#pragma unroll
+                    for (int b = 0; b < kBlocks / 2; ++b) scales[i][b] = is_v ? 0u : 0x7fff7fffu;
+                    if (is_v && u == 0) atomicOr(&info.bad[row >> 5], 1u << (row & 31));
+                }
                 if (is_v) {
-                    bool bad = false;
-#pragma unroll
-                    for (int b = 0; b < kBlocks / 2; ++b)
-                        bad |= (scales[i][b] & 0x7c00u) == 0x7c00u || (scales[i][b] & 0x7c000000u) == 0x7c000000u;
-                    if (bad) {
-#pragma unroll
-                        for (int b = 0; b < kBlocks / 2; ++b) scales[i][b] = 0;
-                        if (u == 0) atomicOr(&info.bad[row >> 5], 1u << (row & 31));
-                    }
 #pragma unroll
                     for (int x = 0; x < 4; ++x) s[x] = scales[i][kBlocks == 4 ? (x & 1) : 0];
                 } else {

@@ -68,7 +68,9 @@ __global__ void __launch_bounds__(kWarps * 32) attn_simple_kernel(const AttnArgs
                                static_cast<float>(static_cast<int>((w >> (8 * e + 4)) & 15u) - 8);
                     }
                 }
-                s += f16_bits_to_f32(scales[blk]) * sum;
+                // a scale that is not finite makes its values NaN, whatever their sum
+                const float d = f16_bits_to_f32(scales[blk]);
+                s += (d - d == 0.0f ? d : __int_as_float(0x7fffffff)) * sum;
             }
             s *= p.scale;
         }

@@ -108,6 +108,15 @@ PFNG_DEV uint32_t larger(uint32_t x, uint32_t y) {
     asm("max.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(z) : "r"(x), "r"(y));
     return z;
 }
+// x with the halves that are not finite (infinities, NaN) as 0.
+PFNG_DEV uint32_t finite_halves(uint32_t x) {
+    uint32_t mask;
+    asm("{\n\t.reg .b32 a;\n\tand.b32 a, %1, 0x7fff7fff;\n\tset.lt.u32.f16x2 %0, a, %2;\n\t}"
+        : "=r"(mask)
+        : "r"(x), "r"(0x7c007c00u));
+    return x & mask;
+}
+PFNG_DEV bool all_finite(uint32_t x) { return (x & 0x7c00u) != 0x7c00u && (x & 0x7c000000u) != 0x7c000000u; }
 PFNG_DEV uint32_t h2(__half2 x) { return *reinterpret_cast<uint32_t *>(&x); }
 PFNG_DEV __half2 as_h2(uint32_t x) { return *reinterpret_cast<__half2 *>(&x); }
 // fp16 halves of a register as fp32.  As a mixed-precision add, which runs at
@@ -547,25 +556,31 @@ PFNG_DEV void attend(const RowTile<DIM, NT> &t, const WarpState<DIM, NT> &w, Row
             }
 
     // ---- maximum, renewed when a score or a scale passes its limit ----
-    // V scales of the groups, in words of two: read once, kWords / 32 a lane
+    // Scales of the groups, in words of two: read once, kWords / 32 a lane.  The
+    // limit follows the finite ones of V; a scale of K that is not finite makes
+    // the scores of its key NaN.
     float d_top;
+    bool k_finite = true;
     {
         constexpr int kGroupWords = kKvGroup * kScaleRow / 4, kWords = kGroups * kGroupWords;
         uint32_t d2 = 0;
 #pragma unroll
         for (int i = 0; i < (kWords + 31) / 32; ++i) {
             const int at = (i * 32 + lane) % kWords, j = at / kGroupWords, in_group = at % kGroupWords;
-            uint32_t x = lds32(vg + kScales + j * kGroup + 4 * in_group);
+            const uint32_t off = kScales + j * kGroup + 4 * in_group;
+            uint32_t x = lds32(vg + off);
             if constexpr (MASKED) {  // a key that no row sees may be anything: its scales are not looked at
                 const int key = key0 + j * kKvGroup + 4 * in_group / kScaleRow;
                 if (!(key >= t.lo_min && key < t.hi_max)) x = 0;
             }
+            x = finite_halves(x);
             d2 = i == 0 ? x : larger(d2, x);
+            k_finite &= all_finite(lds32(kg + off));
         }
         d_top = fmaxf(fabsf(low_half(d2)), fabsf(high_half(d2)));
     }
     float tops[NT][2];
-    bool past = d_top > s.d_limit;
+    bool past = d_top > s.d_limit || !k_finite;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -577,11 +592,30 @@ PFNG_DEV void attend(const RowTile<DIM, NT> &t, const WarpState<DIM, NT> &w, Row
             past |= top > s.m[n][x] + s.limit;
         }
     if (__any_sync(0xffffffffu, past)) {
+#pragma unroll 1
+        for (int j = 0; !__all_sync(0xffffffffu, k_finite) && j < kGroups; ++j)
+#pragma unroll
+            for (int b = 0; b < kBlocks / 2; ++b) {
+                const uint32_t at = kg + kScales + j * kGroup + 4 * b;
+                const bool a_bad = !all_finite(lds32(at + ka * kScaleRow)), b_bad = !all_finite(lds32(at + kb * kScaleRow));
+#pragma unroll
+                for (int jj = 0; jj < kGroups; ++jj)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int key = key0 + j * kKvGroup + (i < 2 ? ka : kb), row = n * 8 + 2 * q4 + (i & 1);
+                            const bool seen = !MASKED || (key >= w.lo[row] && key < w.hi[row]);
+                            if (jj == j && seen && (i < 2 ? a_bad : b_bad)) sc[jj][n][i] = __int_as_float(0x7fffffff);
+                        }
+            }
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) d_top = fmaxf(d_top, __shfl_xor_sync(0xffffffffu, d_top, o));
-        float up = s.limit - kSlack;  // log2 of the power of two that P carries
-        if (d_top > s.d_limit) {
-            const int e = d_top < INFINITY ? exponent_of(d_top) + 1 : 16;  // |d| <= 2^e
+        const float limit = s.limit;
+        float up = limit - kSlack;  // log2 of the power of two that P carries
+        const bool larger_d = d_top > s.d_limit;
+        if (larger_d) {
+            const int e = exponent_of(d_top) + 1;  // |d| <= 2^e
             s.d_limit = power_of_two(e);
             up = static_cast<float>(8 - e);
             s.limit = up + kSlack;
@@ -594,7 +628,8 @@ PFNG_DEV void attend(const RowTile<DIM, NT> &t, const WarpState<DIM, NT> &w, Row
                 float top = tops[n][x];
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                top = fmaxf(top - up, s.m[n][x]);
+                // a row within its limit stays as it is, whatever the other rows do
+                top = larger_d || top > s.m[n][x] + limit ? fmaxf(top - up, s.m[n][x]) : s.m[n][x];
                 f[x] = exp2_approx(s.m[n][x] - top);
                 s.m[n][x] = top;
                 s.l[n][x] *= f[x];

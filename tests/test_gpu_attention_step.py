@@ -350,6 +350,107 @@ def test_attention_on_another_stream():
     assert torch.equal(want, got)
 
 
+@pytest.mark.parametrize("path", PATHS)
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_attention_scales_that_are_not_finite(path, bad, which):
+    """A key with such a scale changes the rows that see it, and no other."""
+    c = Case([200, 70], [180, 1], 4, 2, 128, 16)
+    window, key = 60, 90
+    want = c.run("f32", path, window=window)[0]
+    raw = c.caches[which].cpu()
+    n, d = kv_plain.unpack(raw, c.pages, c.page, c.hk, c.dim, which == "k")
+    d[c.table[0][key // c.page], :, key % c.page] = bad
+    c.caches[which] = kv_plain.pack(n, d, which == "k").cuda()
+    got = c.run("f32", path, window=window)[0]
+    pos = torch.arange(180) + 20
+    sees = torch.cat([(pos >= key) & (pos - key < window), torch.zeros(1, dtype=torch.bool)])
+    assert torch.equal(got[~sees], want[~sees])
+    heads = got[sees].reshape(-1, c.hq, c.dim)
+    assert bool((~heads.isfinite()).any(-1).all())
+
+
+@pytest.mark.parametrize("path", PATHS)
+def test_attention_output_rows_apart(path):
+    """An output with a row stride of its own, aligned and not; what lies between the rows stays."""
+    c = Case([150, 40], [30, 2], 4, 2, 64, 16)
+    want = c.run(path=path)[0]
+    for pad, offset in ((64, 0), (3, 0), (5, 1)):
+        width = c.hq * c.dim + pad
+        flat = torch.full((c.q.shape[0] * width + offset,), 5.0, dtype=torch.bfloat16, device="cuda")
+        rows = flat[offset:].reshape(-1, width)
+        pb.attention_q4_0(c.q.cuda(), c.caches["k"], c.caches["v"], torch.tensor(c.table, dtype=torch.int32).cuda(),
+                          torch.tensor(c.seq, dtype=torch.int32).cuda(), torch.tensor(c.cu, dtype=torch.int32).cuda(),
+                          c.hq, c.hk, c.dim, c.page, max_q=30, max_kv=150, out=rows[:, :c.hq * c.dim], path=path)
+        assert torch.equal(rows[:, :c.hq * c.dim].cpu(), want) and bool((rows[:, c.hq * c.dim:] == 5).all())
+
+
+@pytest.mark.parametrize("path,q_len", [("gemv", 1), ("mma", 40), ("simple", 2)])
+def test_cache_past_32_bits(path, q_len):
+    """Pages whose bytes lie past 4 GB: the same bits as on the first pages."""
+    heads, dim, page, n = 8, 128, 64, 150
+    per_page = pb.kv_cache_bytes(1, page, heads, dim)
+    pages = (1 << 32) // per_page + 40
+    g = torch.Generator("cuda").manual_seed(1)
+    k = torch.randn(n, heads * dim, generator=g, device="cuda").bfloat16()
+    v = torch.randn(n, heads * dim, generator=g, device="cuda")
+    q = torch.randn(q_len, 2 * heads * dim, generator=g, device="cuda").bfloat16()
+    outs = []
+    for count, ids in ((3, [2, 0, 1]), (pages, [pages - 1, pages - 30, pages - 2])):
+        caches = [torch.empty(count * per_page, dtype=torch.uint8, device="cuda") for _ in range(2)]
+        table = torch.tensor([ids], dtype=torch.int32, device="cuda")
+        slots = torch.tensor([ids[j // page] * page + j % page for j in range(n)], device="cuda")
+        pb.kv_append_q4_0(k, v, slots, *caches, heads, dim, page)
+        outs.append(pb.attention_q4_0(q, *caches, table, torch.tensor([n], dtype=torch.int32, device="cuda"),
+                                      torch.tensor([0, q_len], dtype=torch.int32, device="cuda"), 2 * heads, heads, dim,
+                                      page, max_q=q_len, max_kv=n, path=path))
+    assert torch.equal(outs[0], outs[1]) and bool(outs[0].isfinite().all())
+
+
+def test_step_in_a_graph():
+    """Plan, rotation, append and attention captured once and replayed on new values."""
+    c = Case([100, 33, 260], [1, 1, 1], 8, 2, 128, 16)
+    table = torch.tensor(c.table, dtype=torch.int32).cuda()
+    seq = torch.tensor(c.seq, dtype=torch.int32).cuda()
+    cu = torch.tensor(c.cu, dtype=torch.int32).cuda()
+    q = c.q.cuda()
+    call = lambda: pb.attention_q4_0(q, c.caches["k"], c.caches["v"], table, seq, cu, 8, 2, 128, 16, max_q=1, max_kv=260)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        call()
+        s.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            out = call()
+    q.mul_(-1.5)
+    graph.replay()
+    torch.cuda.synchronize()
+    got = out.clone()
+    assert torch.equal(got, call())
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_pieces_are_joined(dim):
+    """Few blocks of rows over many keys (keys cut into pieces), ragged, on both tensor-core paths."""
+    for path in ("gemv", "mma"):
+        Case([3000, 700, 1], [20, 3, 1], 4, 2, dim, 64).check(path=path)
+        Case([2500], [70], 4, 1, dim, 16).check("f32", path=path, window=900)
+
+
+def test_example_runs():
+    import importlib.util
+    import pathlib
+    path = pathlib.Path(__file__).resolve().parent.parent / "examples" / "quantized_attention.py"
+    spec = importlib.util.spec_from_file_location("quantized_attention", path)
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    layer, table, held, q, a, out = m.run(steps=3)
+    off, size = m.check(layer, table, held, q, a)
+    # fp32 output: d P rounded to fp16 (2^-11 at most) of a mean of values of this size
+    assert bool(out.isfinite().all()) and off <= 2 ** -10 * 4 * size
+
+
 # ------------------------------------------------------------------- the step as a whole
 def test_step_of_a_layer_over_two_steps():
     """Plan, rotate, append, attend for a prompt step and a decode step; against 64 bits on the cache's own values."""
