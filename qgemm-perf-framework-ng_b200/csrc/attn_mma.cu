@@ -255,18 +255,18 @@ PFNG_DEV float load_q(const MmaParams &mp, int64_t at, bool live, uint8_t *to, i
             for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[k][j]));
 #pragma unroll
             for (int o = 1; o < kLanes; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            // largest value into [2^13, 2^14)
+            // largest value into [2^13, 2^14) (rows below 2^-113: less)
             int e = 0;
-            if (top > 0.0f && top < INFINITY) e = exponent_of(top) - 13;
-            const float up0 = power_of_two(-(e / 2)) * (p.scale < 0.0f ? -1.0f : 1.0f), up1 = power_of_two(-(e - e / 2));
+            if (top > 0.0f && top < INFINITY) e = max(exponent_of(top) - 13, -126);
+            const float up = power_of_two(-e) * (p.scale < 0.0f ? -1.0f : 1.0f);
             // a floor keeps -inf * mul at -inf for a scale of 0
-            const float row_mul = fmaxf(fabsf(p.scale) * kLog2e * power_of_two(e / 2) * power_of_two(e - e / 2), 1e-35f);
+            const float row_mul = fmaxf(fabsf(p.scale) * kLog2e * power_of_two(e), 1e-35f);
             uint32_t h[4];
             // values 0, 2 and 1, 3 of each four in a register
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const int v = 4 * (j >> 1) + (j & 1);
-                h[j] = h2(__floats2half2_rn(x[k][v] * up0 * up1, x[k][v + 2] * up0 * up1));
+                h[j] = h2(__floats2half2_rn(x[k][v] * up, x[k][v + 2] * up));
             }
             // chunk t of a block: values 4 t .. and 16 + 4 t ..; this lane has values 8 (sub % 4) .. of its
             // block: t = 0, 1 are made by lanes 0 and 2 of the four, t = 2, 3 by lanes 1 and 3

@@ -399,10 +399,10 @@ PFNG_DEV void load_rows(const StreamParams &sp, const Cursor &c, RowTile<DIM, NT
             }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // largest value into [2^13, 2^14): exact, and room for the 1/16
+        // largest value into [2^13, 2^14) (rows below 2^-113: less): exact, and room for the 1/16
         int e = 0;
-        if (top > 0.0f && top < INFINITY) e = exponent_of(top) - 13;
-        const float up0 = power_of_two(-(e / 2)), up1 = power_of_two(-(e - e / 2));
+        if (top > 0.0f && top < INFINITY) e = max(exponent_of(top) - 13, -126);
+        const float up = power_of_two(-e);
         float sum[DIM / 32];
 #pragma unroll
         for (int b = 0; b < DIM / 32; ++b) {
@@ -413,7 +413,7 @@ PFNG_DEV void load_rows(const StreamParams &sp, const Cursor &c, RowTile<DIM, NT
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     // high nibbles carry a factor 16: their q is divided by it
-                    const __half y = __float2half_rn(v[b][h][i] * up0 * up1 * (h ? 0.0625f : 1.0f));
+                    const __half y = __float2half_rn(v[b][h][i] * (h ? up * 0.0625f : up));
                     x[h][i] = __half2float(y);
                     sum[b] += x[h][i] * (h ? 16.0f : 1.0f);
                 }
@@ -424,7 +424,7 @@ PFNG_DEV void load_rows(const StreamParams &sp, const Cursor &c, RowTile<DIM, NT
             sum[b] += __shfl_xor_sync(0xffffffffu, sum[b], 1);
             sum[b] += __shfl_xor_sync(0xffffffffu, sum[b], 2);
         }
-        const float mul = p.scale * kLog2e * power_of_two((e + 24) / 2) * power_of_two(e + 24 - (e + 24) / 2);
+        const float mul = p.scale * kLog2e * power_of_two(e) * 0x1p24f;
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
             const int from = (2 * q4 + x) * 4;  // a lane that loaded row 2 q4 + x

@@ -118,7 +118,8 @@ int pfng_b200_qk_norm_rope(const void *x, int in_format, int64_t ldx, const floa
     const int st = device_status();
     if (st != PFNG_B200_OK) return st;
     const RopeArgs a{x, in_format, out_format, ldx, q_weight, k_weight, eps, positions, cos_sin, max_pos, rot_dim,
-                     interleaved, q_out, k_out, ldq, ldk, tokens, heads_q, heads_k, head_dim};
+                     interleaved, q_out, k_out, ldq, ldk, tokens, heads_q, heads_k, head_dim,
+                     1.0f / static_cast<float>(head_dim)};
     return status_of(launch_qk_norm_rope(a, static_cast<cudaStream_t>(stream)));
 }
 

@@ -78,18 +78,24 @@ PFNG_DEV void append(const AppendArgs &p, bool is_v) {
         }
         const float d = m * -0.125f;  // m / -8: the same rounding
         const float inv = d != 0.0f ? __frcp_rn(d) : 0.0f;
-        // x / d + 8.5 lies in [0.5, 16.5] (NaN counts as 0): with 2^23 added
-        // towards zero its whole part is the low bits
+        // x / d + 8.5 lies in [0.5, 16.5]; as (x / d + 8.5) / 16, the same rounding,
+        // it saturates to [0, 1], and NaN to 0.  With 2^23 added towards zero the
+        // whole part of 16 times it is in the low bits; 16 becomes 15.
         uint32_t q[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const float y = fminf(fmaxf(__fadd_rn(__fmul_rn(v[j], inv), 8.5f), 0.0f), 15.5f);
-            q[j] = __float_as_uint(__fadd_rz(y, 8388608.0f));
+            float z;
+            asm("fma.rn.sat.f32 %0, %1, %2, %3;" : "=f"(z) : "f"(__fmul_rn(v[j], inv)), "f"(0.0625f), "f"(0.53125f));
+            q[j] = __float_as_uint(__fmaf_rz(z, 16.0f, 8388608.0f));
         }
         // nibbles of values 8 quad .. + 3 and + 4 .. + 7, one a byte
-        const uint32_t n[2] = {
-            __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410),
-            __byte_perm(__byte_perm(q[4], q[5], 0x0040), __byte_perm(q[6], q[7], 0x0040), 0x5410)};
+        uint32_t n[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            n[h] = __byte_perm(__byte_perm(q[4 * h], q[4 * h + 1], 0x0040), __byte_perm(q[4 * h + 2], q[4 * h + 3], 0x0040),
+                               0x5410);
+            n[h] -= (n[h] >> 4) & 0x01010101u;
+        }
         // bytes 8 a .. 8 a + 7 of the block are lanes a (low nibbles) and a + 2
         // (high nibbles), a = 0, 1: lane a keeps the first four, lane a + 2 the
         // last four, so each needs one word of the other

@@ -155,6 +155,7 @@ struct RopeArgs {
     void *q_out, *k_out;
     int64_t ldq, ldk;
     int64_t tokens, heads_q, heads_k, head_dim;
+    float inv_dim;  // 1 / head_dim
 };
 cudaError_t launch_qk_norm_rope(const RopeArgs &args, cudaStream_t s);
 

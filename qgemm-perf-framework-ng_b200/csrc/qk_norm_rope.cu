@@ -10,16 +10,14 @@
 // consecutive slots, so both values of a pair are in one lane and the only
 // exchange is the sum of squares over the lanes of a head.  Everything is in
 // fp32 registers between one read and one write (rounded once, at the write).
+#include <type_traits>
+
 #include "kv_cache.cuh"
 
-#ifndef KT
-#define KT 128
-#define KH 4
-#endif
 namespace pfng {
 namespace {
 
-constexpr int kThreads = KT;
+constexpr int kThreads = 128;
 
 // Elements of slots s .. s + N - 1: N values from a and N from b.  Interleaved
 // pairs are adjacent: 2 N values in a row, b = a + N.
@@ -39,7 +37,8 @@ PFNG_DEV void slot_elements(const RopeArgs &p, int s, int &a, int &b, bool &turn
 // H heads of one token (all query or all key heads) by one group of `lanes`
 // lanes: their loads are in flight together, and cosines, sines and weights
 // are read once for all of them.
-template <int FMT, int N, int H, bool INTERLEAVED>
+// OUT: the output format, or -1 to take it from the arguments.
+template <int FMT, int OUT, int N, int H, bool INTERLEAVED>
 __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const RopeArgs p, int lanes) {
     const uint32_t q_parts = static_cast<uint32_t>((p.heads_q + H - 1) / H);
     const uint32_t parts = q_parts + static_cast<uint32_t>((p.heads_k + H - 1) / H);
@@ -86,15 +85,25 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const RopeArgs p
 #pragma unroll
                 for (int j = 0; j < N; ++j) sum += x[h][i][0][j] * x[h][i][0][j] + x[h][i][1][j] * x[h][i][1][j];
             for (int o = 1; o < lanes; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            scale[h] = 1.0f / sqrtf(sum / static_cast<float>(dim) + p.eps);
+            scale[h] = rsqrtf(sum * p.inv_dim + p.eps);
         }
     }
     if (count <= 0) return;
     const bool known = pos >= 0 && pos < p.max_pos;
-    // padding rows (no position) are zeros, a position past the table is NaN
-    const float blank = pos < 0 ? 0.0f : __int_as_float(0x7fffffff);
+    const int out_format = OUT < 0 ? p.out_format : OUT;
     void *out = is_q ? p.q_out : p.k_out;
     const int64_t to = token * (is_q ? p.ldq : p.ldk) + static_cast<int64_t>(head0) * dim;
+    if (!known) {  // padding rows (no position) are zeros, a position past the table is NaN
+        float blank[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) blank[j] = pos < 0 ? 0.0f : __int_as_float(0x7fffffff);
+        for (int h = 0; h < count; ++h)
+            for (int s = sub * N; s < slots; s += lanes * N) {
+                store_values<N>(out_format, out, to + h * dim + 2 * s, blank);
+                store_values<N>(out_format, out, to + h * dim + 2 * s + N, blank);
+            }
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
         const int s = (i * lanes + sub) * N;
@@ -106,7 +115,7 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const RopeArgs p
         float c[N], z[N], w0[N], w1[N];
 #pragma unroll
         for (int j = 0; j < N; ++j) c[j] = 1.0f, z[j] = 0.0f, w0[j] = w1[j] = 1.0f;
-        if (turns && known) {
+        if (turns) {
             load_values<N>(kOutF32, p.cos_sin, pos * p.rot_dim + s, c);
             load_values<N>(kOutF32, p.cos_sin, pos * p.rot_dim + p.rot_dim / 2 + s, z);
         }
@@ -129,16 +138,16 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const RopeArgs p
             for (int j = 0; j < N; ++j) {
                 const float v0 = adjacent ? (2 * j < N ? u[(2 * j) % N] : w[(2 * j) % N]) : u[j];
                 const float v1 = adjacent ? (2 * j + 1 < N ? u[(2 * j + 1) % N] : w[(2 * j + 1) % N]) : w[j];
-                y[j] = known ? v0 * c[j] - v1 * z[j] : blank;
-                y[N + j] = known ? v1 * c[j] + v0 * z[j] : blank;
+                y[j] = v0 * c[j] - v1 * z[j];
+                y[N + j] = v1 * c[j] + v0 * z[j];
             }
 #pragma unroll
             for (int j = 0; j < N; ++j) {
                 u[j] = adjacent ? y[(j & 1) * N + j / 2] : y[j];
                 w[j] = adjacent ? y[((N + j) & 1) * N + (N + j) / 2] : y[N + j];
             }
-            store_values<N>(p.out_format, out, to + h * dim + a, u);
-            store_values<N>(p.out_format, out, to + h * dim + b, w);
+            store_values<N>(out_format, out, to + h * dim + a, u);
+            store_values<N>(out_format, out, to + h * dim + b, w);
         }
     }
 }
@@ -149,15 +158,24 @@ cudaError_t launch(const RopeArgs &p, int lanes, cudaStream_t s) {
     const int64_t per_block = kThreads / lanes;
     const unsigned grid = static_cast<unsigned>((parts + per_block - 1) / per_block);
     const auto run = [&](auto kernel) { kernel<<<grid, kThreads, 0, s>>>(p, lanes); };
-    if (p.interleaved) {
-        if (p.in_format == kOutF32) run(qk_norm_rope_kernel<kOutF32, N, H, true>);
-        else if (p.in_format == kOutF16) run(qk_norm_rope_kernel<kOutF16, N, H, true>);
-        else run(qk_norm_rope_kernel<kOutBF16, N, H, true>);
-    } else {
-        if (p.in_format == kOutF32) run(qk_norm_rope_kernel<kOutF32, N, H, false>);
-        else if (p.in_format == kOutF16) run(qk_norm_rope_kernel<kOutF16, N, H, false>);
-        else run(qk_norm_rope_kernel<kOutBF16, N, H, false>);
-    }
+    const auto by_out = [&](auto in, auto interleaved) {
+        constexpr int kIn = decltype(in)::value;
+        constexpr bool kInterleaved = decltype(interleaved)::value;
+        if constexpr (H == 1) {
+            run(qk_norm_rope_kernel<kIn, -1, N, H, kInterleaved>);
+        } else {
+            if (p.out_format == kOutF32) run(qk_norm_rope_kernel<kIn, kOutF32, N, H, kInterleaved>);
+            else if (p.out_format == kOutF16) run(qk_norm_rope_kernel<kIn, kOutF16, N, H, kInterleaved>);
+            else run(qk_norm_rope_kernel<kIn, kOutBF16, N, H, kInterleaved>);
+        }
+    };
+    const auto by_in = [&](auto interleaved) {
+        if (p.in_format == kOutF32) by_out(std::integral_constant<int, kOutF32>{}, interleaved);
+        else if (p.in_format == kOutF16) by_out(std::integral_constant<int, kOutF16>{}, interleaved);
+        else by_out(std::integral_constant<int, kOutBF16>{}, interleaved);
+    };
+    if (p.interleaved) by_in(std::true_type{});
+    else by_in(std::false_type{});
     return cudaGetLastError();
 }
 
@@ -179,7 +197,7 @@ cudaError_t launch_qk_norm_rope(const RopeArgs &p, cudaStream_t s) {
     if (!vec) return launch<1, 1>(p, lanes, s);
     // Four heads a lane group where that still leaves every SM its threads.
     const bool many = p.head_dim <= 256 && p.tokens * (p.heads_q + p.heads_k) * lanes >= int64_t{4} * 2048 * device_sm_count();
-    return many ? launch<4, KH>(p, lanes, s) : launch<4, 1>(p, lanes, s);
+    return many ? launch<4, 4>(p, lanes, s) : launch<4, 1>(p, lanes, s);
 }
 
 }  // namespace pfng
