@@ -233,6 +233,33 @@ PFNG_DEV uint32_t operand_at(int r, int c) {
     return static_cast<uint32_t>((c >> 3) * (kTile * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
 }
 
+// Shared memory at a 32-bit address plus a constant.
+PFNG_DEV uint32_t lds32(uint32_t at) {
+    uint32_t x;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(x) : "r"(at));
+    return x;
+}
+PFNG_DEV uint2 lds64(uint32_t at) {
+    uint2 x;
+    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(x.x), "=r"(x.y) : "r"(at));
+    return x;
+}
+PFNG_DEV uint4 lds128(uint32_t at) {
+    uint4 x;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(at));
+    return x;
+}
+PFNG_DEV void sts128(uint32_t at, uint4 x) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
+}
+// All ones in the halves of x that are finite.
+PFNG_DEV uint32_t finite_mask(uint32_t x) {
+    uint32_t mask;
+    asm("{\n\t.reg .b32 a;\n\tand.b32 a, %1, 0x7fff7fff;\n\tset.lt.u32.f16x2 %0, a, %2;\n\t}"
+        : "=r"(mask)
+        : "r"(x), "r"(0x7c007c00u));
+    return mask;
+}
 // A word of a cache row as 8 fp16 values (n - 8) * s, in pairs: low nibbles of
 // bytes 0, 2; of bytes 1, 3; high nibbles of bytes 0, 2; of bytes 1, 3.
 PFNG_DEV uint4 unpack_word(uint32_t w, uint32_t scale, uint32_t magic) {
@@ -456,63 +483,80 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
     const auto dequantize = [&](int first_task) {
         uint32_t magic;
         asm volatile("mov.b32 %0, 0x64006400;" : "=r"(magic));
-        constexpr int kPieces = DIM / 64;  // 16-byte pieces of a group's rows per lane
-        constexpr int kQuads = DIM / 32;   // pieces of a row
+        constexpr int kQuads = DIM / 32;     // 16-byte pieces of a row
+        constexpr int kPieces = DIM / 64;    // of them per lane and group: rows lane / kQuads + i * 32 / kQuads
+        const int u = lane % kQuads, row0 = lane / kQuads;
+        // A lane's rows have the same number modulo 8 in every group, so where its four chunks 4 u + x go within a
+        // row is known once.
+        uint32_t chunk_at[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) chunk_at[x] = base + L::kKV + operand_at(row0 & 7, 4 * u + x) + (row0 & ~7) * 128;
+        const uint32_t raw_at = base + L::kRawAt + row0 * kv_row_bytes(DIM) + 16 * u;
+        const uint32_t scales_at = base + L::kRawAt + kv_scale_offset(DIM) + row0 * (DIM / 16);
         int g = first_task, slot = 0, buf = 0;
         uint32_t raw_phase = 0, op_phase = 1;  // op_empty: the first round does not wait
         for (int j = 0; j < 2 * count;) {
             const int n = j >> 1;
             const bool is_v = j & 1;
             if (!wait_bar(&raw_full[slot], raw_phase, &abort_flag, mp.err, kErrWaitFull)) return false;
-            const uint8_t *raw = smem + L::kRawAt + slot * L::kRaw + g * kv_group_bytes(DIM);
-            TileInfo &info = infos[n % kInfoSlots];
-            const bool there = (info.groups >> g) & 1u;
-            const int keys = seq - (first + n) * kTile - g * kKvGroup;  // rows past the last key are zeros
+            const uint32_t group = slot * L::kRaw + g * kv_group_bytes(DIM);
             uint4 words[kPieces];
             uint32_t scales[kPieces][kBlocks / 2];
 #pragma unroll
             for (int i = 0; i < kPieces; ++i) {
-                const int row = (i * 32 + lane) / kQuads, u = lane % kQuads;
-                words[i] = *reinterpret_cast<const uint4 *>(raw + row * kv_row_bytes(DIM) + 16 * u);
-#pragma unroll
-                for (int b = 0; b < kBlocks / 2; ++b) {
-                    scales[i][b] = *reinterpret_cast<const uint32_t *>(raw + kv_scale_offset(DIM) + row * (DIM / 16) + 4 * b);
-                    if (!there || row >= keys) scales[i][b] = 0;
+                words[i] = lds128(raw_at + group + i * (32 / kQuads) * kv_row_bytes(DIM));
+                const uint32_t at = scales_at + group + i * (32 / kQuads) * (DIM / 16);
+                if constexpr (kBlocks == 4) {
+                    const uint2 x = lds64(at);
+                    scales[i][0] = x.x, scales[i][1] = x.y;
+                } else {
+                    scales[i][0] = lds32(at);
                 }
             }
+            TileInfo &info = infos[n % kInfoSlots];
+            const int keys = (info.groups >> g) & 1u ? seq - (first + n) * kTile - g * kKvGroup : 0;
             __syncwarp();
             if (lane == 0) mbar_arrive(&raw_empty[slot]);
-            if (!wait_bar(&op_empty[buf], op_phase, &abort_flag, mp.err, kErrWaitEmpty)) return false;
-            uint8_t *to = smem + L::kKV + buf * L::kOperand;
+            if (keys < kKvGroup) {  // rows past the last key, or a group that is not there, are zeros
 #pragma unroll
-            for (int i = 0; i < kPieces; ++i) {
-                const int row = g * kKvGroup + (i * 32 + lane) / kQuads, u = lane % kQuads;
-                uint32_t s[4];
-                // scales that are not finite: of V 0 and the key marked, as 0 * inf would reach the rows that do
-                // not see it; of K NaN, which is masked with the score
-                bool bad = false;
+                for (int i = 0; i < kPieces; ++i)
 #pragma unroll
-                for (int b = 0; b < kBlocks / 2; ++b)
-                    bad |= (scales[i][b] & 0x7c00u) == 0x7c00u || (scales[i][b] & 0x7c000000u) == 0x7c000000u;
-                if (bad) {
+                    for (int b = 0; b < kBlocks / 2; ++b)
+                        if (row0 + i * (32 / kQuads) >= keys) scales[i][b] = 0;
+            }
+            // Scales that are not finite: of V 0 and the key marked, as 0 * inf would reach the rows that do not see
+            // it; of K NaN, which is masked with the score.
+            uint32_t finite = 0xffffffffu;
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i)
+#pragma unroll
+                for (int b = 0; b < kBlocks / 2; ++b) finite &= finite_mask(scales[i][b]);
+            if (finite != 0xffffffffu) {
+#pragma unroll
+                for (int i = 0; i < kPieces; ++i) {
+                    uint32_t own = 0xffffffffu;
+#pragma unroll
+                    for (int b = 0; b < kBlocks / 2; ++b) own &= finite_mask(scales[i][b]);
+                    if (own == 0xffffffffu) continue;
 #pragma unroll
                     for (int b = 0; b < kBlocks / 2; ++b) scales[i][b] = is_v ? 0u : 0x7fff7fffu;
+                    const int row = g * kKvGroup + row0 + i * (32 / kQuads);
                     if (is_v && u == 0) atomicOr(&info.bad[row >> 5], 1u << (row & 31));
                 }
-                if (is_v) {
+            }
+            if (!wait_bar(&op_empty[buf], op_phase, &abort_flag, mp.err, kErrWaitEmpty)) return false;
+            const uint32_t to = buf * L::kOperand + g * kKvGroup * 128;
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) s[x] = scales[i][kBlocks == 4 ? (x & 1) : 0];
-                } else {
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        const int b = x % kBlocks;
-                        s[x] = __byte_perm(scales[i][b / 2], 0, (b & 1) ? 0x3232 : 0x1010);
-                    }
-                }
+            for (int i = 0; i < kPieces; ++i) {
                 const uint32_t w[4] = {words[i].x, words[i].y, words[i].z, words[i].w};
 #pragma unroll
-                for (int x = 0; x < 4; ++x)
-                    *reinterpret_cast<uint4 *>(to + operand_at(row, 4 * u + x)) = unpack_word(w[x], s[x], magic);
+                for (int x = 0; x < 4; ++x) {
+                    // K: a word is of one block; V: of two, whose scales are a register
+                    const int b = x % kBlocks;
+                    const uint32_t s = is_v ? scales[i][kBlocks == 4 ? (x & 1) : 0]
+                                            : __byte_perm(scales[i][b / 2], 0, (b & 1) ? 0x3232 : 0x1010);
+                    sts128(chunk_at[x] + to + i * (32 / kQuads) * 128, unpack_word(w[x], s, magic));
+                }
             }
             fence_proxy_async_smem();
             __syncwarp();
