@@ -71,6 +71,18 @@ struct TileInfo {
     uint32_t bad[4];  // keys whose V scale is not finite (their V operand is zero)
 };
 
+// A piece of work: a block of rows with the key tiles that they see (or a piece of those).
+struct Item {
+    int id;            // CTA of the grid whose work this is; -1: there is none any more
+    int row0, rows;    // first row of the block; rows of the request
+    int seq, all;      // keys and new tokens of the request
+    int first, count;  // key tiles
+    int tile0;         // key tiles of the items before
+    int head_kv;
+    int64_t token0;    // first token of the request
+};
+constexpr int kItems = 4;  // the copying warp is ahead of the others by as many at most
+
 template <int DIM>
 struct Layout {
     static constexpr uint32_t kOperand = kTile * DIM * 2;  // an operand tile, fp16
@@ -80,7 +92,7 @@ struct Layout {
     static constexpr uint32_t kRawAt = kKV + kOperands * kOperand;  // [kRawSlots]
     static constexpr uint32_t kInfo = kRawAt + kRawSlots * kRaw;
     static constexpr uint32_t kBars = kInfo + ((kInfoSlots * sizeof(TileInfo) + 7) & ~7u);
-    static constexpr uint32_t kNumBars = 2 * kRawSlots + 2 * kOperands + 2 + 4 + 2 + 2;
+    static constexpr uint32_t kNumBars = 2 * kRawSlots + 2 * kOperands + 2 + 4 + 2 + 2 + 1 + 2 * kItems + 1;
     static constexpr uint32_t kBytes = kBars + 8 * kNumBars + 16 + 1024;
 };
 
@@ -93,6 +105,31 @@ struct MmaParams {
     float2 *part_ml;     // and [block][split][kRows] reference (log2) and sum
     int *err;
 };
+
+// The work of a CTA of this grid that has not started, if there is one, becomes
+// this CTA's: `response` then names it (asked for once after the other, and not
+// after the answer that there is none).
+PFNG_DEV void steal_ask(uint4 *response, uint64_t *bar) {
+    mbar_arrive_expect_tx(bar, 16);
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                     smem_u32(response)),
+                 "r"(smem_u32(bar))
+                 : "memory");
+}
+PFNG_DEV int stolen(const uint4 *response) {
+    int x;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b128 b;\n\t.reg .b32 x, y, z;\n\t"
+        "ld.shared.b128 b, [%1];\n\t"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, b;\n\t"
+        "mov.b32 x, -1;\n\t"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {x, y, z, _}, b;\n\t"
+        "mov.b32 %0, x;\n\t}"
+        : "=r"(x)
+        : "r"(smem_u32(response))
+        : "memory");
+    return x;
+}
 
 // The MMAs run in a warp whose control flow is uniform, so that descriptors
 // stay in uniform registers; `leader` is 1 in the one lane that issues.
@@ -272,83 +309,112 @@ PFNG_DEV uint4 unpack_word(uint32_t w, uint32_t scale, uint32_t magic) {
                       h2(__hmul2(__hfma2(as_h2(and_or<0x00F000F0u>(w8, magic)), sixteenth, minus72), s)));
 }
 
+// The larger of each half's magnitude of two words, a NaN aside; the larger of the two of one.
+template <int FMT>
+PFNG_DEV uint32_t larger_magnitude(uint32_t x, uint32_t y) {
+    uint32_t z;
+    if constexpr (FMT == kOutBF16)
+        asm("max.bf16x2 %0, %1, %2;" : "=r"(z) : "r"(x & 0x7fff7fffu), "r"(y & 0x7fff7fffu));
+    else
+        asm("max.f16x2 %0, %1, %2;" : "=r"(z) : "r"(x & 0x7fff7fffu), "r"(y & 0x7fff7fffu));
+    return z;
+}
+
 // The 32 query rows of a warp into their rows of the Q operand: scaled by a
 // power of two each (and the sign of the softmax scale), in the order of K's
-// words.  DIM / 8 lanes read a row, eight values each, so that a load covers
-// whole lines (a row per lane took 15000 cycles for a CTA's rows).  Returns,
-// for the row of this lane, the factor from accumulators to scores in log2
-// units.  row: the warp's first row; `at`, `live`: where this lane's row is.
+// words.  DIM / 8 lanes read a row, a chunk of the operand each (values 4 t ..
+// and 16 + 4 t .. of a block of 32), so that a load covers whole sectors.  A
+// CTA runs this once, with a cold instruction cache: few instructions in a
+// rolled loop (16 rows' reductions by halving across the lanes instead of one
+// butterfly each) took the CTA's Q from 10500 to QCYC cycles.  Returns, for the
+// row of this lane, the factor from accumulators to scores in log2 units.
+// row: the warp's first row; `at`: where this lane's row is (some row of q for
+// one that is not there: nothing is made of it).
 template <int DIM, int FMT>
-PFNG_DEV float load_q(const MmaParams &mp, int64_t at, bool live, uint8_t *to, int row) {
+PFNG_DEV float load_q(const MmaParams &mp, int64_t at, uint8_t *to, int row) {
     const AttnArgs &p = mp.a;
-    constexpr int kLanes = DIM / 8, kAtOnce = 32 / kLanes, kSteps = 32 / kAtOnce, kBatch = FMT == kOutF32 ? 4 : 8;
-    const int lane = threadIdx.x & 31, sub = lane % kLanes, part = lane / kLanes;
+    constexpr int kBlocks = DIM / 32, kLanes = DIM / 8, kBatch = 8;  // lane group `part` reads rows kLanes part ..
+    const int lane = threadIdx.x & 31, sub = lane % kLanes, first_row = lane - sub;
+    const int col = 32 * (sub % kBlocks) + 4 * (sub / kBlocks);
+    const bool wide = mp.vec_q;
+    const float sign = p.scale < 0.0f ? -1.0f : 1.0f;
     float mul = 0.0f;
 #pragma unroll 1
-    for (int step0 = 0; step0 < kSteps; step0 += kBatch) {
-        RawValues<FMT, 8> x[kBatch];
+    for (int step = 0; step < kLanes; step += kBatch) {
+        RawValues<FMT, 4> x[kBatch][2];
+        if (wide) {
 #pragma unroll
-        for (int k = 0; k < kBatch; ++k) {
-            const int mine = (step0 + k) * kAtOnce + part;  // of the warp's rows
-            const int64_t from = __shfl_sync(0xffffffffu, at, mine) + 8 * sub;
-            x[k].zero();
-            if (!__shfl_sync(0xffffffffu, static_cast<int>(live), mine)) continue;
-            if (mp.vec_q) {
-                x[k].load(p.q, from);
-            } else {
+            for (int k = 0; k < kBatch; ++k) {
+                const int64_t from = __shfl_sync(0xffffffffu, at, first_row + step + k) + col;
+                x[k][0].load(p.q, from), x[k][1].load(p.q, from + 16);
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) {
+                const int64_t from = __shfl_sync(0xffffffffu, at, first_row + step + k) + col;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     RawValues<FMT, 1> one;
-                    one.load(p.q, from + j);
-                    if constexpr (FMT == kOutF32) x[k].w[j] = one.w[0];
-                    else x[k].w[j / 2] |= one.w[0] << (16 * (j & 1));
+                    one.load(p.q, from + 16 * (j >> 2) + (j & 3));
+                    if constexpr (FMT == kOutF32) x[k][j >> 2].w[j & 3] = one.w[0];
+                    else if (j & 1) x[k][j >> 2].w[(j & 3) / 2] |= one.w[0] << 16;
+                    else x[k][j >> 2].w[(j & 3) / 2] = one.w[0];
                 }
             }
         }
+        float top[kBatch];
 #pragma unroll
         for (int k = 0; k < kBatch; ++k) {
-            float top = 0.0f;
+            if constexpr (FMT == kOutF32) {
+                top[k] = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[k][j]));
+                for (int j = 0; j < 8; ++j) top[k] = fmaxf(top[k], fabsf(x[k][j >> 2][j & 3]));
+            } else {
+                const uint32_t z = larger_magnitude<FMT>(larger_magnitude<FMT>(x[k][0].w[0], x[k][0].w[1]),
+                                                         larger_magnitude<FMT>(x[k][1].w[0], x[k][1].w[1]));
+                RawValues<FMT, 2> two;
+                two.w[0] = z;
+                top[k] = fmaxf(fmaxf(two[0], two[1]), 0.0f);
+            }
+        }
+        // lane 8 i + k of a row's lanes gets the largest of row k
 #pragma unroll
-            for (int o = 1; o < kLanes; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            // largest value into [2^13, 2^14) (rows below 2^-113: less)
-            int e = 0;
-            if (top > 0.0f && top < INFINITY) e = max(exponent_of(top) - 13, -126);
-            const float up = power_of_two(-e) * (p.scale < 0.0f ? -1.0f : 1.0f);
-            // a floor keeps -inf * mul at -inf for a scale of 0
-            const float row_mul = fmaxf(fabsf(p.scale) * kLog2e * power_of_two(e), 1e-35f);
+        for (int d = kBatch / 2; d > 0; d >>= 1)
+#pragma unroll
+            for (int k = 0; k < d; ++k) {
+                const float other = __shfl_xor_sync(0xffffffffu, (sub & d) ? top[k] : top[k + d], d);
+                top[k] = fmaxf((sub & d) ? top[k + d] : top[k], other);
+            }
+        if constexpr (kLanes > kBatch) top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], kBatch));
+        // largest value into [2^13, 2^14) (rows below 2^-113: less)
+        int e = 0;
+        if (top[0] > 0.0f && top[0] < INFINITY) e = max(exponent_of(top[0]) - 13, -126);
+        const float up = power_of_two(-e) * sign;
+        // a floor keeps -inf * mul at -inf for a scale of 0; lane `sub` owns row `sub` of its group
+        if (sub / kBatch == step / kBatch) mul = fmaxf(fabsf(p.scale) * kLog2e * power_of_two(e), 1e-35f);
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+            const float f = __shfl_sync(0xffffffffu, up, (lane & ~(kBatch - 1)) + k);
             uint32_t h[4];
             // values 0, 2 and 1, 3 of each four in a register
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int v = 4 * (j >> 1) + (j & 1);
-                h[j] = h2(__floats2half2_rn(x[k][v] * up, x[k][v + 2] * up));
-            }
-            // chunk t of a block: values 4 t .. and 16 + 4 t ..; this lane has values 8 (sub % 4) .. of its
-            // block: t = 0, 1 are made by lanes 0 and 2 of the four, t = 2, 3 by lanes 1 and 3
-            const bool upper = sub & 2;
-            const uint32_t r0 = __shfl_xor_sync(0xffffffffu, upper ? h[0] : h[2], 2);
-            const uint32_t r1 = __shfl_xor_sync(0xffffffffu, upper ? h[1] : h[3], 2);
-            const int t = 2 * (sub & 1) + (upper ? 1 : 0), c = t * (DIM / 32) + sub / 4;
-            *reinterpret_cast<uint4 *>(to + operand_at(row + (step0 + k) * kAtOnce + part, c)) =
-                upper ? make_uint4(r0, r1, h[2], h[3]) : make_uint4(h[0], h[1], r0, r1);
-            // the lane that owns a row takes its factor
-            const float m = __shfl_sync(0xffffffffu, row_mul, (lane % kAtOnce) * kLanes);
-            if (lane / kAtOnce == step0 + k) mul = m;
+            for (int j = 0; j < 4; ++j) h[j] = h2(__floats2half2_rn(x[k][j >> 1][j & 1] * f, x[k][j >> 1][(j & 1) + 2] * f));
+            *reinterpret_cast<uint4 *>(to + operand_at(row + first_row + step + k, sub)) = make_uint4(h[0], h[1], h[2], h[3]);
         }
     }
     return mul;
 }
 
 // The O rows of a warp, times f of each row, from TMEM to memory in format FMT.
-// Through shared memory (`mine`, 64 DIM bytes), so that a store covers whole
-// lines: rows of 16-byte pieces, piece x of row y at x ^ y.  `at`, `live`: where
-// this lane's row goes; zeros where there is no O (`have`).
+// Through shared memory (the warp's own rows of Q, from `row` on, in the same
+// swizzle), so that a store covers whole lines.  `at`, `live`: where this lane's
+// row goes; zeros where there is no O (`have`).
 template <int DIM, int FMT>
-PFNG_DEV void write_rows(void *out, int64_t at, bool live, bool wide, float f, uint32_t o_at, bool have, uint8_t *mine) {
+PFNG_DEV void write_rows(void *out, int64_t at, bool live, bool wide, float f, uint32_t o_at, bool have, uint8_t *q, int row) {
     constexpr int kBlocks = DIM / 32, kSize = FMT == kOutF32 ? 4 : 2, kAtOnce = 64 / kSize, kPieces = DIM * kSize / 16;
     const int lane = threadIdx.x & 31;
+    constexpr int kChunks = DIM / 8;  // of a row of Q: an fp32 output row takes two
+    const auto piece_of = [&](int y, int x) { return q + operand_at(row + y * (kPieces / kChunks) + x / kChunks, x % kChunks); };
     const uint32_t rows_live = __ballot_sync(0xffffffffu, live);
 #pragma unroll 1
     for (int row1 = 0; row1 < 32; row1 += kAtOnce) {
@@ -384,7 +450,7 @@ PFNG_DEV void write_rows(void *out, int64_t at, bool live, bool wide, float f, u
                         }
                         if (staged) {
                             const int piece = dim * kSize / 16, in_piece = dim * kSize % 16;
-                            store_values<4>(FMT, mine + (y * kPieces + (piece ^ (y % kPieces))) * 16 + in_piece, 0, v);
+                            store_values<4>(FMT, piece_of(y, piece) + in_piece, 0, v);
                         }
                         if (direct) {
 #pragma unroll 1
@@ -401,7 +467,7 @@ PFNG_DEV void write_rows(void *out, int64_t at, bool live, bool wide, float f, u
             for (int idx = lane; idx < kAtOnce * kPieces; idx += 32) {
                 const int z = idx / kPieces, x = idx % kPieces;
                 const int64_t to = __shfl_sync(0xffffffffu, at, row1 + z) * kSize + 16 * x;
-                const uint4 piece = *reinterpret_cast<const uint4 *>(mine + (z * kPieces + (x ^ (z % kPieces))) * 16);
+                const uint4 piece = *reinterpret_cast<const uint4 *>(piece_of(z, x));
                 if ((rows_live >> (row1 + z)) & 1u) *reinterpret_cast<uint4 *>(static_cast<uint8_t *>(out) + to) = piece;
             }
         }
@@ -419,38 +485,17 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
     uint64_t *raw_full = bars, *raw_empty = raw_full + kRawSlots;
     uint64_t *op_full = raw_empty + kRawSlots, *op_empty = op_full + kOperands;
     uint64_t *s_full = op_empty + kOperands, *p_full = s_full + 2, *o_full = p_full + 4;
-    uint64_t *q_full = o_full + 2, *mma_done = q_full + 1;
+    uint64_t *q_full = o_full + 2, *mma_done = q_full + 2, *item_full = mma_done + 1, *item_empty = item_full + kItems;
+    uint64_t *steal_full = item_empty + kItems;
     uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(bars + L::kNumBars);
     TileInfo *infos = reinterpret_cast<TileInfo *>(smem + L::kInfo);
     __shared__ int abort_flag;
+    __shared__ Item items[kItems];
+    __shared__ __align__(16) uint4 steal_response;
 
     const AttnArgs &p = mp.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    // the last row tiles see the most keys: they come first
-    const uint32_t per_tile = static_cast<uint32_t>(p.requests * p.heads_kv * mp.splits);
-    const int tile = mp.tiles - 1 - static_cast<int>(blockIdx.x / per_tile);
-    const uint32_t rest = blockIdx.x % per_tile;
-    const int split = static_cast<int>(rest % mp.splits), head_kv = static_cast<int>(rest / mp.splits % p.heads_kv);
-    const int64_t r = rest / (static_cast<uint32_t>(mp.splits) * p.heads_kv);
     const int group = p.group;
-    int all;
-    const int rows = attn_new_tokens(p, r, all) * group;
-    const int row0 = tile * kRows;
-    if (row0 >= rows) return;
-    const int seq = attn_seq_len(p, r);
-    const int row_tiles = rows - row0 > kTile ? 2 : 1;
-    int first, count;  // key tiles
-    {
-        int lo, hi, lo2, hi2;
-        attn_visible(p, seq, all, row0 / group, lo, hi2);
-        attn_visible(p, seq, all, (min(row0 + kRows, rows) - 1) / group, lo2, hi);
-        first = max(lo, 0) / kTile;
-        count = hi > first * kTile ? (hi + kTile - 1) / kTile - first : 0;
-        // this CTA's piece of them
-        const int begin = static_cast<int>(static_cast<int64_t>(count) * split / mp.splits);
-        count = static_cast<int>(static_cast<int64_t>(count) * (split + 1) / mp.splits) - begin;
-        first += begin;
-    }
     pdl_trigger();
 
     if (tid == 0) {
@@ -458,12 +503,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
         for (int i = 0; i < kRawSlots; ++i) mbar_init(&raw_full[i], 1), mbar_init(&raw_empty[i], kGroups);
         for (int i = 0; i < kOperands; ++i) mbar_init(&op_full[i], kGroups), mbar_init(&op_empty[i], 1);
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&s_full[i], 1), mbar_init(&o_full[i], 1);
+            mbar_init(&s_full[i], 1), mbar_init(&o_full[i], 1), mbar_init(&q_full[i], 4);
             mbar_init(&p_full[2 * i], 4), mbar_init(&p_full[2 * i + 1], 4);
-
         }
-        mbar_init(q_full, 4 * row_tiles);
-        mbar_init(mma_done, 1);
+        for (int i = 0; i < kItems; ++i) mbar_init(&item_full[i], 1), mbar_init(&item_empty[i], kThreads / 32 - 1);
+        mbar_init(mma_done, 1), mbar_init(steal_full, 1);
         fence_mbar_init();
     }
     if (warp == 12) {
@@ -475,6 +519,22 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
     tc_fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(tmem_holder);
     const uint32_t base = smem_u32(smem);
+
+    // Every warp but the copying one takes the items in turn; false at the end
+    // (or when a role gave up).
+    int item_no = 0;
+    const auto next_item = [&](Item &it) {
+        const int slot = item_no % kItems;
+        if (!wait_bar(&item_full[slot], (item_no / kItems) & 1, &abort_flag, mp.err, kErrWaitFull)) {
+            abort_flag = 1;
+            return false;
+        }
+        it = items[slot];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&item_empty[slot]);
+        ++item_no;
+        return it.id >= 0;
+    };
 
     // ---------------- dequantization ----------------
     // The tasks are the 16-key groups of the units in order, dealt to the
@@ -495,10 +555,16 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
         const uint32_t scales_at = base + L::kRawAt + kv_scale_offset(DIM) + row0 * (DIM / 16);
         int g = first_task, slot = 0, buf = 0;
         uint32_t raw_phase = 0, op_phase = 1;  // op_empty: the first round does not wait
-        for (int j = 0; j < 2 * count;) {
+        Item it;
+        if (!next_item(it)) return;
+        for (int j = 0;;) {
+            while (j >= 2 * it.count) {
+                j -= 2 * it.count;
+                if (!next_item(it)) return;
+            }
             const int n = j >> 1;
             const bool is_v = j & 1;
-            if (!wait_bar(&raw_full[slot], raw_phase, &abort_flag, mp.err, kErrWaitFull)) return false;
+            if (!wait_bar(&raw_full[slot], raw_phase, &abort_flag, mp.err, kErrWaitFull)) break;
             const uint32_t group = slot * L::kRaw + g * kv_group_bytes(DIM);
             uint4 words[kPieces];
             uint32_t scales[kPieces][kBlocks / 2];
@@ -513,8 +579,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
                     scales[i][0] = lds32(at);
                 }
             }
-            TileInfo &info = infos[n % kInfoSlots];
-            const int keys = (info.groups >> g) & 1u ? seq - (first + n) * kTile - g * kKvGroup : 0;
+            TileInfo &info = infos[(it.tile0 + n) % kInfoSlots];
+            const int keys = (info.groups >> g) & 1u ? it.seq - (it.first + n) * kTile - g * kKvGroup : 0;
             __syncwarp();
             if (lane == 0) mbar_arrive(&raw_empty[slot]);
             if (keys < kKvGroup) {  // rows past the last key, or a group that is not there, are zeros
@@ -544,7 +610,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
                     if (is_v && u == 0) atomicOr(&info.bad[row >> 5], 1u << (row & 31));
                 }
             }
-            if (!wait_bar(&op_empty[buf], op_phase, &abort_flag, mp.err, kErrWaitEmpty)) return false;
+            if (!wait_bar(&op_empty[buf], op_phase, &abort_flag, mp.err, kErrWaitEmpty)) break;
             const uint32_t to = buf * L::kOperand + g * kKvGroup * 128;
 #pragma unroll
             for (int i = 0; i < kPieces; ++i) {
@@ -569,7 +635,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
                 if (++buf == kOperands) buf = 0, op_phase ^= 1;
             }
         }
-        return true;
+        abort_flag = 1;
     };
 
     // Registers: 512 threads x 128 at launch, 2 x 192 + 2 x 64 a thread of the
@@ -578,26 +644,34 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
         // ---------------- softmax ----------------
         registers_up<192>();
         const int i = warp >> 2;  // row tile
-        const int in_tile = (warp & 3) * 32 + lane, row = row0 + i * kTile + in_tile;
-        const bool live = row < rows;
-        const int64_t token = p.cu_q[r] + (live ? row / group : 0);
-        const int64_t head = static_cast<int64_t>(head_kv) * group + (live ? row % group : 0);
-        int lo = 0, hi = 0;
-        if (live) attn_visible(p, seq, all, row / group, lo, hi);
-        if (i < row_tiles) {
-            float mul;
-            {  // Q: largest value of the row into [2^13, 2^14), sign of the softmax scale included
+        const int in_tile = tid % kTile;
+        uint8_t *const q_rows = smem + L::kQ + i * L::kOperand;
+        uint32_t s_phase = 0, o_phase = 0;
+        Item it;
+        while (next_item(it)) {
+            const int row = it.row0 + i * kTile + in_tile, count = it.count, first = it.first;
+            if (it.row0 + i * kTile >= it.rows) {  // a row tile that is not there: the MMAs wait for both all the same,
+                                                   // so that no warp is an item behind
+                if (count > 0 && lane == 0) mbar_arrive(&q_full[i]);
+                continue;
+            }
+            const bool live = row < it.rows;
+            const int64_t token = it.token0 + (live ? row / group : 0);
+            const int64_t head = static_cast<int64_t>(it.head_kv) * group + (live ? row % group : 0);
+            int lo = 0, hi = 0;
+            if (live) attn_visible(p, it.seq, it.all, row / group, lo, hi);
+            float mul = 0.0f;
+            if (count > 0) {  // Q: largest value of the row into [2^13, 2^14), sign of the softmax scale included
                 const int64_t at = token * p.ldq + head * DIM;
-                uint8_t *to = smem + L::kQ + i * L::kOperand;
                 if (p.q_format == kOutF32)
-                    mul = load_q<DIM, kOutF32>(mp, at, live, to, (warp & 3) * 32);
+                    mul = load_q<DIM, kOutF32>(mp, at, q_rows, (warp & 3) * 32);
                 else if (p.q_format == kOutF16)
-                    mul = load_q<DIM, kOutF16>(mp, at, live, to, (warp & 3) * 32);
+                    mul = load_q<DIM, kOutF16>(mp, at, q_rows, (warp & 3) * 32);
                 else
-                    mul = load_q<DIM, kOutBF16>(mp, at, live, to, (warp & 3) * 32);
+                    mul = load_q<DIM, kOutBF16>(mp, at, q_rows, (warp & 3) * 32);
                 fence_proxy_async_smem();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(q_full);
+                if (lane == 0) mbar_arrive(&q_full[i]);
             }
             const uint32_t s_at = tmem + static_cast<uint32_t>(i * kTile) + (static_cast<uint32_t>((warp & 3) * 32) << 16);
             const uint32_t o_at = s_at + 256;
@@ -605,7 +679,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
             bool ok = true;
             // a key with a bad V scale makes the rows that see it NaN
             const auto bad_keys = [&](int n) {
-                const TileInfo &info = infos[n % kInfoSlots];
+                const TileInfo &info = infos[(it.tile0 + n) % kInfoSlots];
                 const int key0 = (first + n) * kTile;
                 if (info.bad[0] | info.bad[1] | info.bad[2] | info.bad[3])
                     for (int c = 0; c < kTile; ++c)
@@ -613,12 +687,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
                             l = __int_as_float(0x7fffffff);
             };
             for (int n = 0; n < count; ++n) {
-                if (!wait_bar(&s_full[i], n & 1, &abort_flag, mp.err, kErrWaitFull)) {
+                if (!wait_bar(&s_full[i], s_phase, &abort_flag, mp.err, kErrWaitFull)) {
                     ok = false;
                     break;
                 }
+                s_phase ^= 1;
                 tc_fence_after();
-                const uint32_t groups = infos[n % kInfoSlots].groups;
+                const uint32_t groups = infos[(it.tile0 + n) % kInfoSlots].groups;
                 if (n > 0) bad_keys(n - 1);  // V of the last tile is complete: this tile's MMA came after its own
                 const int from = lo - (first + n) * kTile, to = hi - (first + n) * kTile;
                 const bool masked = __any_sync(0xffffffffu, from > 0 || to < kTile) || groups != 0xffu;
@@ -680,27 +755,30 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
                 l += first_of(sum[0]) + second_of(sum[0]);
             }
             if (ok && count > 0) {
-                ok = wait_bar(&o_full[i], 0, &abort_flag, mp.err, kErrWaitFull);
+                ok = wait_bar(&o_full[i], o_phase, &abort_flag, mp.err, kErrWaitFull);
+                o_phase ^= 1;
                 if (ok) bad_keys(count - 1);
             }
-            if (!ok) abort_flag = 1;
+            if (!ok) {
+                abort_flag = 1;
+                break;
+            }
             tc_fence_after();
             const bool none = m == kNoMax, have = count > 0;  // no visible key
             const float f = none ? 0.0f : 1.0f / l;
-            // this row tile's Q is read by no MMA any more
-            uint8_t *mine = smem + L::kQ + i * L::kOperand + (warp & 3) * (L::kOperand / 4);
-            if (ok && mp.splits > 1) {
-                const int64_t slot = static_cast<int64_t>(blockIdx.x) * kRows + i * kTile + in_tile;
-                write_rows<DIM, kOutF32>(mp.part_o, slot * DIM, live, true, 1.0f, o_at, have, mine);
+            // this row tile's Q is read by no MMA any more: its rows stage the output's
+            if (mp.splits > 1) {
+                const int64_t slot = static_cast<int64_t>(it.id) * kRows + i * kTile + in_tile;
+                write_rows<DIM, kOutF32>(mp.part_o, slot * DIM, live, true, 1.0f, o_at, have, q_rows, (warp & 3) * 32);
                 if (live) mp.part_ml[slot] = make_float2(m, l);
-            } else if (ok) {
+            } else {
                 const int64_t at = token * p.ldo + head * DIM;
                 if (p.out_format == kOutF32)
-                    write_rows<DIM, kOutF32>(p.out, at, live, mp.vec_out, f, o_at, have, mine);
+                    write_rows<DIM, kOutF32>(p.out, at, live, mp.vec_out, f, o_at, have, q_rows, (warp & 3) * 32);
                 else if (p.out_format == kOutF16)
-                    write_rows<DIM, kOutF16>(p.out, at, live, mp.vec_out, f, o_at, have, mine);
+                    write_rows<DIM, kOutF16>(p.out, at, live, mp.vec_out, f, o_at, have, q_rows, (warp & 3) * 32);
                 else
-                    write_rows<DIM, kOutBF16>(p.out, at, live, mp.vec_out, f, o_at, have, mine);
+                    write_rows<DIM, kOutBF16>(p.out, at, live, mp.vec_out, f, o_at, have, q_rows, (warp & 3) * 32);
                 if (live && p.lse)
                     p.lse[token * p.heads_q + head] = none ? -INFINITY : (m + log2f(l)) / kLog2e;
             }
@@ -718,7 +796,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
             constexpr uint32_t kHalf = (kTile * 128) >> 4, kBuf = L::kOperand >> 4;
             const uint64_t q_desc = sw128_desc(base + L::kQ);
             const uint64_t k_desc = sw128_desc(base + L::kKV), v_desc0 = v_desc(base + L::kKV);
-            bool ok = count > 0;
+            bool ok = true;
             const auto scores = [&](int i, uint32_t buf) {  // S_i = Q_i K^T
                 const uint64_t q = q_desc + i * kBuf, k = k_desc + buf * kBuf;
 #pragma unroll
@@ -731,99 +809,191 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
                 return __all_sync(0xffffffffu, mbar_test_wait(bar, parity) ||
                                                    wait_bar(bar, parity, &abort_flag, mp.err, kErrWaitFull)) != 0;
             };
-            if (ok) ok = ready(q_full, 0) && ready(&op_full[0], 0);
-            if (ok) {
-                tc_fence_after();
-                scores(0, 0);
-                if (row_tiles > 1) scores(1, 0);
-                umma_commit_by(leader, &op_empty[0]);
-            }
-            uint32_t vb = 1, v_phase = 0;  // buffer of V(n); K(n + 1) is in the one after it
+            uint32_t ob = 0, o_phase = 0;         // buffer of the next unit and its phase
+            uint32_t q_phase = 0, p_phases = 0;   // bit i: of row tile i
+            Item it;
+            while (ok && next_item(it)) {
+                const int count = it.count, row_tiles = it.rows - it.row0 > kTile ? 2 : 1;
+                if (count == 0) continue;
+                ok = ready(&op_full[ob], o_phase);
 #pragma unroll 1
-            for (int n = 0; n < count && ok; ++n) {
-                const uint32_t kb = vb + 1 == kOperands ? 0 : vb + 1, k_phase = vb + 1 == kOperands ? v_phase ^ 1 : v_phase;
-                const bool more = n + 1 < count;
-                const uint64_t v = v_desc0 + vb * kBuf;
-                ok = ready(&op_full[vb], v_phase);
-#pragma unroll 1
-                for (int i = 0; i < row_tiles && ok; ++i) {
-#pragma unroll
-                    for (int h = 0; h < 2 && ok; ++h) {  // O_i += P_i V, by halves of the keys
-                        ok = ready(&p_full[2 * i + h], n & 1);
-                        tc_fence_after();
-                        if (!ok) break;
-#pragma unroll
-                        for (int x = 4 * h; x < 4 * h + 4; ++x)
-                            umma_f16_ts(leader, tmem + 256 + i * kTile, tmem + i * kTile + 8 * x, v + x * (2048 >> 4), kIdescO,
-                                        n > 0 || x > 0);
-                    }
+                for (int i = 0; i < 2 && ok; ++i) {
+                    ok = ready(&q_full[i], q_phase);
                     if (!ok) break;
-                    if (i == row_tiles - 1) umma_commit_by(leader, &op_empty[vb]);
-                    if (!more) {
-                        umma_commit_by(leader, &o_full[i]);
-                        continue;
-                    }
-                    if (i == 0) ok = ready(&op_full[kb], k_phase);
-                    if (!ok) break;
-                    scores(i, kb);
-                    if (i == row_tiles - 1) umma_commit_by(leader, &op_empty[kb]);
+                    tc_fence_after();
+                    if (i < row_tiles) scores(i, ob);
+                    if (i == 1) umma_commit_by(leader, &op_empty[ob]);
                 }
-                vb = kb + 1 == kOperands ? 0 : kb + 1;
-                v_phase = kb + 1 == kOperands ? k_phase ^ 1 : k_phase;
+                q_phase ^= 1;
+                if (++ob == kOperands) ob = 0, o_phase ^= 1;
+#pragma unroll 1
+                for (int n = 0; n < count && ok; ++n) {
+                    const uint32_t vb = ob, v_phase = o_phase;
+                    if (++ob == kOperands) ob = 0, o_phase ^= 1;
+                    const bool more = n + 1 < count;
+                    const uint64_t v = v_desc0 + vb * kBuf;
+                    ok = ready(&op_full[vb], v_phase);
+#pragma unroll 1
+                    for (int i = 0; i < row_tiles && ok; ++i) {
+#pragma unroll
+                        for (int h = 0; h < 2 && ok; ++h) {  // O_i += P_i V, by halves of the keys
+                            ok = ready(&p_full[2 * i + h], ((p_phases >> i) ^ n) & 1);
+                            tc_fence_after();
+                            if (!ok) break;
+#pragma unroll
+                            for (int x = 4 * h; x < 4 * h + 4; ++x)
+                                umma_f16_ts(leader, tmem + 256 + i * kTile, tmem + i * kTile + 8 * x, v + x * (2048 >> 4),
+                                            kIdescO, n > 0 || x > 0);
+                        }
+                        if (!ok) break;
+                        if (i == row_tiles - 1) umma_commit_by(leader, &op_empty[vb]);
+                        if (!more) {
+                            umma_commit_by(leader, &o_full[i]);
+                            continue;
+                        }
+                        if (i == 0) ok = ready(&op_full[ob], o_phase);
+                        if (!ok) break;
+                        scores(i, ob);
+                        if (i == row_tiles - 1) umma_commit_by(leader, &op_empty[ob]);
+                    }
+                    if (more && ++ob == kOperands) ob = 0, o_phase ^= 1;
+                }
+                p_phases ^= count & 1 ? (row_tiles > 1 ? 3u : 1u) : 0u;
             }
-            if (!ok && count > 0) abort_flag = 1;
+            if (!ok) abort_flag = 1;
             umma_commit_by(leader, mma_done);  // TMEM is freed at the end: no MMA may be in flight
             if (!mbar_wait(mma_done, 0, mp.err, kErrWaitFull)) abort_flag = 1;
         } else if (warp == 8) {
             // ---------------- copies from the pages ----------------
             const uint64_t policy = l2_policy_evict_normal();
-            bool ok = true;
-            int j = 0;
-            // the pages of a key tile are looked up while the copies before it wait
-            int64_t at = -1, next = -1;  // this lane's group in the caches
-            int run = 0, next_run = 0;   // groups that its copy takes: those of a page go in one
-            const auto look_up = [&](int n) {
-                const int key = (first + n) * kTile + lane * kKvGroup;
-                next = -1;
-                if (n >= count || lane >= kGroups || key >= seq) return;
-                next = attn_group_at<DIM>(p, r, head_kv, key);
-                int in_page;
-                attn_page_index(p, key, in_page);
-                next_run = lane > 0 && in_page > 0
-                               ? 0 : min(min(kGroups - lane, p.page_groups - in_page), (seq - key + kKvGroup - 1) / kKvGroup);
-            };
-            look_up(0);
-            for (; j < 2 * count; ++j) {
-                const int n = j >> 1, slot = j % kRawSlots;
-                const bool is_v = j & 1;
-                if (j >= kRawSlots &&
-                    !wait_bar(&raw_empty[slot], ((j / kRawSlots) - 1) & 1, &abort_flag, mp.err, kErrWaitEmpty)) {
+            const uint32_t splits = static_cast<uint32_t>(mp.splits), heads_kv = static_cast<uint32_t>(p.heads_kv);
+            const uint32_t per_tile = static_cast<uint32_t>(p.requests) * heads_kv * splits;
+            bool ok = true, asked = false;
+            int units = 0;  // K and V tiles of the items before
+            uint32_t steal_phase = 0;
+            Item it;
+            it.id = static_cast<int>(blockIdx.x);
+            it.tile0 = 0;
+#pragma unroll 1
+            for (int k = 0; ok; ++k) {
+                // ---- the item: what the other warps need to know of it ----
+                // the last row tiles see the most keys: they come first
+                const uint32_t id = static_cast<uint32_t>(max(it.id, 0)), rest = id % per_tile;
+                const int split = static_cast<int>(rest % splits);
+                const int64_t r = rest / splits / heads_kv;
+                if (it.id >= 0) {
+                    it.head_kv = static_cast<int>(rest / splits % heads_kv);
+                    it.row0 = (mp.tiles - 1 - static_cast<int>(id / per_tile)) * kRows;
+                    it.seq = attn_seq_len(p, r);
+                    it.rows = attn_new_tokens(p, r, it.all) * group;
+                    it.token0 = p.cu_q[r];
+                    it.first = it.count = 0;
+                    if (it.row0 < it.rows) {
+                        int lo, hi, lo2, hi2;
+                        attn_visible(p, it.seq, it.all, it.row0 / group, lo, hi2);
+                        attn_visible(p, it.seq, it.all, (min(it.row0 + kRows, it.rows) - 1) / group, lo2, hi);
+                        const int first = max(lo, 0) / kTile;
+                        const int64_t all_tiles = hi > first * kTile ? (hi + kTile - 1) / kTile - first : 0;
+                        // this piece of them
+                        const int begin = static_cast<int>(all_tiles * split / mp.splits);
+                        it.first = first + begin;
+                        it.count = static_cast<int>(all_tiles * (split + 1) / mp.splits) - begin;
+                    }
+                }
+                const int slot_of_item = k % kItems;
+                if (k >= kItems && !wait_bar(&item_empty[slot_of_item], ((k / kItems) - 1) & 1, &abort_flag, mp.err, kErrWaitEmpty)) {
                     ok = false;
                     break;
                 }
-                if (!is_v) at = next, run = next_run;
-                const uint32_t there = __ballot_sync(0xffffffffu, at >= 0);
                 if (lane == 0) {
-                    if (!is_v) {
-                        TileInfo &info = infos[n % kInfoSlots];
-                        info.groups = there;
-                        info.bad[0] = info.bad[1] = info.bad[2] = info.bad[3] = 0;
-                    }
-                    mbar_arrive_expect_tx(&raw_full[slot], kv_group_bytes(DIM) * __popc(there));
+                    items[slot_of_item] = it;
+                    mbar_arrive(&item_full[slot_of_item]);
                 }
                 __syncwarp();
-                if (at >= 0 && run > 0)
-                    bulk_copy_g2s(smem + L::kRawAt + slot * L::kRaw + lane * kv_group_bytes(DIM),
-                                  (is_v ? p.v_cache : p.k_cache) + at, run * kv_group_bytes(DIM), &raw_full[slot], policy);
-                if (!is_v) look_up(n + 1);
+                if (it.id < 0) break;
+                const int count = it.count, first = it.first, seq = it.seq;
+                if (count > 0) {  // its Q into L2 while the item before is worked on
+                    const int size = p.q_format == kOutF32 ? 4 : 2;
+                    const int end = min(it.row0 + kRows, it.rows);
+#pragma unroll 1
+                    for (int row = it.row0 + lane; row < end; row += 32) {
+                        const int64_t head = static_cast<int64_t>(it.head_kv) * group + row % group;
+                        const char *q = static_cast<const char *>(p.q) + ((it.token0 + row / group) * p.ldq + head * DIM) * size;
+                        for (int x = 0; x < DIM * size; x += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(q + x));
+                    }
+                }
+                // ---- its tiles ----
+                // the pages of a key tile are looked up while the copies before it wait
+                int64_t at = -1, next = -1;  // this lane's group in the caches
+                int run = 0, next_run = 0;   // groups that its copy takes: those of a page go in one
+                const auto look_up = [&](int n) {
+                    const int key = (first + n) * kTile + lane * kKvGroup;
+                    next = -1;
+                    if (n >= count || lane >= kGroups || key >= seq) return;
+                    next = attn_group_at<DIM>(p, r, it.head_kv, key);
+                    int in_page;
+                    attn_page_index(p, key, in_page);
+                    next_run = lane > 0 && in_page > 0
+                                   ? 0 : min(min(kGroups - lane, p.page_groups - in_page), (seq - key + kKvGroup - 1) / kKvGroup);
+                };
+                look_up(0);
+                asked = false;
+                int j = 0;
+                for (; j < 2 * count; ++j) {
+                    const int n = j >> 1, unit = units + j, slot = unit % kRawSlots;
+                    const bool is_v = j & 1;
+                    if (unit >= kRawSlots &&
+                        !wait_bar(&raw_empty[slot], ((unit / kRawSlots) - 1) & 1, &abort_flag, mp.err, kErrWaitEmpty)) {
+                        ok = false;
+                        break;
+                    }
+                    if (!is_v) at = next, run = next_run;
+                    const uint32_t there = __ballot_sync(0xffffffffu, at >= 0);
+                    if (lane == 0) {
+                        if (!is_v) {
+                            TileInfo &info = infos[(it.tile0 + n) % kInfoSlots];
+                            info.groups = there;
+                            info.bad[0] = info.bad[1] = info.bad[2] = info.bad[3] = 0;
+                        }
+                        mbar_arrive_expect_tx(&raw_full[slot], kv_group_bytes(DIM) * __popc(there));
+                    }
+                    __syncwarp();
+                    if (at >= 0 && run > 0)
+                        bulk_copy_g2s(smem + L::kRawAt + slot * L::kRaw + lane * kv_group_bytes(DIM),
+                                      (is_v ? p.v_cache : p.k_cache) + at, run * kv_group_bytes(DIM), &raw_full[slot], policy);
+                    if (!is_v) look_up(n + 1);
+                    if (!asked && j + kRawSlots >= 2 * count) {  // soon done: what is next?
+                        asked = true;
+                        if (lane == 0) steal_ask(&steal_response, steal_full);
+                    }
+                }
+                units += j;
+                if (!ok) break;
+                it.tile0 += count;
+                if (count == 0) {
+                    asked = true;
+                    if (lane == 0) steal_ask(&steal_response, steal_full);
+                }
+                __syncwarp();
+                if (!wait_bar(steal_full, steal_phase, &abort_flag, mp.err, kErrWaitFull)) {
+                    ok = false;
+                    break;
+                }
+                asked = false;
+                steal_phase ^= 1;
+                it.id = stolen(&steal_response);
+                fence_proxy_async_smem();  // read before the next answer is written
+                __syncwarp();
             }
             if (!ok) abort_flag = 1;
-            // copies in flight end before the CTA does
-            if (!ok || aborted(&abort_flag))
-                for (int x = max(j - kRawSlots, 0); x < j; ++x)
+            // copies in flight, and an answer, end before the CTA does
+            if (!ok || aborted(&abort_flag)) {
+                if (asked) mbar_wait(steal_full, steal_phase, mp.err, kErrWaitFull);
+                for (int x = max(units - kRawSlots, 0); x < units; ++x)
                     mbar_wait(&raw_full[x % kRawSlots], (x / kRawSlots) & 1, mp.err, kErrWaitFull);
-        } else if (!dequantize(warp < 12 ? warp - 9 : warp - 10)) {
-            abort_flag = 1;
+            }
+        } else {
+            dequantize(warp < 12 ? warp - 9 : warp - 10);
         }
         __syncwarp();
     }
