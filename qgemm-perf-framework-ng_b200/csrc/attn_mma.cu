@@ -56,7 +56,7 @@ constexpr int kRows = 2 * kTile;
 constexpr int kThreads = 512;
 constexpr int kDequantWarps = 6;
 constexpr int kGroups = kTile / kKvGroup;  // 16-key groups of a unit: the tasks of the dequantizing warps
-constexpr int kRawSlots = 6;
+constexpr int kRawSlots = 3;  // as fast as 6, as are 4 operand tiles instead of 3
 constexpr int kOperands = 3;     // dequantized K or V tiles: unit 2 n is K of key tile n, unit 2 n + 1 its V
 constexpr int kInfoSlots = 16;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -309,15 +309,33 @@ PFNG_DEV uint4 unpack_word(uint32_t w, uint32_t scale, uint32_t magic) {
                       h2(__hmul2(__hfma2(as_h2(and_or<0x00F000F0u>(w8, magic)), sixteenth, minus72), s)));
 }
 
-// The larger of each half's magnitude of two words, a NaN aside; the larger of the two of one.
+// The larger magnitude of each half of two words (of either sign), a NaN aside.
 template <int FMT>
 PFNG_DEV uint32_t larger_magnitude(uint32_t x, uint32_t y) {
     uint32_t z;
     if constexpr (FMT == kOutBF16)
-        asm("max.bf16x2 %0, %1, %2;" : "=r"(z) : "r"(x & 0x7fff7fffu), "r"(y & 0x7fff7fffu));
+        asm("max.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(z) : "r"(x), "r"(y));
     else
-        asm("max.f16x2 %0, %1, %2;" : "=r"(z) : "r"(x & 0x7fff7fffu), "r"(y & 0x7fff7fffu));
+        asm("max.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(z) : "r"(x), "r"(y));
     return z;
+}
+// Values j and j + 2 of four, times f (a power of two and a sign), as fp16.
+template <int FMT>
+PFNG_DEV uint32_t scaled_pair(const RawValues<FMT, 4> &x, int j, float f) {
+    if constexpr (FMT == kOutBF16) {
+        float a, b;
+        const auto scaled = [&](uint32_t w) {
+            float y;
+            asm("fma.rn.f32.bf16 %0, %1, %2, %3;"
+                : "=f"(y)
+                : "h"(static_cast<uint16_t>(w >> (16 * j))), "h"(static_cast<uint16_t>(__float_as_uint(f) >> 16)), "f"(-0.0f));
+            return y;
+        };
+        a = scaled(x.w[0]), b = scaled(x.w[1]);
+        return h2(__floats2half2_rn(a, b));
+    } else {
+        return h2(__floats2half2_rn(x[j] * f, x[j + 2] * f));
+    }
 }
 
 // The 32 query rows of a warp into their rows of the Q operand: scaled by a
@@ -326,7 +344,7 @@ PFNG_DEV uint32_t larger_magnitude(uint32_t x, uint32_t y) {
 // and 16 + 4 t .. of a block of 32), so that a load covers whole sectors.  A
 // CTA runs this once, with a cold instruction cache: few instructions in a
 // rolled loop (16 rows' reductions by halving across the lanes instead of one
-// butterfly each) took the CTA's Q from 10500 to QCYC cycles.  Returns, for the
+// butterfly each) took a row tile's Q from 10500 to about 6000 cycles.  Returns, for the
 // row of this lane, the factor from accumulators to scores in log2 units.
 // row: the warp's first row; `at`: where this lane's row is (some row of q for
 // one that is not there: nothing is made of it).
@@ -374,7 +392,7 @@ PFNG_DEV float load_q(const MmaParams &mp, int64_t at, uint8_t *to, int row) {
                                                          larger_magnitude<FMT>(x[k][1].w[0], x[k][1].w[1]));
                 RawValues<FMT, 2> two;
                 two.w[0] = z;
-                top[k] = fmaxf(fmaxf(two[0], two[1]), 0.0f);
+                top[k] = fmaxf(fmaxf(fabsf(two[0]), fabsf(two[1])), 0.0f);
             }
         }
         // lane 8 i + k of a row's lanes gets the largest of row k
@@ -398,7 +416,7 @@ PFNG_DEV float load_q(const MmaParams &mp, int64_t at, uint8_t *to, int row) {
             uint32_t h[4];
             // values 0, 2 and 1, 3 of each four in a register
 #pragma unroll
-            for (int j = 0; j < 4; ++j) h[j] = h2(__floats2half2_rn(x[k][j >> 1][j & 1] * f, x[k][j >> 1][(j & 1) + 2] * f));
+            for (int j = 0; j < 4; ++j) h[j] = scaled_pair<FMT>(x[k][j >> 1], j & 1, f);
             *reinterpret_cast<uint4 *>(to + operand_at(row + first_row + step + k, sub)) = make_uint4(h[0], h[1], h[2], h[3]);
         }
     }
@@ -475,7 +493,7 @@ PFNG_DEV void write_rows(void *out, int64_t at, bool live, bool wide, float f, u
     }
 }
 
-template <int DIM>
+template <int DIM, bool STEAL>
 __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams mp) {
     using L = Layout<DIM>;
     constexpr int kBlocks = DIM / 32;
@@ -498,6 +516,37 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
     const int group = p.group;
     pdl_trigger();
 
+    // The copying warp's item; its request comes first, as CTAs are short where there are few keys.
+    Item it{};
+    int64_t r = 0;
+    const auto describe = [&]() {
+        const uint32_t splits = static_cast<uint32_t>(mp.splits), heads_kv = static_cast<uint32_t>(p.heads_kv);
+        const uint32_t per_tile = static_cast<uint32_t>(p.requests) * heads_kv * splits, id = static_cast<uint32_t>(it.id);
+        const uint32_t rest = id % per_tile, block = rest / splits, split = rest % splits;
+        r = block / heads_kv;
+        it.seq = attn_seq_len(p, r);
+        it.rows = attn_new_tokens(p, r, it.all) * group;
+        it.token0 = p.cu_q[r];
+        it.head_kv = static_cast<int>(block % heads_kv);
+        // the last row tiles see the most keys: they come first
+        it.row0 = (mp.tiles - 1 - static_cast<int>(id / per_tile)) * kRows;
+        it.first = it.count = 0;
+        if (it.row0 >= it.rows) return;
+        int lo, hi, lo2, hi2;
+        attn_visible(p, it.seq, it.all, it.row0 / group, lo, hi2);
+        attn_visible(p, it.seq, it.all, (min(it.row0 + kRows, it.rows) - 1) / group, lo2, hi);
+        const int first = max(lo, 0) / kTile;
+        const uint32_t tiles = hi > first * kTile ? (hi + kTile - 1) / kTile - first : 0;  // below 2^23; splits below 2^8
+        // this piece of them
+        const uint32_t begin = tiles * split / splits;
+        it.first = first + static_cast<int>(begin);
+        it.count = static_cast<int>(tiles * (split + 1) / splits - begin);
+    };
+    if (warp == 8) {
+        it.id = static_cast<int>(blockIdx.x);
+        it.tile0 = 0;
+        describe();
+    }
     if (tid == 0) {
         abort_flag = 0;
         for (int i = 0; i < kRawSlots; ++i) mbar_init(&raw_full[i], 1), mbar_init(&raw_empty[i], kGroups);
@@ -866,40 +915,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
         } else if (warp == 8) {
             // ---------------- copies from the pages ----------------
             const uint64_t policy = l2_policy_evict_normal();
-            const uint32_t splits = static_cast<uint32_t>(mp.splits), heads_kv = static_cast<uint32_t>(p.heads_kv);
-            const uint32_t per_tile = static_cast<uint32_t>(p.requests) * heads_kv * splits;
             bool ok = true, asked = false;
             int units = 0;  // K and V tiles of the items before
             uint32_t steal_phase = 0;
-            Item it;
-            it.id = static_cast<int>(blockIdx.x);
-            it.tile0 = 0;
 #pragma unroll 1
             for (int k = 0; ok; ++k) {
                 // ---- the item: what the other warps need to know of it ----
-                // the last row tiles see the most keys: they come first
-                const uint32_t id = static_cast<uint32_t>(max(it.id, 0)), rest = id % per_tile;
-                const int split = static_cast<int>(rest % splits);
-                const int64_t r = rest / splits / heads_kv;
-                if (it.id >= 0) {
-                    it.head_kv = static_cast<int>(rest / splits % heads_kv);
-                    it.row0 = (mp.tiles - 1 - static_cast<int>(id / per_tile)) * kRows;
-                    it.seq = attn_seq_len(p, r);
-                    it.rows = attn_new_tokens(p, r, it.all) * group;
-                    it.token0 = p.cu_q[r];
-                    it.first = it.count = 0;
-                    if (it.row0 < it.rows) {
-                        int lo, hi, lo2, hi2;
-                        attn_visible(p, it.seq, it.all, it.row0 / group, lo, hi2);
-                        attn_visible(p, it.seq, it.all, (min(it.row0 + kRows, it.rows) - 1) / group, lo2, hi);
-                        const int first = max(lo, 0) / kTile;
-                        const int64_t all_tiles = hi > first * kTile ? (hi + kTile - 1) / kTile - first : 0;
-                        // this piece of them
-                        const int begin = static_cast<int>(all_tiles * split / mp.splits);
-                        it.first = first + begin;
-                        it.count = static_cast<int>(all_tiles * (split + 1) / mp.splits) - begin;
-                    }
-                }
                 const int slot_of_item = k % kItems;
                 if (k >= kItems && !wait_bar(&item_empty[slot_of_item], ((k / kItems) - 1) & 1, &abort_flag, mp.err, kErrWaitEmpty)) {
                     ok = false;
@@ -912,7 +933,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
                 __syncwarp();
                 if (it.id < 0) break;
                 const int count = it.count, first = it.first, seq = it.seq;
-                if (count > 0) {  // its Q into L2 while the item before is worked on
+                if (k > 0 && count > 0) {  // its Q into L2 while the item before is worked on
                     const int size = p.q_format == kOutF32 ? 4 : 2;
                     const int end = min(it.row0 + kRows, it.rows);
 #pragma unroll 1
@@ -962,13 +983,17 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
                         bulk_copy_g2s(smem + L::kRawAt + slot * L::kRaw + lane * kv_group_bytes(DIM),
                                       (is_v ? p.v_cache : p.k_cache) + at, run * kv_group_bytes(DIM), &raw_full[slot], policy);
                     if (!is_v) look_up(n + 1);
-                    if (!asked && j + kRawSlots >= 2 * count) {  // soon done: what is next?
+                    if (STEAL && !asked && j + kRawSlots >= 2 * count) {  // soon done: what is next?
                         asked = true;
                         if (lane == 0) steal_ask(&steal_response, steal_full);
                     }
                 }
                 units += j;
                 if (!ok) break;
+                if constexpr (!STEAL) {
+                    it.id = -1;
+                    continue;
+                }
                 it.tile0 += count;
                 if (count == 0) {
                     asked = true;
@@ -984,6 +1009,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
                 it.id = stolen(&steal_response);
                 fence_proxy_async_smem();  // read before the next answer is written
                 __syncwarp();
+                if (it.id >= 0) describe();
             }
             if (!ok) abort_flag = 1;
             // copies in flight, and an answer, end before the CTA does
@@ -1065,13 +1091,18 @@ int splits_of(const AttnArgs &p) {
     return static_cast<int>(std::max<int64_t>(1, std::min(want, most)));
 }
 
+// Whole blocks (one piece each): the CTAs of the first wave take the others'
+// work.  Pieces are one short wave or so: each its own CTA, as taking the last
+// ones early costs balance (96 blocks of heads of 64 in 4 pieces: 62.7 us
+// against 59.4) and the join then starts later (32 blocks in 4 pieces: 69 us
+// against 66).
 template <int DIM>
 cudaError_t launch(const MmaParams &mp, cudaStream_t s) {
-    cudaError_t e = cudaFuncSetAttribute(attn_mma_kernel<DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         static_cast<int>(Layout<DIM>::kBytes));
+    const auto kernel = mp.splits == 1 ? attn_mma_kernel<DIM, true> : attn_mma_kernel<DIM, false>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Layout<DIM>::kBytes));
     if (e != cudaSuccess) return e;
     const int64_t blocks = blocks_of(mp.a);
-    attn_mma_kernel<DIM><<<static_cast<unsigned>(blocks * mp.splits), kThreads, Layout<DIM>::kBytes, s>>>(mp);
+    kernel<<<static_cast<unsigned>(blocks * mp.splits), kThreads, Layout<DIM>::kBytes, s>>>(mp);
     if ((e = cudaGetLastError()) != cudaSuccess || mp.splits == 1) return e;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(blocks * (kRows / kJoinWarps)));
