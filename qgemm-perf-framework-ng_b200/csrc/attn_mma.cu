@@ -699,9 +699,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
         Item it;
         while (next_item(it)) {
             const int row = it.row0 + i * kTile + in_tile, count = it.count, first = it.first;
-            if (it.row0 + i * kTile >= it.rows) {  // a row tile that is not there: the MMAs wait for both all the same,
-                                                   // so that no warp is an item behind
-                if (count > 0 && lane == 0) mbar_arrive(&q_full[i]);
+            if (it.row0 + i * kTile >= it.rows) {  // a row tile that is not there keeps the same order, so that its
+                                                   // warps are no item behind or ahead
+                if (count == 0) continue;
+                if (lane == 0) mbar_arrive(&q_full[i]);
+                if (!wait_bar(&o_full[i], o_phase, &abort_flag, mp.err, kErrWaitFull)) {
+                    abort_flag = 1;
+                    break;
+                }
+                o_phase ^= 1;
                 continue;
             }
             const bool live = row < it.rows;
@@ -907,6 +913,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
                     }
                     if (more && ++ob == kOperands) ob = 0, o_phase ^= 1;
                 }
+                if (ok && row_tiles == 1) umma_commit_by(leader, &o_full[1]);
                 p_phases ^= count & 1 ? (row_tiles > 1 ? 3u : 1u) : 0u;
             }
             if (!ok) abort_flag = 1;

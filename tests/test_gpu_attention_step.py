@@ -438,6 +438,23 @@ def test_attention_pieces_are_joined(dim):
         Case([2500], [70], 4, 1, dim, 16).check("f32", path=path, window=900)
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("requests,hq,hk,most_q,most_kv", [(90, 8, 4, 90, 400), (60, 8, 2, 150, 300), (400, 2, 2, 5, 60)])
+def test_attention_more_blocks_than_run_at_once(dim, requests, hq, hk, most_q, most_kv):
+    """Blocks of rows that a CTA takes one after the other: of one and two row tiles, without keys, without rows."""
+    rng = np.random.default_rng(requests + dim)
+    q_len = rng.integers(0, most_q + 1, requests)
+    seq = rng.integers(0, most_kv + 1, requests)
+    seq[::3] = np.maximum(seq[::3], q_len[::3])
+    q_len[::7] = 0
+    seq[5], q_len[5], q_len[8] = 1500, most_q, 1
+    c = Case(seq.tolist(), q_len.tolist(), hq, hk, dim, 16, "bf16", extra_rows=2)
+    c.check(path="mma")
+    c.check("f32", path="mma", window=70)
+    c.check("f16", path="mma", causal=False)
+    assert all(torch.equal(x, y) for x, y in zip(c.run(path="mma"), c.run(path="mma")))
+
+
 def test_example_runs():
     import importlib.util
     import pathlib
