@@ -53,4 +53,28 @@ PFNG_DEV int64_t attn_group_at(const AttnArgs &p, int64_t r, int head_kv, int j)
     return page * p.page_bytes + (static_cast<int64_t>(head_kv) * p.page_groups + group) * kv_group_bytes(DIM);
 }
 
+// Two fp32 values in a register pair, and arithmetic on both in one instruction.
+PFNG_DEV uint64_t pair(float x, float y) {
+    uint64_t p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(x), "f"(y));
+    return p;
+}
+PFNG_DEV float first_of(uint64_t p) { return __uint_as_float(static_cast<uint32_t>(p)); }
+PFNG_DEV float second_of(uint64_t p) { return __uint_as_float(static_cast<uint32_t>(p >> 32)); }
+PFNG_DEV uint64_t fma2(uint64_t x, uint64_t y, uint64_t z) {
+    uint64_t p;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(p) : "l"(x), "l"(y), "l"(z));
+    return p;
+}
+PFNG_DEV uint64_t add2(uint64_t x, uint64_t y) {
+    uint64_t p;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(p) : "l"(x), "l"(y));
+    return p;
+}
+PFNG_DEV uint64_t mul2(uint64_t x, uint64_t y) {
+    uint64_t p;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(p) : "l"(x), "l"(y));
+    return p;
+}
+
 }  // namespace pfng

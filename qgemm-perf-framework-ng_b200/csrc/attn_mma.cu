@@ -220,24 +220,6 @@ PFNG_DEV float exp2_approx(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// Two fp32 values in a register pair, and arithmetic on both.
-PFNG_DEV uint64_t pair(float x, float y) {
-    uint64_t p;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(x), "f"(y));
-    return p;
-}
-PFNG_DEV float first_of(uint64_t p) { return __uint_as_float(static_cast<uint32_t>(p)); }
-PFNG_DEV float second_of(uint64_t p) { return __uint_as_float(static_cast<uint32_t>(p >> 32)); }
-PFNG_DEV uint64_t fma2(uint64_t x, uint64_t y, uint64_t z) {
-    uint64_t p;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(p) : "l"(x), "l"(y), "l"(z));
-    return p;
-}
-PFNG_DEV uint64_t add2(uint64_t x, uint64_t y) {
-    uint64_t p;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(p) : "l"(x), "l"(y));
-    return p;
-}
 PFNG_DEV uint32_t h2(__half2 x) { return *reinterpret_cast<uint32_t *>(&x); }
 PFNG_DEV __half2 as_h2(uint32_t x) { return *reinterpret_cast<__half2 *>(&x); }
 template <uint32_t MASK>

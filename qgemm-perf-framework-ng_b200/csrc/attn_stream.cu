@@ -515,6 +515,7 @@ PFNG_DEV void attend(const RowTile<DIM, NT> &t, const WarpState<DIM, NT> &w, Row
             }
 #pragma unroll
         for (int j = 0; j < kGroups; ++j) {
+            uint64_t top2[NT], bottom2[NT];  // scores of key ka, of key kb: pairs of query rows
             uint32_t wa[kBlocks], wb[kBlocks], da[kBlocks / 2], db[kBlocks / 2];
             const uint32_t kw = kg + ka * kRow + q4 * 4 * kBlocks + j * kGroup;
             const uint32_t ks = kg + ka * kScaleRow + kScales + j * kGroup;
@@ -530,7 +531,7 @@ PFNG_DEV void attend(const RowTile<DIM, NT> &t, const WarpState<DIM, NT> &w, Row
                 da[0] = lds32(ks), db[0] = lds32(ks + 8 * kScaleRow);
             }
 #pragma unroll
-            for (int n = 0; n < NT; ++n) sc[j][n][0] = sc[j][n][1] = sc[j][n][2] = sc[j][n][3] = 0.0f;
+            for (int n = 0; n < NT; ++n) top2[n] = bottom2[n] = 0;
 #pragma unroll
             for (int b = 0; b < kBlocks; ++b) {
                 const uint32_t a8 = wa[b] >> 8, b8 = wb[b] >> 8;
@@ -543,11 +544,17 @@ PFNG_DEV void attend(const RowTile<DIM, NT> &t, const WarpState<DIM, NT> &w, Row
                             t.q[n][b][1]);
                     mma_f16(c, wa[b] & 0x00F000F0u, wb[b] & 0x00F000F0u, a8 & 0x00F000F0u, b8 & 0x00F000F0u, t.q[n][b][2],
                             t.q[n][b][3]);
-                    sc[j][n][0] = fmaf(fa, c[0] + start[n][b][0], sc[j][n][0]);
-                    sc[j][n][1] = fmaf(fa, c[1] + start[n][b][1], sc[j][n][1]);
-                    sc[j][n][2] = fmaf(fb, c[2] + start[n][b][0], sc[j][n][2]);
-                    sc[j][n][3] = fmaf(fb, c[3] + start[n][b][1], sc[j][n][3]);
+                    const uint64_t st = pair(start[n][b][0], start[n][b][1]);
+                    top2[n] = fma2(pair(fa, fa), add2(pair(c[0], c[1]), st), top2[n]);
+                    bottom2[n] = fma2(pair(fb, fb), add2(pair(c[2], c[3]), st), bottom2[n]);
                 }
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const uint64_t m2 = pair(t.mul[n][0], t.mul[n][1]);
+                top2[n] = mul2(top2[n], m2), bottom2[n] = mul2(bottom2[n], m2);
+                sc[j][n][0] = first_of(top2[n]), sc[j][n][1] = second_of(top2[n]);
+                sc[j][n][2] = first_of(bottom2[n]), sc[j][n][3] = second_of(bottom2[n]);
             }
         }
     }
@@ -557,7 +564,6 @@ PFNG_DEV void attend(const RowTile<DIM, NT> &t, const WarpState<DIM, NT> &w, Row
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                sc[j][n][i] *= t.mul[n][i & 1];
                 if constexpr (MASKED) {
                     const int key = key0 + j * kKvGroup + (i < 2 ? ka : kb), row = n * 8 + 2 * q4 + (i & 1);
                     if (!(key >= w.lo[row] && key < w.hi[row])) sc[j][n][i] = -INFINITY;
@@ -661,9 +667,12 @@ PFNG_DEV void attend(const RowTile<DIM, NT> &t, const WarpState<DIM, NT> &w, Row
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) pr[n][i] = exp2_approx(sc[j][n][i] - s.m[n][i & 1]);
-            s.l[n][0] += pr[n][0] + pr[n][2];
-            s.l[n][1] += pr[n][1] + pr[n][3];
+            for (int i = 0; i < 4; i += 2) {
+                const uint64_t e = add2(pair(sc[j][n][i], sc[j][n][i + 1]), pair(-s.m[n][0], -s.m[n][1]));
+                pr[n][i] = exp2_approx(first_of(e)), pr[n][i + 1] = exp2_approx(second_of(e));
+            }
+            const uint64_t l2 = add2(pair(s.l[n][0], s.l[n][1]), add2(pair(pr[n][0], pr[n][1]), pair(pr[n][2], pr[n][3])));
+            s.l[n][0] = first_of(l2), s.l[n][1] = second_of(l2);
             rows_to_columns(pr[n][0], pr[n][1]);
             rows_to_columns(pr[n][2], pr[n][3]);
         }
@@ -696,8 +705,12 @@ PFNG_DEV void attend(const RowTile<DIM, NT> &t, const WarpState<DIM, NT> &w, Row
             for (int n = 0; n < NT; ++n) {
                 float dp[4];
 #pragma unroll
+                for (int i = 0; i < 4; i += 2) {
+                    const uint64_t x2 = mul2(pair(pr[n][i], pr[n][i + 1]), pair(d[i], d[i + 1]));
+                    dp[i] = first_of(x2), dp[i + 1] = second_of(x2);
+                }
+#pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    dp[i] = pr[n][i] * d[i];
                     // 0 times an infinite scale is 0 where the row does not see the key
                     if constexpr (MASKED) dp[i] = pr[n][i] == 0.0f ? 0.0f : dp[i];
                 }
