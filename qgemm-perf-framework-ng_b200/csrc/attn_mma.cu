@@ -11,27 +11,38 @@
 // other's softmax runs.  Roles (512 threads, one CTA per SM):
 //   warps 0-7    softmax, a warpgroup per row tile; they load Q, rescale O
 //                and write the output
-//   warp 8       copies the tiles' groups from the pages (bulk copies, a ring
-//                of six raw K or V tiles)
+//   warp 8       finds the work (items), copies the tiles' groups from the
+//                pages (bulk copies, a ring of three raw K or V tiles)
 //   warp 12      issues the MMAs
 //   warps 9-11, 13-15  dequantization: nibbles and scales of a tile -> fp16
 //                operand rows in the 128-byte swizzled layout; none of them on
 //                the scheduler that the MMA warp shares with softmax warps
-// One dequantization serves 256 rows: 13 instructions per 8 values.  Where there
-// are few blocks of rows the keys of each are cut into pieces (splits_of) that a
-// second kernel joins.
+// One dequantization serves 256 rows: 13 instructions per 8 values.
+//
+// An item is a block of 256 rows with its keys.  A CTA that comes to the end of
+// its own takes over the item of a CTA that has not started (cluster launch
+// control), so that copies, dequantization and Q (into L2) run ahead into the
+// next item while the softmax finishes this one, and barriers and TMEM are set
+// up once; the blocks with the most keys come first.  Where there are few
+// blocks of rows the keys of each are cut into pieces (splits_of) that a second
+// kernel joins.
 //
 // Measured (32 query and 8 key heads of 128, causal): a prompt of 8192 tokens
-// 598 us = 920 TFLOP/s of visible work, 0.56 of the measured bf16 rate; five
-// chunks of 300..1400 tokens over up to 7000 keys, window 4096, 399 us = 717.
-// A 256 x 128 step takes about 4000 cycles against 2048 of MMA, 2048 of
+// 548 us = 1004 TFLOP/s of visible work, 0.61 of the measured bf16 rate; five
+// chunks of 300..1400 tokens over up to 7000 keys, window 4096, 369 us = 775.
+// A 256 x 128 step takes about 3830 cycles against 2048 of MMA, 2048 of
 // exponentials (16 per cycle and SM) and 2300 of shared memory (operands read
-// by the MMAs, tiles written): per row tile the softmax (about 2700 cycles from
-// S to P) and the MMAs (1200) follow each other, and with two row tiles in
-// turn they overlap only in part.  TMEM is full, so a third row tile does not
-// fit.  S in two 64-key buffers per row tile (MMAs ahead of the softmax; more
-// operand reads) was slower, 645 us; rolled softmax loops of 64 columns 785.
-// Loading Q and storing O take about 20000 cycles of a CTA.
+// by the MMAs, tiles written).  No part bounds it alone: without the
+// exponentials the prompt takes 3 % less, without the unpacking of nibbles 6 %,
+// without both 12 %, and with an eighth of the MMAs 2 % (569 us as a whole
+// then); softmax warps wait half of a step for S, the MMA warp as long for P
+// and K.  TMEM is full, so a third row tile does not fit.  S in two 64-key
+// buffers per row tile (MMAs ahead of the softmax; more operand reads) was
+// slower, 10 %; rolled softmax loops of 64 columns 30 %; a quarter of the
+// exponentials as polynomials on the FMA pipe 7 %; a task's words read while
+// the one before is unpacked 2 %.  Between two items about 16000 cycles of a
+// row tile's warps pass: Q 6000, the first S 1300, the last O 1200, the output
+// 5600.
 //
 // Precision: d (n - 8) is rounded to fp16 (2^-12 on average), P to fp16 with
 // the row's largest at 2^8..2^15 (so that small ones stay normal numbers);
@@ -323,11 +334,12 @@ PFNG_DEV uint32_t scaled_pair(const RawValues<FMT, 4> &x, int j, float f) {
 // The 32 query rows of a warp into their rows of the Q operand: scaled by a
 // power of two each (and the sign of the softmax scale), in the order of K's
 // words.  DIM / 8 lanes read a row, a chunk of the operand each (values 4 t ..
-// and 16 + 4 t .. of a block of 32), so that a load covers whole sectors.  A
-// CTA runs this once, with a cold instruction cache: few instructions in a
-// rolled loop (16 rows' reductions by halving across the lanes instead of one
-// butterfly each) took a row tile's Q from 10500 to about 6000 cycles.  Returns, for the
-// row of this lane, the factor from accumulators to scores in log2 units.
+// and 16 + 4 t .. of a block of 32), so that a load covers whole sectors.  One
+// warp per scheduler works on it, so that it is bound by its instructions one
+// after the other: 8 rows' largest values by halving across the lanes instead
+// of a butterfly each, and no exchange of chunks, took a row tile's Q from 10500
+// to 6000 cycles.  Returns, for the row of this lane, the factor from
+// accumulators to scores in log2 units.
 // row: the warp's first row; `at`: where this lane's row is (some row of q for
 // one that is not there: nothing is made of it).
 template <int DIM, int FMT>
@@ -770,7 +782,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
                     }
                 }
                 // Packed pairs: the step is bound by instruction issue, and a packed FMA or add is one instruction for
-                // two values (a quarter of the exponentials on the FMA pipe instead cost 7 %).
+                // two values (585 us against 598 with one value each).
                 const uint64_t mul2 = pair(mul, mul), minus_m = pair(-m, -m);
                 uint64_t sum[2] = {0, 0};
 #pragma unroll

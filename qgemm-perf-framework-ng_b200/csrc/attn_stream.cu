@@ -16,9 +16,9 @@
 // the loop synchronises with another warp.
 //
 // Measured (32 query and 8 key heads of 128, one token a request): 8 requests
-// of 60000..100000 keys, 680 MB: 154 us, 4.4 TB/s, 0.67 of the measured 6.54;
-// 48 requests of 64..8000 keys, 214 MB: 69 us, 3.1 TB/s.  What bounds the
-// first is instruction issue: 336 instructions per 16 keys and warp at 0.62 a
+// of 60000..100000 keys, 680 MB: 148 us, 4.6 TB/s, 0.70 of the measured 6.54;
+// 48 requests of 64..8000 keys, 214 MB: 67 us, 3.2 TB/s.  What bounds the
+// first is instruction issue: 306 instructions per 16 keys and warp at 0.6 a
 // cycle, the ALU pipe half busy with nibbles (see attend); the second adds the
 // start (launch, lengths, first copies) and the joining kernel, about 15 us.
 //
@@ -492,7 +492,9 @@ PFNG_DEV int key_of_row(int r) { return (r & 8) | ((r & 7) >> 1) | ((r & 1) << 2
 // keys.  magic: 0x64006400, 1024 in both halves.
 // All scores first, then one look at maximum and scales, then all of O: a few
 // long runs of independent instructions, which the pipes (ALU for the nibbles,
-// FMA, tensor cores, shuffles) overlap.
+// FMA, tensor cores, shuffles) overlap.  Arithmetic on the two query rows of a
+// thread is packed in pairs (148 us against 155 for 8 requests of up to 100000
+// keys).
 template <int DIM, int NT, int kGroups, bool MASKED>
 PFNG_DEV void attend(const RowTile<DIM, NT> &t, const WarpState<DIM, NT> &w, RowSums<DIM, NT> &s, uint32_t kg,
                      uint32_t vg, int key0, uint32_t magic) {

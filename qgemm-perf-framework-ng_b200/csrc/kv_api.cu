@@ -39,8 +39,8 @@ int resolve_attention(const AttnArgs &a, int path) {
         // kernel.  Up to 32 (two tiles, each reading the cache) it still wins
         // unless there are so few (request, key head) pairs that the MMA
         // kernel can cut the keys of each into four pieces and more: 32 rows,
-        // 8 x 8 pairs, 16000 keys 131 us against 200; 1 x 8 pairs, 8000 keys
-        // 51 against 33.  With 64 rows the MMA kernel wins (232 against 200).
+        // 8 x 8 pairs, 16000 keys 127 us against 203; 1 x 8 pairs, 8000 keys
+        // 50 against 34.  With 64 rows the MMA kernel wins (223 against 202).
         const int64_t rows = a.max_q * a.group, pairs = a.requests * a.heads_kv;
         const bool few = rows <= 16 || (rows <= 32 && 4 * pairs > device_sm_count());
         if (few && stream) return PFNG_B200_PATH_GEMV;
