@@ -23,13 +23,15 @@
 // its own takes over the item of a CTA that has not started (cluster launch
 // control), so that copies, dequantization and Q (into L2) run ahead into the
 // next item while the softmax finishes this one, and barriers and TMEM are set
-// up once; the blocks with the most keys come first.  Where there are few
-// blocks of rows the keys of each are cut into pieces (splits_of) that a second
+// up once.  Blocks without rows are no items (BlockLine): the grid is bounded by
+// the tokens, not by the longest request (five ragged chunks: 331 us against
+// 369).  Where there are few blocks of rows the keys of each are cut into pieces (splits_of) that a second
 // kernel joins.
 //
 // Measured (32 query and 8 key heads of 128, causal): a prompt of 8192 tokens
 // 548 us = 1004 TFLOP/s of visible work, 0.61 of the measured bf16 rate; five
-// chunks of 300..1400 tokens over up to 7000 keys, window 4096, 369 us = 775.
+// chunks of 300..1400 tokens over up to 7000 keys, window 4096, 331 us = 862;
+// 255 requests of one token and one of 2000, 500 keys, 301 us.
 // A 256 x 128 step takes about 3830 cycles against 2048 of MMA, 2048 of
 // exponentials (16 per cycle and SM) and 2300 of shared memory (operands read
 // by the MMAs, tiles written).  No part bounds it alone: without the
@@ -110,7 +112,6 @@ struct Layout {
 struct MmaParams {
     AttnArgs a;
     int vec_q, vec_out;  // rows allow 16-byte accesses
-    int tiles;           // blocks of kRows per request and key head in the grid
     int splits;          // pieces that the keys of a block are cut into
     float *part_o;       // splits > 1: [block][split][kRows][dim] unnormalised outputs
     float2 *part_ml;     // and [block][split][kRows] reference (log2) and sum
@@ -487,6 +488,49 @@ PFNG_DEV void write_rows(void *out, int64_t at, bool live, bool wide, float f, u
     }
 }
 
+// Blocks of rows in a line: those of request 0 (the last, which sees the most
+// keys, first), then of request 1, and so on.  A warp looks for block k in 32
+// requests at a time; it keeps its place, as it mostly asks for larger ones.
+struct BlockLine {
+    int64_t chunk = 0;  // requests chunk .. chunk + 31
+    int64_t before = 0; // blocks of the requests before them
+    // Block k: its request, tile and what the request says, all read at once;
+    // false past the last block.  By a whole warp.
+    PFNG_DEV bool find(const AttnArgs &p, int64_t k, int64_t &r, Item &it) {
+        const int lane = threadIdx.x & 31;
+        if (k < before) chunk = before = 0;
+        for (; chunk < p.requests; chunk += 32) {
+            int all = 0, seq = 0, rows = 0;
+            int64_t token0 = 0;
+            if (chunk + lane < p.requests) {
+                seq = attn_seq_len(p, chunk + lane);
+                token0 = p.cu_q[chunk + lane];
+                rows = attn_new_tokens(p, chunk + lane, all) * static_cast<int>(p.group);
+            }
+            int sum = (rows + kRows - 1) / kRows;  // blocks of lanes 0 .. lane
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int other = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) sum += other;
+            }
+            const int total = __shfl_sync(0xffffffffu, sum, 31);
+            if (k < before + total) {
+                const int at = static_cast<int>(k - before);
+                const int owner = __ffs(static_cast<int>(__ballot_sync(0xffffffffu, at < sum))) - 1;
+                r = chunk + owner;
+                it.row0 = (__shfl_sync(0xffffffffu, sum, owner) - 1 - at) * kRows;
+                it.rows = __shfl_sync(0xffffffffu, rows, owner);
+                it.all = __shfl_sync(0xffffffffu, all, owner);
+                it.seq = __shfl_sync(0xffffffffu, seq, owner);
+                it.token0 = __shfl_sync(0xffffffffu, token0, owner);
+                return true;
+            }
+            before += total;
+        }
+        return false;
+    }
+};
+
 template <int DIM, bool STEAL>
 __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams mp) {
     using L = Layout<DIM>;
@@ -510,22 +554,16 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const MmaParams m
     const int group = p.group;
     pdl_trigger();
 
-    // The copying warp's item; its request comes first, as CTAs are short where there are few keys.
+    // The copying warp's item; it is looked for first, as CTAs are short where there are few keys.
     Item it{};
     int64_t r = 0;
+    BlockLine line;
     const auto describe = [&]() {
         const uint32_t splits = static_cast<uint32_t>(mp.splits), heads_kv = static_cast<uint32_t>(p.heads_kv);
-        const uint32_t per_tile = static_cast<uint32_t>(p.requests) * heads_kv * splits, id = static_cast<uint32_t>(it.id);
-        const uint32_t rest = id % per_tile, block = rest / splits, split = rest % splits;
-        r = block / heads_kv;
-        it.seq = attn_seq_len(p, r);
-        it.rows = attn_new_tokens(p, r, it.all) * group;
-        it.token0 = p.cu_q[r];
-        it.head_kv = static_cast<int>(block % heads_kv);
-        // the last row tiles see the most keys: they come first
-        it.row0 = (mp.tiles - 1 - static_cast<int>(id / per_tile)) * kRows;
-        it.first = it.count = 0;
-        if (it.row0 >= it.rows) return;
+        const uint32_t id = static_cast<uint32_t>(it.id), split = id % splits;
+        it.rows = it.row0 = it.first = it.count = 0;
+        if (!line.find(p, id / splits / heads_kv, r, it)) return;
+        it.head_kv = static_cast<int>(id / splits % heads_kv);
         int lo, hi, lo2, hi2;
         attn_visible(p, it.seq, it.all, it.row0 / group, lo, hi2);
         attn_visible(p, it.seq, it.all, (min(it.row0 + kRows, it.rows) - 1) / group, lo2, hi);
@@ -1040,16 +1078,16 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attn_mma_join_kernel(const Mm
     const AttnArgs &p = mp.a;
     const int lane = threadIdx.x & 31;
     const int64_t at = static_cast<int64_t>(blockIdx.x) * kJoinWarps + (threadIdx.x >> 5);
-    const int64_t block = at / kRows;  // (tile, request, key head), as in the grid
+    const int64_t block = at / kRows;  // (block of the line, key head), as in the grid
     const int in_block = static_cast<int>(at % kRows);
-    const int64_t per_tile = p.requests * p.heads_kv;
-    const int tile = mp.tiles - 1 - static_cast<int>(block / per_tile);
-    const int64_t r = block % per_tile / p.heads_kv;
     const int head_kv = static_cast<int>(block % p.heads_kv);
-    int all;
-    const int rows = attn_new_tokens(p, r, all) * p.group, row = tile * kRows + in_block;
+    int64_t r = 0;
+    Item it{};
+    BlockLine line;
+    const bool there = line.find(p, block / p.heads_kv, r, it);
+    const int row = it.row0 + in_block;
     pdl_wait();
-    if (tile < 0 || row >= rows) return;
+    if (!there || row >= it.rows) return;
     const int64_t slot0 = block * mp.splits * kRows + in_block;
     float m = kNoMax;
     for (int s = lane; s < mp.splits; s += 32) m = fmaxf(m, mp.part_ml[slot0 + static_cast<int64_t>(s) * kRows].x);
@@ -1067,7 +1105,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attn_mma_join_kernel(const Mm
     }
     const bool none = m == kNoMax;
     const float f = none ? 0.0f : 1.0f / l;
-    const int64_t token = p.cu_q[r] + row / p.group, head = static_cast<int64_t>(head_kv) * p.group + row % p.group;
+    const int64_t token = it.token0 + row / p.group, head = static_cast<int64_t>(head_kv) * p.group + row % p.group;
 #pragma unroll
     for (int x = 0; x < DIM / 32; ++x) {
         const float v[1] = {acc[x] * f};
@@ -1076,25 +1114,31 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attn_mma_join_kernel(const Mm
     if (p.lse && lane == 0) p.lse[token * p.heads_q + head] = none ? -INFINITY : (m + log2f(l)) / kLog2e;
 }
 
-int64_t row_blocks(const AttnArgs &p) { return (p.max_q * p.group + kRows - 1) / kRows; }
-int64_t blocks_of(const AttnArgs &p) { return row_blocks(p) * p.requests * p.heads_kv; }
+// Blocks of rows at most: of requests of max_q tokens, or of all tokens with a
+// block begun per request, whichever is less (256 requests, one of 2000 tokens
+// and the others of one, would otherwise be 65536 CTAs with work for 2296).
+int64_t blocks_of(const AttnArgs &p) {
+    const int64_t each = (p.max_q * p.group + kRows - 1) / kRows;
+    return std::min(each * p.requests, p.tokens * p.group / kRows + p.requests) * p.heads_kv;
+}
 // Pieces per block of rows, none shorter than kMinTiles key tiles.  Few blocks:
-// as many pieces as make one wave of CTAs (10 blocks over 16000 keys: 55 us with
+// as many pieces as make one wave of CTAs (10 blocks over 16000 keys: 53 us with
 // 14 pieces, 74 with 29, a second wave that is not full).  Where no two pieces
-// per block fit one wave, three waves even out ragged lengths (96 blocks over
-// 1000..4000 keys: 86 us with 1 piece, 65 with 3, 60 with 4); from three waves
-// of blocks on there is nothing to cut.
+// per block fit one wave, two waves even out ragged lengths (80 blocks, 56 with
+// rows, over 1000..4000 keys: 58 us with 3 pieces, 67 with 5).  With more
+// blocks than SMs two pieces fill three waves better than one fills two; from
+// three waves of blocks on there is nothing to cut.
 constexpr int kMinTiles = 4;
 int splits_of(const AttnArgs &p) {
     const int64_t sms = device_sm_count(), blocks = blocks_of(p);
-    const int64_t want = sms / blocks >= 2 ? sms / blocks : 3 * sms / blocks;
+    const int64_t want = sms / blocks >= 2 ? sms / blocks : (blocks <= sms ? 2 : 3) * sms / blocks;
     const int64_t most = (p.max_kv + kTile - 1) / kTile / kMinTiles;
     return static_cast<int>(std::max<int64_t>(1, std::min(want, most)));
 }
 
 // Whole blocks (one piece each): the CTAs of the first wave take the others'
 // work.  Pieces are one short wave or so: each its own CTA, as taking the last
-// ones early costs balance (96 blocks of heads of 64 in 4 pieces: 62.7 us
+// ones early costs balance (56 blocks of heads of 64 in 4 pieces: 62.7 us
 // against 59.4) and the join then starts later (32 blocks in 4 pieces: 69 us
 // against 66).
 template <int DIM>
@@ -1137,7 +1181,6 @@ cudaError_t launch_attn_mma(const AttnArgs &p, void *workspace, int *err, cudaSt
     };
     mp.vec_q = wide(p.q, p.ldq, p.q_format);
     mp.vec_out = wide(p.out, p.ldo, p.out_format);
-    mp.tiles = static_cast<int>(row_blocks(p));
     mp.splits = splits_of(p);
     mp.part_o = static_cast<float *>(workspace);
     mp.part_ml = reinterpret_cast<float2 *>(mp.part_o + blocks_of(p) * mp.splits * kRows * p.head_dim);
